@@ -358,8 +358,10 @@ def _own(s, c):
                 inverse=c["inverse"])
         return [out] if out2 is None else [out, out2]
     if c["op"] == "adamw":
-        nn.adamw(s["p"], s["g"], s["m"], s["v"], s["t"], LR, B1, B2, EPS, DECAY, masters=s["w"], m_scales=s.get("ms"),
-                 v_scales=s.get("vs"))
+        if "opt" not in s:
+            s["opt"] = nn.AdamW(s["p"], s["g"], s["m"], s["v"], s["t"], LR, B1, B2, EPS, DECAY, masters=s["w"],
+                                m_scales=s.get("ms"), v_scales=s.get("vs"))
+        s["opt"].step()
         return _adamw_outputs(s)
     q, k, v, train = s["q"], s["k"], s["v"], c["op"] == "diff_train"
     if "ws" not in s:
