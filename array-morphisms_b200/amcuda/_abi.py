@@ -16,6 +16,8 @@ AMC_OK = 0
 ERR_NAMES = {1: "INVALID", 2: "UNSUPPORTED", 3: "CUDA", 4: "OOM", 5: "STATE", 6: "INJECTED", 7: "TIMEOUT"}
 
 F32, F64, S32, S64, U32, U64 = 0, 1, 2, 3, 4, 5
+# 16-bit storage types and 8-bit optimizer states of the layer entry points
+BF16, F16, E4M3 = 16, 17, 18
 MAX_RANK = 8
 
 OP = dict(LOAD=1, CONST=2, ICONST=3, CVT=4, NEG=10, ABS=11, FLOOR=12, CEIL=13, SQRT=14, EXP=15, LOG=16, SIN=17,
@@ -50,6 +52,25 @@ class Node(C.Structure):
                 ("shape", C.c_int64 * MAX_RANK), ("in_", C.c_int32 * NODE_MAX_IN), ("in_ext", C.POINTER(C.c_int32)),
                 ("iparam", C.c_int64 * 24), ("fparam", C.c_double * 4), ("prog", C.POINTER(Insn)),
                 ("prog_len", C.c_int32), ("_pad", C.c_int32), ("leaf", View)]
+
+
+class RopeTensor(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("heads", C.c_int64), ("xs", C.c_int64 * 3),
+                ("os", C.c_int64 * 3)]
+
+
+class DiffAttention(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "causal", "batch", "heads", "kv_heads", "nq", "nk", "d", "dv",
+                                          "lam_rows")]
+                + [("scale", C.c_float), ("lam_init", C.c_float)]
+                + [(n, C.c_void_p) for n in ("q", "k", "v", "lam", "q_lens", "kv_lens", "o", "o2", "lse", "d_o", "dq",
+                                             "dk", "dv_", "dlam", "workspace")]
+                + [("workspace_bytes", C.c_int64)]
+                + [(n, C.c_int64 * 3) for n in ("qs", "ks", "vs", "os", "o2s", "dos", "dqs", "dks", "dvs")])
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("p", "g", "m", "v", "master", "m_scale", "v_scale")] + [("n", C.c_int64)]
 
 
 _P = C.c_void_p
@@ -122,6 +143,12 @@ SIGNATURES = {
     "amc_peer_group_destroy": [_U64],
     "amc_probe_bounded_wait": [_I32, _I32, _P],
     "amc_colfold_launch_count": [_P],
+    "amc_rope": [_P, _I32, _I32, _I64, _I64, _I32, _I32, _P, _I64, _P, _F, _I32, _I32, _P],
+    "amc_rope_freqs": [_PD, _I32, _D, _I32, _D, _I64, _D, _D, _PF],
+    "amc_diff_attention_fwd": [_P, _P],
+    "amc_diff_attention_bwd": [_P, _P],
+    "amc_diff_attention_workspace": [_P, _I32, _PI64],
+    "amc_adamw": [_P, _I32, _I32, _I32, _I32, _P, _P, _D, _D, _D, _D, _D, _P],
 }
 
 _lib = None

@@ -1,0 +1,561 @@
+// Differential attention, entry points and the kernels of every case:
+//   P_m = softmax(scale Q_m K_m^T), m = 1, 2;  O = (P_1 - lam P_2) V
+// with lam = exp(l0.l1) - exp(l2.l3) + lam_init per head.
+// Backward, from the rows' log-sum-exps and D_m = rowsum(dO * O_m), G = dO V^T:
+//   dS_1 = P_1 (G - D_1)          dS_2 = -lam P_2 (G - D_2)
+//   dQ_m = scale dS_m K_m         dK_m = scale dS_m^T Q_m
+//   dV   = (P_1 - lam P_2)^T dO   dlam = -sum over rows of D_2
+// dlam is summed from P_2 G of the rebuilt map, in f32 before any rounding to
+// 16 bits, not from the stored O_2.
+//
+// These kernels keep everything in f32 on the FMA pipes: a CTA of 16 x 16
+// threads owns TT rows (or keys), streams TT-wide tiles of the other side
+// through shared memory, and each thread owns a (TT/16)^2 patch of a score
+// tile and TT/16 rows x DV/16 columns of an output.  They run f32 tensors,
+// where a tensor core would round the operands, and the shapes the
+// tensor-core kernels do not take.
+#include <cmath>
+
+#include "amc_diffattn.h"
+#include "amc_half.cuh"
+
+namespace amc {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// lam of head h, on every lane; each warp calls it converged.
+template <typename T>
+__device__ __forceinline__ float2 lam_exps(const amc_diff_attention& p, int row) {
+  const T* l = (const T*)p.lam + (size_t)row * 4 * p.d;
+  float a = 0.f, c = 0.f;
+  for (int i = threadIdx.x & 31; i < p.d; i += 32) {
+    a = fmaf(to_f32(l[i]), to_f32(l[p.d + i]), a);
+    c = fmaf(to_f32(l[2 * p.d + i]), to_f32(l[3 * p.d + i]), c);
+  }
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    c += __shfl_xor_sync(0xffffffffu, c, o);
+  }
+  return make_float2(expf(a), expf(c));
+}
+template <typename T>
+__device__ __forceinline__ float lam_of(const amc_diff_attention& p, int h) {
+  const float2 e = lam_exps<T>(p, p.lam_rows == 1 ? 0 : h);
+  return e.x - e.y + p.lam_init;
+}
+
+// rows r0 .. r0+TT of a (rows, dim) matrix into dst[TT][W], zero outside
+// rows < rows_end and columns < dim.
+template <typename T, int TT, int W, int PITCH>
+__device__ __forceinline__ void load_tile(float* dst, const T* src, int64_t stride, int r0, int rows_end, int dim) {
+  for (int i = threadIdx.x; i < TT * W; i += 256) {
+    const int r = i / W, c = i % W;
+    dst[r * PITCH + c] = (r0 + r < rows_end && c < dim) ? to_f32(src[(int64_t)(r0 + r) * stride + c]) : 0.f;
+  }
+}
+
+// acc[i][j] += sum_c A[ty + 16 i][c] B[tx + 16 j][c]
+template <int R, int PITCH>
+__device__ __forceinline__ void dot_rows(float (&acc)[R][R], const float* A, const float* B, int dim, int ty, int tx) {
+  for (int c = 0; c < dim; c += 4) {
+    float4 a[R], b[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) a[i] = *reinterpret_cast<const float4*>(A + (ty + 16 * i) * PITCH + c);
+#pragma unroll
+    for (int j = 0; j < R; ++j) b[j] = *reinterpret_cast<const float4*>(B + (tx + 16 * j) * PITCH + c);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+        acc[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, acc[i][j]))));
+  }
+}
+
+// out[i][4 g + e] += sum_k W(ty + 16 i, k) X[k][4 tx + 64 g + e]; W is
+// w[row * PW + k], or transposed w[k * PW + row].
+template <int R, int NC, int TT, int PW, int PX, bool TRANS>
+__device__ __forceinline__ void mul_rows(float (&out)[R][NC], const float* w, const float* X, int ty, int tx) {
+#pragma unroll 4
+  for (int k = 0; k < TT; ++k) {
+    float a[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) a[i] = TRANS ? w[k * PW + ty + 16 * i] : w[(ty + 16 * i) * PW + k];
+#pragma unroll
+    for (int g = 0; g < NC / 4; ++g) {
+      const float4 x = *reinterpret_cast<const float4*>(X + k * PX + 4 * tx + 64 * g);
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        out[i][4 * g] = fmaf(a[i], x.x, out[i][4 * g]);
+        out[i][4 * g + 1] = fmaf(a[i], x.y, out[i][4 * g + 1]);
+        out[i][4 * g + 2] = fmaf(a[i], x.z, out[i][4 * g + 2]);
+        out[i][4 * g + 3] = fmaf(a[i], x.w, out[i][4 * g + 3]);
+      }
+    }
+  }
+}
+
+template <typename T, int R, int NC>
+__device__ __forceinline__ void store_rows(T* dst, int64_t stride, const float (&v)[R][NC], float f, int r0, int rows,
+                                           int dim, int ty, int tx) {
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int r = r0 + ty + 16 * i;
+    if (r >= rows) continue;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = 4 * tx + 64 * (c / 4) + (c % 4);
+      if (col < dim) dst[(int64_t)r * stride + col] = from_f32<T>(v[i][c] * f);
+    }
+  }
+}
+
+template <int TT, int DM, int DV>
+struct Tile {
+  static constexpr int R = TT / 16, PD = DM + 4, PV = DV + 4, PP = TT + 4;
+  static constexpr int fwd = (4 * TT * PD + TT * PV + 2 * TT * PP) * 4;
+  static constexpr int dkv = (4 * TT * PD + 2 * TT * PV + 3 * TT * PP) * 4;
+  static constexpr int dq = (4 * TT * PD + 2 * TT * PV + 2 * TT * PP) * 4;
+};
+
+}  // namespace
+
+template <typename T, int TT, int DM, int DV>
+__global__ void __launch_bounds__(256, 1) k_diff_fwd_simt(const __grid_constant__ amc_diff_attention p) {
+  using L = Tile<TT, DM, DV>;
+  constexpr int R = L::R;
+  extern __shared__ float diff_sm[];
+  float *sQ = diff_sm, *sK = sQ + 2 * TT * L::PD, *sV = sK + 2 * TT * L::PD, *sP = sV + TT * L::PV;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int r0 = blockIdx.x * TT, h = blockIdx.y, b = blockIdx.z, g = h / (p.heads / p.kv_heads);
+  const DiffLens len = diff_lens(p, b);
+  const float lam = lam_of<T>(p, h);
+  const float c2 = p.scale * kLog2e;
+  const int dim4 = (p.d + 3) & ~3;
+  for (int m = 0; m < 2; ++m)
+    load_tile<T, TT, DM, L::PD>(sQ + m * TT * L::PD, (const T*)p.q + b * p.qs[0] + (2 * h + m) * p.qs[1], p.qs[2], r0,
+                                len.nq, p.d);
+  int lim[R];
+  float top[2][R], sum[2][R], o[2][R][DV / 16];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    lim[i] = diff_limit(len, p.causal, r0 + ty + 16 * i);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      top[m][i] = -INFINITY;
+      sum[m][i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < DV / 16; ++c) o[m][i][c] = 0.f;
+    }
+  }
+  const int last = min(r0 + TT, len.nq) - 1;
+  const int kend = last >= r0 ? diff_limit(len, p.causal, last) : 0;
+  for (int k0 = 0; k0 < kend; k0 += TT) {
+    __syncthreads();
+    for (int m = 0; m < 2; ++m)
+      load_tile<T, TT, DM, L::PD>(sK + m * TT * L::PD, (const T*)p.k + b * p.ks[0] + (2 * g + m) * p.ks[1], p.ks[2], k0,
+                                  len.nk, p.d);
+    load_tile<T, TT, DV, L::PV>(sV, (const T*)p.v + b * p.vs[0] + g * p.vs[1], p.vs[2], k0, len.nk, p.dv);
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      float s[R][R] = {};
+      dot_rows<R, L::PD>(s, sQ + m * TT * L::PD, sK + m * TT * L::PD, dim4, ty, tx);
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        float mx = top[m][i];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+          s[i][j] = k0 + tx + 16 * j < lim[i] ? s[i][j] * c2 : -INFINITY;
+          mx = fmaxf(mx, s[i][j]);
+        }
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+        const float base = mx == -INFINITY ? 0.f : mx;   // a row that has seen no key yet
+        const float corr = exp2f(top[m][i] - base);
+        float add = 0.f;
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+          const float e = exp2f(s[i][j] - base);
+          add += e;
+          sP[m * TT * L::PP + (ty + 16 * i) * L::PP + tx + 16 * j] = e;
+        }
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) add += __shfl_xor_sync(0xffffffffu, add, w);
+        sum[m][i] = sum[m][i] * corr + add;
+        top[m][i] = mx;
+#pragma unroll
+        for (int c = 0; c < DV / 16; ++c) o[m][i][c] *= corr;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+      mul_rows<R, DV / 16, TT, L::PP, L::PV, false>(o[m], sP + m * TT * L::PP, sV, ty, tx);
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int r = r0 + ty + 16 * i;
+    float inv[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      inv[m] = sum[m][i] > 0.f ? 1.f / sum[m][i] : 0.f;
+      if (p.lse && tx == 0 && r < p.nq)
+        p.lse[((int64_t)b * 2 * p.heads + 2 * h + m) * p.nq + r] =
+            sum[m][i] > 0.f ? fmaf(top[m][i], kLn2, logf(sum[m][i])) : -INFINITY;
+    }
+#pragma unroll
+    for (int c = 0; c < DV / 16; ++c) {
+      o[1][i][c] *= inv[1];
+      o[0][i][c] = fmaf(-lam, o[1][i][c], o[0][i][c] * inv[0]);
+    }
+  }
+  store_rows<T, R, DV / 16>((T*)p.o + b * p.os[0] + h * p.os[1], p.os[2], o[0], 1.f, r0, p.nq, p.dv, ty, tx);
+  if (p.o2) store_rows<T, R, DV / 16>((T*)p.o2 + b * p.o2s[0] + h * p.o2s[1], p.o2s[2], o[1], 1.f, r0, p.nq, p.dv, ty, tx);
+}
+
+// One warp per row: DiffRow from lse, o, o2 and dO.
+template <typename T>
+__global__ void __launch_bounds__(256) k_diff_bwd_rows(const __grid_constant__ amc_diff_attention p,
+                                                       DiffRow* __restrict__ rows) {
+  const int lane = threadIdx.x & 31;
+  const int i = blockIdx.x * 8 + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
+  if (i >= p.nq) return;
+  const DiffLens len = diff_lens(p, b);
+  DiffRow r{INFINITY, 0.f, INFINITY, 0.f};
+  if (diff_limit(len, p.causal, i) > 0) {
+    const T* o = (const T*)p.o + b * p.os[0] + h * p.os[1] + (int64_t)i * p.os[2];
+    const T* o2 = (const T*)p.o2 + b * p.o2s[0] + h * p.o2s[1] + (int64_t)i * p.o2s[2];
+    const T* go = (const T*)p.d_o + b * p.dos[0] + h * p.dos[1] + (int64_t)i * p.dos[2];
+    const float lam = lam_of<T>(p, h);
+    float d = 0.f, d2 = 0.f;
+    for (int c = lane; c < p.dv; c += 32) {
+      const float x = to_f32(go[c]);
+      d = fmaf(x, to_f32(o[c]), d);
+      d2 = fmaf(x, to_f32(o2[c]), d2);
+    }
+    for (int w = 16; w > 0; w >>= 1) {
+      d += __shfl_xor_sync(0xffffffffu, d, w);
+      d2 += __shfl_xor_sync(0xffffffffu, d2, w);
+    }
+    const float* lse = p.lse + ((int64_t)b * 2 * p.heads + 2 * h) * p.nq + i;
+    r.lse1 = lse[0] * kLog2e;
+    r.lse2 = lse[p.nq] * kLog2e;
+    r.d1 = fmaf(lam, d2, d);   // dO . O_1 = dO . (O + lam O_2)
+    r.d2 = d2;
+  }
+  if (lane == 0) rows[((int64_t)b * p.heads + h) * p.nq + i] = r;
+}
+
+// dK, dV of TT keys of one key head: streams the rows of its query heads.
+template <typename T, int TT, int DM, int DV>
+__global__ void __launch_bounds__(256, 1) k_diff_dkv_simt(const __grid_constant__ amc_diff_attention p,
+                                                          const DiffRow* __restrict__ rows) {
+  using L = Tile<TT, DM, DV>;
+  constexpr int R = L::R;
+  extern __shared__ float diff_sm[];
+  float *sK = diff_sm, *sQ = sK + 2 * TT * L::PD, *sV = sQ + 2 * TT * L::PD, *sG = sV + TT * L::PV;
+  float *sB = sG + TT * L::PV, *sS = sB + TT * L::PP;   // P_1 - lam P_2, then dS_1 and dS_2, as [row][key]
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int k0 = blockIdx.x * TT, g = blockIdx.y, b = blockIdx.z, group = p.heads / p.kv_heads;
+  const DiffLens len = diff_lens(p, b);
+  const float c2 = p.scale * kLog2e;
+  const int dim4 = (p.d + 3) & ~3, dimv4 = (p.dv + 3) & ~3;
+  for (int m = 0; m < 2; ++m)
+    load_tile<T, TT, DM, L::PD>(sK + m * TT * L::PD, (const T*)p.k + b * p.ks[0] + (2 * g + m) * p.ks[1], p.ks[2], k0,
+                                len.nk, p.d);
+  load_tile<T, TT, DV, L::PV>(sV, (const T*)p.v + b * p.vs[0] + g * p.vs[1], p.vs[2], k0, len.nk, p.dv);
+  float dk[2][R][DM / 16] = {}, dv[R][DV / 16] = {};
+  const int first = diff_first_row(len, p.causal, k0) / TT * TT;
+  for (int h = g * group; h < (g + 1) * group; ++h) {
+    const float lam = lam_of<T>(p, h);
+    for (int r0 = first; r0 < len.nq; r0 += TT) {
+      __syncthreads();
+      for (int m = 0; m < 2; ++m)
+        load_tile<T, TT, DM, L::PD>(sQ + m * TT * L::PD, (const T*)p.q + b * p.qs[0] + (2 * h + m) * p.qs[1], p.qs[2],
+                                    r0, len.nq, p.d);
+      load_tile<T, TT, DV, L::PV>(sG, (const T*)p.d_o + b * p.dos[0] + h * p.dos[1], p.dos[2], r0, len.nq, p.dv);
+      __syncthreads();
+      float gv[R][R] = {}, both[R][R];
+      dot_rows<R, L::PV>(gv, sG, sV, dimv4, ty, tx);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        float s[R][R] = {};
+        dot_rows<R, L::PD>(s, sQ + m * TT * L::PD, sK + m * TT * L::PD, dim4, ty, tx);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const int r = r0 + ty + 16 * i;
+          const int lim = diff_limit(len, p.causal, r);
+          const DiffRow e = lim > 0 ? rows[((int64_t)b * p.heads + h) * p.nq + r] : DiffRow{INFINITY, 0.f, INFINITY, 0.f};
+#pragma unroll
+          for (int j = 0; j < R; ++j) {
+            const float pr = k0 + tx + 16 * j < lim ? exp2f(fmaf(s[i][j], c2, -(m ? e.lse2 : e.lse1))) : 0.f;
+            const float w = m ? -lam * pr : pr;
+            both[i][j] = m ? both[i][j] + w : w;
+            sS[m * TT * L::PP + (ty + 16 * i) * L::PP + tx + 16 * j] = w * (gv[i][j] - (m ? e.d2 : e.d1));
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < R; ++j) sB[(ty + 16 * i) * L::PP + tx + 16 * j] = both[i][j];
+      __syncthreads();
+      mul_rows<R, DV / 16, TT, L::PP, L::PV, true>(dv, sB, sG, ty, tx);
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+        mul_rows<R, DM / 16, TT, L::PP, L::PD, true>(dk[m], sS + m * TT * L::PP, sQ + m * TT * L::PD, ty, tx);
+    }
+  }
+  for (int m = 0; m < 2; ++m)
+    store_rows<T, R, DM / 16>((T*)p.dk + b * p.dks[0] + (2 * g + m) * p.dks[1], p.dks[2], dk[m], p.scale, k0, p.nk, p.d,
+                              ty, tx);
+  store_rows<T, R, DV / 16>((T*)p.dv_ + b * p.dvs[0] + g * p.dvs[1], p.dvs[2], dv, 1.f, k0, p.nk, p.dv, ty, tx);
+}
+
+// dQ of TT rows, and this tile's part of sum P_2 G.
+template <typename T, int TT, int DM, int DV>
+__global__ void __launch_bounds__(256, 1) k_diff_dq_simt(const __grid_constant__ amc_diff_attention p,
+                                                         const DiffRow* __restrict__ rows,
+                                                         float* __restrict__ partials) {
+  using L = Tile<TT, DM, DV>;
+  constexpr int R = L::R;
+  extern __shared__ float diff_sm[];
+  float *sQ = diff_sm, *sK = sQ + 2 * TT * L::PD, *sG = sK + 2 * TT * L::PD, *sV = sG + TT * L::PV;
+  float* sS = sV + TT * L::PV;
+  __shared__ float red[8];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int r0 = blockIdx.x * TT, h = blockIdx.y, b = blockIdx.z, g = h / (p.heads / p.kv_heads);
+  const DiffLens len = diff_lens(p, b);
+  const float lam = lam_of<T>(p, h);
+  const float c2 = p.scale * kLog2e;
+  const int dim4 = (p.d + 3) & ~3, dimv4 = (p.dv + 3) & ~3;
+  for (int m = 0; m < 2; ++m)
+    load_tile<T, TT, DM, L::PD>(sQ + m * TT * L::PD, (const T*)p.q + b * p.qs[0] + (2 * h + m) * p.qs[1], p.qs[2], r0,
+                                len.nq, p.d);
+  load_tile<T, TT, DV, L::PV>(sG, (const T*)p.d_o + b * p.dos[0] + h * p.dos[1], p.dos[2], r0, len.nq, p.dv);
+  int lim[R];
+  DiffRow e[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int r = r0 + ty + 16 * i;
+    lim[i] = diff_limit(len, p.causal, r);
+    e[i] = lim[i] > 0 ? rows[((int64_t)b * p.heads + h) * p.nq + r] : DiffRow{INFINITY, 0.f, INFINITY, 0.f};
+  }
+  float dq[2][R][DM / 16] = {}, pg = 0.f;
+  const int last = min(r0 + TT, len.nq) - 1;
+  const int kend = last >= r0 ? diff_limit(len, p.causal, last) : 0;
+  for (int k0 = 0; k0 < kend; k0 += TT) {
+    __syncthreads();
+    for (int m = 0; m < 2; ++m)
+      load_tile<T, TT, DM, L::PD>(sK + m * TT * L::PD, (const T*)p.k + b * p.ks[0] + (2 * g + m) * p.ks[1], p.ks[2], k0,
+                                  len.nk, p.d);
+    load_tile<T, TT, DV, L::PV>(sV, (const T*)p.v + b * p.vs[0] + g * p.vs[1], p.vs[2], k0, len.nk, p.dv);
+    __syncthreads();
+    float gv[R][R] = {}, part = 0.f;
+    dot_rows<R, L::PV>(gv, sG, sV, dimv4, ty, tx);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      float s[R][R] = {};
+      dot_rows<R, L::PD>(s, sQ + m * TT * L::PD, sK + m * TT * L::PD, dim4, ty, tx);
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+          const float pr = k0 + tx + 16 * j < lim[i] ? exp2f(fmaf(s[i][j], c2, -(m ? e[i].lse2 : e[i].lse1))) : 0.f;
+          if (m) part = fmaf(pr, gv[i][j], part);
+          sS[m * TT * L::PP + (ty + 16 * i) * L::PP + tx + 16 * j] =
+              (m ? -lam * pr : pr) * (gv[i][j] - (m ? e[i].d2 : e[i].d1));
+        }
+    }
+    pg += part;
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+      mul_rows<R, DM / 16, TT, L::PP, L::PD, false>(dq[m], sS + m * TT * L::PP, sK + m * TT * L::PD, ty, tx);
+  }
+  for (int m = 0; m < 2; ++m)
+    store_rows<T, R, DM / 16>((T*)p.dq + b * p.dqs[0] + (2 * h + m) * p.dqs[1], p.dqs[2], dq[m], p.scale, r0, p.nq, p.d,
+                              ty, tx);
+  for (int w = 16; w > 0; w >>= 1) pg += __shfl_xor_sync(0xffffffffu, pg, w);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = pg;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float t = 0.f;
+    for (int w = 0; w < 8; ++w) t += red[w];
+    partials[((int64_t)h * p.batch + b) * gridDim.x + blockIdx.x] = t;
+  }
+}
+
+// dlam rows from the partials of sum P_2 G: one CTA per row of lam, a fixed
+// order of summation, in double.
+template <typename T>
+__global__ void __launch_bounds__(256) k_diff_dlam(const __grid_constant__ amc_diff_attention p,
+                                                   const float* __restrict__ partials, int64_t per_head) {
+  __shared__ double red[256];
+  const int64_t n = p.lam_rows == 1 ? per_head * p.heads : per_head;
+  const float* x = partials + (int64_t)blockIdx.x * per_head;
+  double t = 0.0;
+  for (int64_t i = threadIdx.x; i < n; i += 256) t += x[i];
+  red[threadIdx.x] = t;
+  __syncthreads();
+  for (int w = 128; w > 0; w >>= 1) {
+    if (threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
+    __syncthreads();
+  }
+  const float dl = (float)-red[0];
+  const float2 e = lam_exps<T>(p, blockIdx.x);
+  const T* l = (const T*)p.lam + (size_t)blockIdx.x * 4 * p.d;
+  T* o = (T*)p.dlam + (size_t)blockIdx.x * 4 * p.d;
+  for (int i = threadIdx.x; i < p.d; i += 256) {
+    o[i] = from_f32<T>(dl * e.x * to_f32(l[p.d + i]));
+    o[p.d + i] = from_f32<T>(dl * e.x * to_f32(l[i]));
+    o[2 * p.d + i] = from_f32<T>(-dl * e.y * to_f32(l[3 * p.d + i]));
+    o[3 * p.d + i] = from_f32<T>(-dl * e.y * to_f32(l[2 * p.d + i]));
+  }
+}
+
+namespace {
+
+template <typename F>
+int by_type(int32_t dtype, F f) {
+  if (dtype == AMC_F32) return f(float());
+  if (dtype == AMC_BF16) return f(__nv_bfloat16());
+  return f(__half());
+}
+
+template <typename T, int TT, int DM, int DV>
+int fwd_simt(const amc_diff_attention& p, cudaStream_t s) {
+  static std::atomic<uint64_t> attr{0};
+  if (int rc = smem_attr_once(k_diff_fwd_simt<T, TT, DM, DV>, Tile<TT, DM, DV>::fwd, attr)) return rc;
+  k_diff_fwd_simt<T, TT, DM, DV><<<dim3((p.nq + TT - 1) / TT, p.heads, p.batch), 256, Tile<TT, DM, DV>::fwd, s>>>(p);
+  AMC_CUDA(cudaGetLastError());
+  return AMC_OK;
+}
+
+template <typename T, int TT, int DM, int DV>
+int bwd_simt(const amc_diff_attention& p, DiffRow* rows, float* partials, cudaStream_t s) {
+  static std::atomic<uint64_t> attr_dkv{0}, attr_dq{0};
+  using L = Tile<TT, DM, DV>;
+  if (int rc = smem_attr_once(k_diff_dkv_simt<T, TT, DM, DV>, L::dkv, attr_dkv)) return rc;
+  if (int rc = smem_attr_once(k_diff_dq_simt<T, TT, DM, DV>, L::dq, attr_dq)) return rc;
+  if (p.nk) {
+    k_diff_dkv_simt<T, TT, DM, DV><<<dim3((p.nk + TT - 1) / TT, p.kv_heads, p.batch), 256, L::dkv, s>>>(p, rows);
+    AMC_CUDA(cudaGetLastError());
+  }
+  const int tiles = (p.nq + TT - 1) / TT;
+  if (p.nq) {
+    k_diff_dq_simt<T, TT, DM, DV><<<dim3(tiles, p.heads, p.batch), 256, L::dq, s>>>(p, rows, partials);
+    AMC_CUDA(cudaGetLastError());
+  }
+  return launch_diff_dlam(p, partials, tiles, s);
+}
+
+}  // namespace
+
+int launch_diff_fwd_simt(const amc_diff_attention& p, cudaStream_t s) {
+  return by_type(p.dtype, [&](auto t) {
+    using T = decltype(t);
+    return p.d <= 64 && p.dv <= 128 ? fwd_simt<T, 64, 64, 128>(p, s) : fwd_simt<T, 32, 128, 256>(p, s);
+  });
+}
+
+int launch_diff_bwd_rows(const amc_diff_attention& p, DiffRow* rows, cudaStream_t s) {
+  if (!p.nq) return AMC_OK;
+  return by_type(p.dtype, [&](auto t) {
+    k_diff_bwd_rows<decltype(t)><<<dim3((p.nq + 7) / 8, p.heads, p.batch), 256, 0, s>>>(p, rows);
+    AMC_CUDA(cudaGetLastError());
+    return AMC_OK;
+  });
+}
+
+int launch_diff_bwd_simt(const amc_diff_attention& p, DiffRow* rows, float* partials, cudaStream_t s) {
+  return by_type(p.dtype, [&](auto t) {
+    using T = decltype(t);
+    return p.d <= 64 && p.dv <= 128 ? bwd_simt<T, 64, 64, 128>(p, rows, partials, s)
+                                    : bwd_simt<T, 32, 128, 256>(p, rows, partials, s);
+  });
+}
+
+int launch_diff_dlam(const amc_diff_attention& p, const float* partials, int tiles, cudaStream_t s) {
+  return by_type(p.dtype, [&](auto t) {
+    k_diff_dlam<decltype(t)><<<p.lam_rows, 256, 0, s>>>(p, partials, (int64_t)p.batch * tiles);
+    AMC_CUDA(cudaGetLastError());
+    return AMC_OK;
+  });
+}
+
+namespace {
+
+int check_sizes(const amc_diff_attention* p, const char* who) {
+  if (!p) return fail(AMC_ERR_INVALID, std::string(who) + ": null argument");
+  if (p->dtype != AMC_F32 && p->dtype != AMC_BF16 && p->dtype != AMC_F16)
+    return fail(AMC_ERR_INVALID, std::string(who) + ": dtype must be f32, bf16 or f16");
+  if (p->batch < 0 || p->nq < 0 || p->nk < 0 || p->heads <= 0 || p->kv_heads <= 0 || p->heads % p->kv_heads)
+    return fail(AMC_ERR_INVALID, std::string(who) + ": bad sizes (heads must be a multiple of kv_heads)");
+  if (p->d <= 0 || p->d > 128 || p->dv <= 0 || p->dv > 256)
+    return fail(AMC_ERR_INVALID, std::string(who) + ": head dims d 1..128, dv 1..256");
+  if (p->batch > 65535 || p->heads > 32767 || p->nq > (1 << 30) || p->nk > (1 << 30))
+    return fail(AMC_ERR_INVALID, std::string(who) + ": batch up to 65535, heads up to 32767, rows up to 2^30");
+  if (p->lam_rows != 1 && p->lam_rows != p->heads)
+    return fail(AMC_ERR_INVALID, std::string(who) + ": lam has 1 row or one for each head");
+  return AMC_OK;
+}
+
+size_t fwd_bytes(const amc_diff_attention&) { return 0; }
+size_t bwd_bytes(const amc_diff_attention& p) { return diff_rows_bytes(p) + diff_partials(p) * sizeof(float); }
+
+int check_workspace(const amc_diff_attention* p, size_t need, const char* who) {
+  if (!need) return AMC_OK;
+  if (!p->workspace || p->workspace_bytes < 0 || (size_t)p->workspace_bytes < need || ((uintptr_t)p->workspace & 15))
+    return fail(AMC_ERR_INVALID, std::string(who) + ": workspace of " + std::to_string(need) +
+                                     " bytes, 16-byte aligned, expected");
+  return AMC_OK;
+}
+
+}  // namespace
+
+}  // namespace amc
+
+using namespace amc;
+
+extern "C" {
+
+int amc_diff_attention_workspace(const amc_diff_attention* p, int32_t backward, int64_t* bytes) {
+  if (!bytes) return fail(AMC_ERR_INVALID, "amc_diff_attention_workspace: null out");
+  if (int rc = check_sizes(p, "amc_diff_attention_workspace")) return rc;
+  size_t n = fwd_bytes(*p);
+  if (backward && bwd_bytes(*p) > n) n = bwd_bytes(*p);
+  *bytes = (int64_t)n;
+  return AMC_OK;
+}
+
+int amc_diff_attention_fwd(const amc_diff_attention* p, void* stream) {
+  if (int rc = check_sizes(p, "amc_diff_attention_fwd")) return rc;
+  if (!p->batch || !p->nq) return AMC_OK;
+  if (!p->q || !p->o || !p->lam || (p->nk && (!p->k || !p->v)))
+    return fail(AMC_ERR_INVALID, "amc_diff_attention_fwd: null tensor");
+  if (int rc = check_workspace(p, fwd_bytes(*p), "amc_diff_attention_fwd")) return rc;
+  if (fault_injected("launch")) return fail(AMC_ERR_INJECTED, "diff_attention: injected launch failure (AMC_FAULT=launch)");
+  return launch_diff_fwd_simt(*p, pick_stream(stream));
+}
+
+int amc_diff_attention_bwd(const amc_diff_attention* p, void* stream) {
+  if (int rc = check_sizes(p, "amc_diff_attention_bwd")) return rc;
+  if (!p->lam || !p->dlam) return fail(AMC_ERR_INVALID, "amc_diff_attention_bwd: null tensor");
+  if (p->batch && ((p->nq && (!p->q || !p->o || !p->o2 || !p->lse || !p->d_o || !p->dq)) ||
+                   (p->nk && (!p->k || !p->v || !p->dk || !p->dv_))))
+    return fail(AMC_ERR_INVALID, "amc_diff_attention_bwd: null tensor");
+  if (int rc = check_workspace(p, bwd_bytes(*p), "amc_diff_attention_bwd")) return rc;
+  if (fault_injected("launch")) return fail(AMC_ERR_INJECTED, "diff_attention: injected launch failure (AMC_FAULT=launch)");
+  cudaStream_t s = pick_stream(stream);
+  DiffRow* rows = (DiffRow*)p->workspace;
+  float* partials = (float*)((char*)p->workspace + diff_rows_bytes(*p));
+  if (!p->batch) return launch_diff_dlam(*p, partials, 0, s);
+  if (int rc = launch_diff_bwd_rows(*p, rows, s)) return rc;
+  return launch_diff_bwd_simt(*p, rows, partials, s);
+}
+
+}  // extern "C"

@@ -367,6 +367,114 @@ int amc_conv2d_dgrad_f32(const float* dY, const float* W, float* dX, int32_t N, 
 int amc_conv2d_wgrad_f32(const float* X, const float* dY, float* dW, int32_t N, int32_t C, int32_t H, int32_t Wd,
                          int32_t K, int32_t KH, int32_t KW, int32_t SH, int32_t SW, int32_t PH, int32_t PW, void* stream);
 
+/* ---------------------------------------------------------------- differential-attention layer
+ * The operators of a layer whose attention is the difference of two softmax
+ * maps, and of its training step, on device pointers.  No counterpart in the
+ * reference (its attention is one unmasked map, realization.scm:279-396, and
+ * its optimizer the plain step of example 9).  Tensors are (batch, heads,
+ * rows, dim) with any element strides over the first three axes and unit
+ * stride along dim; dtype is AMC_F32, AMC_BF16 or AMC_F16.  All arithmetic
+ * between loads and stores is f32 or wider.  Nothing is allocated: scratch is
+ * the caller's `workspace`, which two calls that may overlap must not share. */
+#define AMC_BF16 16
+#define AMC_F16  17
+#define AMC_E4M3 18   /* 8-bit optimizer states only */
+
+/* Rotary positions.  Pair i of a row at position p turns by p * freqs[i]
+ * radians (formed in f64, so far positions keep their angle) and is scaled by
+ * mscale: out_a = ms (a cos - b sin), out_b = ms (b cos + a sin).  The pair is
+ * elements (i, i + rot/2), or (2i, 2i + 1) when interleaved; elements from
+ * rot on are copied.  inverse != 0 turns back, which is the gradient.  One or
+ * two tensors (queries and keys) of one batch, n, d and dtype in one launch;
+ * out may be x itself, with the same strides.  pos is s64, element (b, i) at
+ * pos[b * pos_stride + i]; freqs rot/2 doubles on the device. */
+typedef struct amc_rope_tensor {
+  const void* x;
+  void* out;
+  int64_t heads;
+  int64_t xs[3];                    /* strides over batch, head, row         */
+  int64_t os[3];
+} amc_rope_tensor;
+int amc_rope(const amc_rope_tensor* t, int32_t count, int32_t dtype, int64_t batch, int64_t n, int32_t d, int32_t rot,
+             const int64_t* pos, int64_t pos_stride, const double* freqs, float mscale, int32_t interleaved,
+             int32_t inverse, void* stream);
+/* The frequencies base^(-2i/rot), i < rot/2, for contexts `factor` times the
+ * original length, into host memory; *mscale receives the factor of
+ * amc_rope.  AMC_ROPE_LINEAR divides every frequency by factor.
+ * AMC_ROPE_BASE raises the base by factor^(rot/(rot-2)), which keeps the
+ * fastest pair and divides the slowest by factor.  AMC_ROPE_PARTS divides the
+ * pairs that turn less than slow times over original_len, keeps those that
+ * turn more than fast times, ramps between, and gives
+ * mscale = 0.1 ln(factor) + 1 (1 for the other kinds). */
+#define AMC_ROPE_PLAIN  0
+#define AMC_ROPE_LINEAR 1
+#define AMC_ROPE_BASE   2
+#define AMC_ROPE_PARTS  3
+int amc_rope_freqs(double* host_out, int32_t rot, double base, int32_t kind, double factor, int64_t original_len,
+                   double slow, double fast, float* mscale);
+
+/* Differential attention.  Query head h has two maps, heads 2h and 2h + 1 of
+ * q; key head g likewise heads 2g and 2g + 1 of k, and one v; query head h
+ * reads key head h / (heads / kv_heads).
+ *   P_m = softmax(scale * Q_m K_m^T),  m = 1, 2
+ *   lam = exp(l0 . l1) - exp(l2 . l3) + lam_init, l the 4 rows of this head
+ *   O   = (P_1 - lam P_2) V
+ * Row i of sequence b attends to the keys j < kv_lens[b] (nk when NULL), and
+ * with causal to j <= i + kv_lens[b] - q_lens[b] only: the last row sees the
+ * last key.  Rows from q_lens[b] on, and rows that see no key, give 0 (lse
+ * -inf) and no gradient.  Elements of q, k, v and d_o behind q_lens and
+ * kv_lens are not used, whatever they hold.
+ * lse (batch, 2 heads, nq, contiguous) receives the natural-log row
+ * log-sum-exp of each map, o2 (optional; the backward needs it) the second
+ * map's P_2 V.  lam is (lam_rows, 4, d) contiguous of `dtype`, lam_rows 1
+ * (one lam for all heads) or heads.  d 1..128, dv 1..256.
+ * The backward reads o, o2 and lse of the forward and writes dq, dk, dv
+ * (gradients of shared heads summed) and dlam, the gradients of all 4 rows.
+ * No atomics: repeated calls give identical bits. */
+typedef struct amc_diff_attention {
+  int32_t dtype, causal;
+  int32_t batch, heads, kv_heads, nq, nk, d, dv, lam_rows;
+  float scale, lam_init;
+  const void *q, *k, *v, *lam;
+  const int32_t *q_lens, *kv_lens;  /* (batch), device, or NULL              */
+  void *o, *o2;
+  float* lse;
+  const void* d_o;                  /* backward only, from here              */
+  void *dq, *dk, *dv_, *dlam;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t qs[3], ks[3], vs[3], os[3], o2s[3], dos[3], dqs[3], dks[3], dvs[3];
+} amc_diff_attention;
+int amc_diff_attention_fwd(const amc_diff_attention* p, void* stream);
+int amc_diff_attention_bwd(const amc_diff_attention* p, void* stream);
+/* The workspace a call of these sizes needs (it may be 0). */
+int amc_diff_attention_workspace(const amc_diff_attention* p, int32_t backward, int64_t* bytes);
+
+/* AdamW step over `count` tensors, in one launch for every 256 of them:
+ *   m = b1 m + (1-b1) g,  v = b2 v + (1-b2) g^2,  t = steps done + 1
+ *   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * p and g are p_dtype and g_dtype (F32, BF16, F16); with `master` the update
+ * is made on that f32 copy and p receives it rounded.  States are f32, or
+ * AMC_E4M3: m and sqrt(v) as 8-bit floats over a scale for every 256
+ * elements (m_scale, v_scale: ceil(n/256) floats), rounded up or down at
+ * random with 20 bits mixed from element, tensor and step, because a moving
+ * average that changes by less than half a code would stand still under
+ * nearest rounding; a nonzero root never rounds to 0.
+ * step_state is two s64 on the device: the steps done, which the call
+ * increments, and a counter that must be 0 before the first call; so a
+ * captured step advances at each replay.  lr_dev, if not NULL, holds lr on
+ * the device.  Contiguous tensors of any length and element alignment. */
+typedef struct amc_adamw_tensor {
+  void* p;
+  const void* g;
+  void *m, *v;
+  float *master, *m_scale, *v_scale;
+  int64_t n;
+} amc_adamw_tensor;
+int amc_adamw(const amc_adamw_tensor* t, int32_t count, int32_t p_dtype, int32_t g_dtype, int32_t state_dtype,
+              int64_t* step_state, const float* lr_dev, double lr, double beta1, double beta2, double eps,
+              double weight_decay, void* stream);
+
 /* ---------------------------------------------------------------- multi-GPU
  * Fixed-order sum over the GPUs of one node (one process per GPU), the
  * reduction that crosses the batch axis of a sharded workload

@@ -1,0 +1,440 @@
+"""The differential-attention layer's operators (amcuda.nn) against plain
+64-bit implementations on the device.
+
+Tolerances count roundings.  u is the half step of the stored type (bf16 2^-8,
+fp16 2^-11, fp32 2^-24 relative).  A 16-bit result carries its own rounding
+(u of the value) and, in the tensor-core and split forms, the rounding of the
+probabilities (and in the backward of dS) to 16 bits, u of each term: bounded
+by u * sum |terms|, the same product with absolute values, so every comparison
+is element by element against u * (|result| + 2 * absolute product) plus f32
+accumulation, 2^-24 times the length of the sums, on the same absolute product.
+"""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+@pytest.fixture(scope="module")
+def nn(amc):
+    from amcuda import nn
+    return nn
+
+
+def randn(shape, seed, dtype, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+# ---------------------------------------------------------------------------- rope
+def rope_ref(x, pos, freqs, mscale, interleaved, inverse):
+    """The rotation in 64 bits, and sum |terms| of each element."""
+    r = 2 * len(freqs)
+    B, n = x.shape[0], x.shape[2]
+    a = pos.expand(B, n).double()[:, None, :, None] * freqs
+    c, s = a.cos() * mscale, a.sin() * (-mscale if inverse else mscale)
+    xd = x.double()
+    y, t = xd.clone(), xd.abs()
+    ia, ib = (slice(0, r, 2), slice(1, r, 2)) if interleaved else (slice(0, r // 2), slice(r // 2, r))
+    xa, xb = xd[..., ia], xd[..., ib]
+    y[..., ia], y[..., ib] = xa * c - xb * s, xb * c + xa * s
+    t[..., ia] = t[..., ib] = (xa.abs() + xb.abs()) * mscale
+    return y, t
+
+
+def rope_close(got, ref, terms, dtype):
+    # f32: the reduced angle (half a turn) is rounded to 2^-25 turns and the
+    # sine and cosine carry 2 ulp, so 2^-25 * 2 pi + 2 * 2^-23 < 2^-21 of the
+    # terms, and the products and their sum 3 more half steps
+    tol = half_step(dtype) * ref.abs() + (2.0 ** -21 + 3 * 2.0 ** -24) * terms + 1e-30
+    if dtype is torch.float16:
+        tol = tol + 2.0 ** -25          # half of fp16's subnormal step
+    bad = (got.double() - ref).abs() > tol
+    assert not bad.any(), ((got.double() - ref).abs() / tol).max().item()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("B,H,H2,n,d,rot", [(2, 3, 1, 17, 64, 64), (1, 1, 0, 1, 2, 2), (3, 2, 5, 1, 80, 48),
+                                           (2, 4, 4, 130, 20, 6), (1, 16, 4, 33, 128, 128)])
+def test_rope(nn, dtype, interleaved, B, H, H2, n, d, rot):
+    t = TYPES[dtype]
+    x, x2 = randn((B, n, H, d), 1, t).transpose(1, 2), randn((B, H2, n, d), 2, t) if H2 else None
+    pos = torch.randint(0, 1 << 20, (B, n), device="cuda")
+    freqs, ms = nn.rope_freqs(rot, kind="parts", factor=4.0, original_len=4096)
+    freqs = freqs.cuda()
+    for inverse in (False, True):
+        out, out2 = torch.full_like(x, 7), torch.full_like(x2, 7) if H2 else None
+        nn.rope(x, pos, freqs, out, x2, out2, mscale=ms, interleaved=interleaved, inverse=inverse)
+        for a, o in ((x, out), (x2, out2)):
+            if a is not None:
+                rope_close(o, *rope_ref(a, pos, freqs, ms, interleaved, inverse), t)
+
+
+def test_rope_in_place_strided_and_far(nn):
+    """In place on a slice of a wider projection (rows not 16-byte aligned), at
+    positions past 2^32, with one (n,) position vector."""
+    for offset in (0, 3):
+        wide = randn((2, 40, 3, 64 + 8), 3, torch.bfloat16)
+        x = wide[..., offset:offset + 64].transpose(1, 2)
+        keep = wide.clone()
+        pos = (1 << 33) + torch.arange(40, device="cuda") * 12345677
+        freqs, _ = nn.rope_freqs(64)
+        freqs = freqs.cuda()
+        ref, terms = rope_ref(x, pos, freqs, 1.0, False, False)
+        nn.rope(x, pos, freqs, x)
+        rope_close(x, ref, terms, torch.bfloat16)
+        assert torch.equal(wide[..., :offset], keep[..., :offset])
+        assert torch.equal(wide[..., offset + 64:], keep[..., offset + 64:])
+
+
+def test_rope_gradient_by_differences(nn):
+    """<w, R(x + h v) - R(x - h v)> / 2h = <R^T w, v>: R is linear."""
+    x, v, w = (randn((1, 2, 9, 12), s, torch.float32) for s in (4, 5, 6))
+    pos = torch.arange(9, device="cuda") * 37
+    freqs, ms = nn.rope_freqs(8, kind="parts", factor=16.0, original_len=512)
+    freqs = freqs.cuda()
+    up, down, back = torch.empty_like(x), torch.empty_like(x), torch.empty_like(x)
+    nn.rope(x + v, pos, freqs, up, mscale=ms, interleaved=True)
+    nn.rope(x - v, pos, freqs, down, mscale=ms, interleaved=True)
+    nn.rope(w, pos, freqs, back, mscale=ms, interleaved=True, inverse=True)
+    lhs = ((up.double() - down.double()) * w).sum() / 2
+    rhs = (back.double() * v).sum()
+    # 216 products of values of a few units, each 2^-21 of its terms
+    assert abs(lhs - rhs) < 216 * 64 * 2.0 ** -21
+
+
+# ---------------------------------------------------------------------------- differential attention
+LAM_INIT = 0.8
+
+
+class Case:
+    def __init__(self, B, H, K, nq, nk, d, dtype, causal=False, q_lens=None, kv_lens=None, dv=None, lam_rows=None,
+                 seed=0, scale=None, heads_inner=True):
+        t = TYPES[dtype]
+        dv = 2 * d if dv is None else dv
+        self.t, self.causal, self.scale = t, causal, scale or 1 / math.sqrt(d)
+
+        def make(h, n, w, s):
+            if heads_inner:
+                return randn((B, n, h, w), seed + s, t).transpose(1, 2)
+            return randn((B, h, n, w), seed + s, t)
+        self.q, self.k, self.v, self.do = make(2 * H, nq, d, 1), make(2 * K, nk, d, 2), make(K, nk, dv, 3), make(H, nq, dv, 4)
+        self.lam = randn((lam_rows or H, 4, d), seed + 5, t, 0.1)
+        lens = [None if x is None else torch.tensor(x, dtype=torch.int32, device="cuda") for x in (q_lens, kv_lens)]
+        self.q_lens, self.kv_lens = lens
+        self.H, self.K = H, K
+
+    def fwd(self, nn, o2=True, **more):
+        B, _, nq, _ = self.q.shape
+        o = torch.full((B, self.H, nq, self.v.shape[3]), 7.0, dtype=self.t, device="cuda")
+        lse = torch.full((B, 2 * self.H, nq), 7.0, device="cuda")
+        second = torch.full_like(o, 7) if o2 else None
+        ws = torch.empty(nn.diff_attention_workspace(self.q, self.k, self.v), dtype=torch.uint8, device="cuda")
+        nn.diff_attention_fwd(self.q, self.k, self.v, self.lam, o, lse, LAM_INIT, self.scale, causal=self.causal,
+                              q_lens=self.q_lens, kv_lens=self.kv_lens, o2=second, workspace=ws, **more)
+        return o, lse, second
+
+    def bwd(self, nn, o, lse, o2, **more):
+        g = [torch.full_like(x, 7) for x in (self.q, self.k, self.v, self.lam)]
+        n = nn.diff_attention_workspace(self.q, self.k, self.v, backward=True)
+        ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+        nn.diff_attention_bwd(self.q, self.k, self.v, self.lam, o, o2, lse, self.do, *g, LAM_INIT, self.scale,
+                              causal=self.causal, q_lens=self.q_lens, kv_lens=self.kv_lens, workspace=ws, **more)
+        return dict(zip(("dq", "dk", "dv", "dlam"), g))
+
+    def reference(self, backward=False):
+        """name -> (value, sum |terms|) in 64 bits, from the formulas."""
+        B, H2, nq, d = self.q.shape
+        nk, dv, H, K = self.k.shape[2], self.v.shape[3], self.H, self.K
+        G = H // K
+        ql = self.q_lens.tolist() if self.q_lens is not None else [nq] * B
+        kl = self.kv_lens.tolist() if self.kv_lens is not None else [nk] * B
+        ok = torch.zeros(B, 1, 1, nq, nk, dtype=torch.bool, device="cuda")
+        for b in range(B):
+            i, j = torch.arange(ql[b], device="cuda")[:, None], torch.arange(kl[b], device="cuda")[None]
+            ok[b, 0, 0, :ql[b], :kl[b]] = (j <= i + kl[b] - ql[b]) if self.causal else True
+
+        def clean(x, lens):
+            x = x.double().clone()
+            for b in range(B):
+                x[b, :, lens[b]:] = 0
+            return x
+        q = clean(self.q, ql).reshape(B, H, 2, nq, d)
+        k = clean(self.k, kl).reshape(B, K, 2, nk, d).repeat_interleave(G, 1)
+        v = clean(self.v, kl).reshape(B, K, 1, nk, dv).repeat_interleave(G, 1)
+        x = (q @ k.transpose(-1, -2)) * self.scale
+        x = x.masked_fill(~ok, -math.inf)
+        lse = torch.logsumexp(x, -1)
+        p = torch.exp(x - lse.masked_fill(lse == -math.inf, 0.0)[..., None])
+        lam4 = self.lam.double().expand(H, 4, d)
+        e1, e2 = torch.exp((lam4[:, 0] * lam4[:, 1]).sum(-1)), torch.exp((lam4[:, 2] * lam4[:, 3]).sum(-1))
+        lam = (e1 - e2 + LAM_INIT).reshape(1, H, 1, 1)
+        om, oa = p @ v, p @ v.abs()
+        r = {"o": (om[:, :, 0] - lam * om[:, :, 1], oa[:, :, 0] + lam.abs() * oa[:, :, 1]),
+             "o2": (om[:, :, 1], oa[:, :, 1]), "lse": (lse.reshape(B, H2, nq), None)}
+        if not backward:
+            return r
+        g = clean(self.do, ql)
+        G1, Ga = (g @ v[:, :, 0].transpose(-1, -2))[:, :, None], (g.abs() @ v[:, :, 0].abs().transpose(-1, -2))[:, :, None]
+        D, Da = (g[:, :, None] * om).sum(-1, keepdim=True), (g.abs()[:, :, None] * (oa + r["o"][1][:, :, None])).sum(-1, keepdim=True)
+        sign = torch.stack([torch.ones_like(lam), -lam], 2)
+        ds, dsa = p * (G1 - D) * sign * self.scale, p * (G1.abs() + D.abs()) * sign.abs() * self.scale
+        # D is formed from outputs stored in 16 bits: a half step of each of its terms
+        dd = p * Da * sign.abs() * self.scale
+
+        def shared(t):
+            return t.reshape(B, K, G, *t.shape[2:]).sum(2)
+        r["dq"] = [(a @ b).reshape(B, H2, nq, d) for a, b in ((ds, k), (dsa + dd, k.abs()))]
+        r["dk"] = [shared(a.transpose(-1, -2) @ b).reshape(B, 2 * K, nk, d) for a, b in ((ds, q), (dsa + dd, q.abs()))]
+        r["dv"] = [shared(a.transpose(-1, -2) @ b) for a, b in ((p[:, :, 0] - lam * p[:, :, 1], g),
+                                                               (p[:, :, 0] + lam.abs() * p[:, :, 1], g.abs()))]
+        w = torch.stack([e1, -e2], 1)
+        dl, dla = -D[:, :, 1].sum((0, 2, 3)), (p[:, :, 1] * Ga[:, :, 0]).sum((0, 2, 3))
+        out = []
+        for t, f in ((dl, 1.0), (dla, -1.0)):
+            lam_t, w_t = (lam4, w) if f > 0 else (lam4.abs(), w.abs())
+            rows = (t[:, None] * w_t).repeat_interleave(2, 1)[..., None] * lam_t[:, [1, 0, 3, 2]]
+            out.append(rows if len(self.lam) == H else rows.sum(0, keepdim=True))
+        r["dlam"] = out
+        return r
+
+    def check(self, got, ref, sums):
+        """|got - ref| <= u |ref| + (2 u' + 2^-24 * sums) * sum |terms| with u
+        the half step of the type; u' is u again where probabilities may be
+        rounded to the type (16-bit types), 0 for f32 and dlam.  The scores
+        themselves: an f32 dot of d terms, exponentiated, moves p by
+        (d + 4) 2^-24 |score terms| <= 2^-16 here (|scores| < 40)."""
+        u = half_step(self.t)
+        for name, x in got.items():
+            y, terms = ref[name]
+            x = x.double()
+            if name == "lse":
+                fine = y > -math.inf
+                assert torch.equal(x == -math.inf, ~fine)
+                # f32 scores and sums: 40 * (d + 8) half steps at most
+                assert ((x - y)[fine].abs() < 2.0 ** -24 * 40 * 72).all(), (x - y)[fine].abs().max()
+                continue
+            u2 = 0.0 if self.t is torch.float32 or name == "dlam" else 2 * u
+            tol = u * y.abs() + (u2 + 2.0 ** -24 * sums + 2.0 ** -16) * terms + 1e-30
+            if self.t is torch.float16:
+                tol = tol + 2.0 ** -24
+            worst = ((x - y).abs() / tol).max().item() if x.numel() else 0.0
+            assert worst <= 1.0 and torch.isfinite(x).all(), (name, worst)
+
+
+FWD = [
+    dict(B=1, H=1, K=1, nq=1, nk=1, d=64),
+    dict(B=2, H=2, K=1, nq=5, nk=7, d=64, causal=True),
+    dict(B=1, H=2, K=2, nq=128, nk=128, d=64),
+    dict(B=2, H=2, K=1, nq=129, nk=257, d=64, causal=True),
+    dict(B=1, H=3, K=1, nq=300, nk=300, d=48, causal=True),
+    dict(B=2, H=1, K=1, nq=200, nk=100, d=32, causal=True),           # rows that see no key
+    dict(B=1, H=2, K=2, nq=64, nk=190, d=8, dv=24),
+    dict(B=4, H=2, K=1, nq=150, nk=150, d=64, causal=True, q_lens=[150, 0, 1, 77], kv_lens=[150, 0, 1, 77]),
+    dict(B=4, H=2, K=2, nq=130, nk=260, d=64, q_lens=[130, 20, 1, 128], kv_lens=[0, 260, 129, 128]),
+    dict(B=3, H=2, K=1, nq=40, nk=300, d=64, causal=True, q_lens=[40, 3, 40], kv_lens=[300, 256, 20]),
+    dict(B=1, H=2, K=1, nq=70, nk=70, d=100, dv=200, causal=True),    # wide head
+    dict(B=1, H=1, K=1, nq=33, nk=65, d=13, dv=7),                    # odd dims
+    dict(B=1, H=2, K=1, nq=33, nk=65, d=64, heads_inner=False, lam_rows=1),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("case", range(len(FWD)))
+def test_diff_attention_forward(nn, dtype, case):
+    c = Case(dtype=dtype, **FWD[case])
+    o, lse, o2 = c.fwd(nn)
+    c.check({"o": o, "lse": lse, "o2": o2}, c.reference(), c.k.shape[2])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("case", range(len(FWD)))
+def test_diff_attention_gradients(nn, dtype, case):
+    c = Case(dtype=dtype, **FWD[case])
+    got = c.bwd(nn, *c.fwd(nn))
+    c.check(got, c.reference(backward=True), max(c.k.shape[2], c.q.shape[2] * c.H // c.K))
+    again = c.bwd(nn, *c.fwd(nn))
+    assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_diff_attention_ignores_what_is_behind_the_lengths(nn, dtype):
+    """NaN and infinities behind the lengths change nothing."""
+    def make():
+        return Case(B=3, H=2, K=1, nq=140, nk=140, d=64, dtype=dtype, causal=True, q_lens=[140, 65, 0],
+                    kv_lens=[140, 65, 0])
+    c, e = make(), make()
+    for x in (e.q, e.k, e.v, e.do):
+        x[1, :, 65:] = math.nan
+        x[2] = math.inf
+    a, b = c.fwd(nn), e.fwd(nn)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    ga, gb = c.bwd(nn, *a), e.bwd(nn, *b)
+    assert all(torch.equal(ga[n], gb[n]) for n in ga)
+    assert ga["dk"][2].abs().max() == 0 and ga["dq"][1, :, 65:].abs().max() == 0
+
+
+def test_diff_attention_gradients_by_differences(nn):
+    """f32: (f(x + h v) - f(x - h v)) / 2h of f = <o, do> against <grad, v>, for each input."""
+    c = Case(B=1, H=2, K=1, nq=12, nk=15, d=16, dtype="f32", causal=True, heads_inner=False)
+    g = c.bwd(nn, *c.fwd(nn))
+    h = 2.0 ** -7
+    for name, x in (("dq", c.q), ("dk", c.k), ("dv", c.v), ("dlam", c.lam)):
+        v = randn(x.shape, 99, torch.float32)
+        v = v / v.norm()
+        x0 = x.clone()
+        f = []
+        for s in (h, -h):
+            x.copy_(x0 + s * v)
+            f.append((c.fwd(nn)[0].double() * c.do).sum().item())
+        x.copy_(x0)
+        # third derivatives along a unit direction are below 60 here, so h^2/6 of them is below 1e-3;
+        # f itself is a sum of 768 f32 values, 1e-5 over 2h
+        assert abs((f[0] - f[1]) / (2 * h) - (g[name].double() * v).sum().item()) < 2e-3, name
+
+
+# ---------------------------------------------------------------------------- AdamW
+def adamw_ref(p, g, m, v, t, lr, b1, b2, eps, wd):
+    """p, m, v after the step, and how far f32 may take p: every operation
+    rounds once (a half step, 2^-24 of its result), and the errors are linear
+    in the terms.  p keep: keep and the product, and the difference, 3 of |p|
+    and 1 of the step (counted in the 4 and 16 below).  The step is
+    rate * (m / (u / root + eps)): m has 3 of its terms b1 |m| and (1-b1) |g|
+    (constant, product, sum); v has 4 of itself, so u = sqrt(v) 2 + 1; u / root
+    2 more, + eps 1, the quotient 1, rate 1 and the product 1: 12 of the step
+    formed with |terms| for m, which near cancellation in m exceeds the step
+    itself."""
+    terms = m.abs() * b1 + g.abs() * (1 - b1)
+    m = m * b1 + g * (1 - b1)
+    v = v * b2 + g * g * (1 - b2)
+    f = lr / (1 - b1 ** t) / ((v / (1 - b2 ** t)).sqrt() + eps)
+    q = p * (1 - lr * wd) - f * m
+    return q, m, v, 2.0 ** -24 * (4 * (p.abs() + q.abs()) + 16 * f * terms)
+
+
+SIZES = [1, 255, 256, 257, 4096, 4097, 0, 100003]
+HYPER = dict(lr=3e-3, beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.1)
+
+
+def make_tensors(sizes, dtype, seed, scale, shift=0):
+    """Tensors of one flat buffer; `shift` elements off its alignment."""
+    flat = randn((sum(sizes) + 4 * len(sizes) + shift,), seed, dtype, scale)
+    out, at = [], shift
+    for n in sizes:
+        out.append(flat[at:at + n])
+        at += n if shift else -(-n // 4) * 4
+    return out
+
+
+@pytest.mark.parametrize("p_type,g_type,masters", [("f32", "f32", False), ("bf16", "bf16", True), ("f16", "f32", True),
+                                                   ("bf16", "bf16", False), ("f32", "f16", False)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_adamw_32(nn, p_type, g_type, masters, shift):
+    t = TYPES[p_type]
+    p, g = make_tensors(SIZES, t, 1, 1.0, shift), make_tensors(SIZES, TYPES[g_type], 2, 1e-2, shift)
+    w = [x.float() for x in p] if masters else None
+    m = make_tensors(SIZES, torch.float32, 3, 1e-2, shift)
+    v = [x.square_() for x in make_tensors(SIZES, torch.float32, 4, 1e-2, shift)]
+    state = torch.tensor([6, 0], device="cuda")
+    a = (0.9, 0.99, 1e-8, 0.1)
+    ref = [adamw_ref((w or p)[i].double(), g[i].double(), m[i].double(), v[i].double(), 7, 3e-3, *a) for i in range(len(p))]
+    nn.AdamW(p, g, m, v, state, masters=w, **HYPER).step()
+    assert state.tolist() == [7, 0]
+    for i in range(len(p)):
+        pr, mr, vr, tol = ref[i]
+        gd = g[i].double()
+        # three roundings of each term of m, four of v
+        assert ((m[i] - mr).abs() <= 3 * 2.0 ** -24 * (mr.abs() + 2 * gd.abs())).all()
+        assert ((v[i] - vr).abs() <= 4 * 2.0 ** -24 * vr.abs() + 1e-37).all()
+        if masters:
+            assert ((w[i] - pr).abs() <= tol).all()
+            assert torch.equal(p[i], w[i].to(t))
+        else:
+            assert ((p[i].double() - pr).abs() <= tol + half_step(t) * pr.abs() * (t is not torch.float32)).all()
+
+
+def mix(n, tensor, t):
+    low = 0xFFFFFFFF
+    x = (torch.arange(n, device="cuda") * 0x9E3779B1 + t * 0x85EBCA77 + tensor * 0xC2B2AE3D) & low
+    x = ((x ^ (x >> 16)) * 0x7FEB352D) & low
+    x = ((x ^ (x >> 15)) * 0x846CA68B) & low
+    return x ^ (x >> 16)
+
+
+E4M3 = sorted({(k / 512 if k < 8 else (8 + k % 8) / 8 * 2.0 ** (k // 8 - 7)) for k in range(127)})
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+def test_adamw_8bit(nn, shift):
+    """Each code is one of the two neighbours of the exact 64-bit value, the
+    upper with the probability of the remainder by the same random bits; three
+    steps, from zero states."""
+    grid = torch.tensor(E4M3, dtype=torch.float64, device="cuda")
+    p = make_tensors(SIZES, torch.float32, 1, 1.0, shift)
+    m = [x.zero_() for x in make_tensors(SIZES, torch.float32, 3, 1.0, shift)]
+    m = [torch.zeros(x.numel() + shift, dtype=torch.float8_e4m3fn, device="cuda")[shift:] for x in m]
+    v = [torch.zeros_like(x) for x in m]
+    ms, vs = ([torch.zeros(-(-n // 256), device="cuda") for n in SIZES] for _ in range(2))
+    state = torch.tensor([0, 0], device="cuda")
+    g = make_tensors(SIZES, torch.float32, 2, 1e-2, shift)
+    opt = nn.AdamW(p, g, m, v, state, m_scales=ms, v_scales=vs, **HYPER)
+    for t in (1, 2, 3):
+        for i, x in enumerate(g):
+            x.copy_(randn(x.shape, 10 * t + i, torch.float32, 1e-2))
+        old = []
+        for i, n in enumerate(SIZES):
+            sm, sv = (s[i].double().repeat_interleave(256)[:n] for s in (ms, vs))
+            old.append((p[i].double(), g[i].double(), m[i].double() * sm, (v[i].double() * sv) ** 2))
+        opt.step()
+        assert state.tolist() == [t, 0]
+        for i, n in enumerate(SIZES):
+            if not n:
+                continue
+            pr, mr, vr, tol = adamw_ref(*old[i], t, 3e-3, 0.9, 0.99, 1e-8, 0.1)
+            assert ((p[i] - pr).abs() <= tol).all()
+            r = mix(n, i, t)
+            for code, scale, x, rnd, least in ((m[i], ms[i], mr, r & 0xFFFFF, False), (v[i], vs[i], vr.sqrt(), r >> 12, True)):
+                pad = torch.cat([x.abs(), x.new_zeros(-n % 256)]).view(-1, 256).amax(1)
+                assert ((scale.double() * 448 - pad).abs() <= 8 * 2.0 ** -24 * pad).all()
+                a = x.abs() / (pad / 448).repeat_interleave(256)[:n]
+                at = torch.searchsorted(grid, a.clamp(max=448.0), right=True) - 1
+                lo, hi = grid[at], grid[(at + 1).clamp(max=126)]
+                got = code.double().abs()
+                # a is right to 16 half steps: a value that close to a code may fall to either side of it
+                near = 16 * 2.0 ** -24 * a
+                ok = ((got == lo) | (got == hi) | ((got - a).abs() <= near) |
+                      ((got < lo) & (a - lo <= near)) | ((got > hi) & (hi - a <= near)))
+                if least:
+                    ok |= (got == 2.0 ** -9) & (a < 2.0 ** -9)
+                assert ok.all()
+                # the random bits decide: up where remainder + bits reach a whole step
+                up = (a - lo) / (hi - lo).clamp(min=1e-30) + rnd.double() * 2.0 ** -20
+                sure = ((up - 1).abs() > 2.0 ** -12) & (a < 448) & (a > 2.0 ** -9)
+                assert torch.equal(got[sure], torch.where(up >= 1, hi, lo)[sure])
+                assert ((code.double() < 0) <= (x < 0)).all()
+
+
+def test_adamw_more_tensors_than_one_launch_holds(nn):
+    sizes = [37 + i % 5 for i in range(600)]
+    p = make_tensors(sizes, torch.float32, 1, 1.0)
+    g, m, v = (make_tensors(sizes, torch.float32, s, 1e-2) for s in (2, 3, 4))
+    v = [x.square_() for x in v]
+    state = torch.tensor([0, 0], device="cuda")
+    ref = [adamw_ref(p[i].double(), g[i].double(), m[i].double(), v[i].double(), 1, 3e-3, 0.9, 0.99, 1e-8, 0.1)
+           for i in range(600)]
+    nn.AdamW(p, g, m, v, state, **HYPER).step()
+    assert state.tolist() == [1, 0]
+    assert all(((p[i] - ref[i][0]).abs() <= ref[i][3]).all() for i in range(600))
+    empty = torch.tensor([4, 0], device="cuda")
+    nn.AdamW([], [], [], [], empty).step()
+    assert empty.tolist() == [5, 0]
