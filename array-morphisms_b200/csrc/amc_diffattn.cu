@@ -499,6 +499,8 @@ int check_sizes(const amc_diff_attention* p, const char* who) {
     return fail(AMC_ERR_INVALID, std::string(who) + ": head dims d 1..128, dv 1..256");
   if (p->batch > 65535 || p->heads > 32767 || p->nq > (1 << 30) || p->nk > (1 << 30))
     return fail(AMC_ERR_INVALID, std::string(who) + ": batch up to 65535, heads up to 32767, rows up to 2^30");
+  if (!std::isfinite(p->scale) || !std::isfinite(p->lam_init))
+    return fail(AMC_ERR_INVALID, std::string(who) + ": scale and lam_init must be finite");
   if (p->lam_rows != 1 && p->lam_rows != p->heads)
     return fail(AMC_ERR_INVALID, std::string(who) + ": lam has 1 row or one for each head");
   return AMC_OK;
@@ -539,7 +541,11 @@ int amc_diff_attention_fwd(const amc_diff_attention* p, void* stream) {
     return fail(AMC_ERR_INVALID, "amc_diff_attention_fwd: null tensor");
   if (int rc = check_workspace(p, fwd_bytes(*p), "amc_diff_attention_fwd")) return rc;
   if (fault_injected("launch")) return fail(AMC_ERR_INJECTED, "diff_attention: injected launch failure (AMC_FAULT=launch)");
-  return launch_diff_fwd_simt(*p, pick_stream(stream));
+  cudaStream_t s = pick_stream(stream);
+  bool handled = false;
+  if (int rc = diff_fwd_tc(*p, s, &handled)) return rc;
+  if (handled) return AMC_OK;
+  return launch_diff_fwd_simt(*p, s);
 }
 
 int amc_diff_attention_bwd(const amc_diff_attention* p, void* stream) {

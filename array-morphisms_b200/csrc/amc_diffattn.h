@@ -42,6 +42,10 @@ inline size_t diff_partials(const amc_diff_attention& p) {
   return (size_t)p.batch * p.heads * ((p.nq + kDiffTile - 1) / kDiffTile);
 }
 
+// Tensor-core forward; *handled = false (and nothing launched) for other
+// types, shapes and alignments.
+bool diff_tc_shape(const amc_diff_attention& p);
+int diff_fwd_tc(const amc_diff_attention& p, cudaStream_t s, bool* handled);
 int launch_diff_fwd_simt(const amc_diff_attention& p, cudaStream_t s);
 int launch_diff_bwd_simt(const amc_diff_attention& p, DiffRow* rows, float* partials, cudaStream_t s);
 int launch_diff_bwd_rows(const amc_diff_attention& p, DiffRow* rows, cudaStream_t s);

@@ -298,6 +298,7 @@ int conv_check_error();
 int rowpass_check_error();
 int colfold_check_error();
 int dist_check_error();
+int diff_check_error();
 int device_check_errors();  // all kernels' bounded-wait flags
 
 }  // namespace amc

@@ -62,6 +62,12 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
       ::"r"(smem_addr(dst)), "l"((uint64_t)map), "r"(x), "r"(y), "r"(smem_addr(bar)) : "memory");
 }
+// Box of a 4-D map (dim, row, head, batch).
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(smem_addr(dst)), "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar)) : "memory");
+}
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // 1-D bulk copy global -> shared (both 16-byte aligned, bytes a multiple of 16),
 // counted on `bar` (the caller posts the expected bytes).  No multicast.
@@ -110,6 +116,21 @@ __device__ __forceinline__ void mma_tf32_ts(uint32_t d_tmem, uint32_t a_tmem, ui
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+}
+// The same two for 16-bit operands (kind::f16, K=16 per product): A and B both
+// bf16 or both fp16, two neighbouring K elements per 32-bit column when A is
+// in tensor memory.
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
 }
 // The mbarrier gets one arrival when all prior tcgen05 ops of this thread complete.
@@ -250,6 +271,16 @@ __device__ __forceinline__ uint64_t sdesc_mn(uint32_t saddr, uint32_t mn_atom_by
   return d;
 }
 
+// Shared-memory descriptor of an MN-major 16-bit operand, 128-byte swizzle:
+// rows of 128 bytes run along K, each holding 64 consecutive M/N elements, so
+// the tile that a K-major descriptor reads as rows of N serves as it is when
+// the contraction runs down those rows.  `mn_block_bytes` is the distance of
+// successive 64-element M/N blocks (LBO); 8-row K groups are 1024 bytes apart
+// (SBO), a K step of 16 is 2048 bytes.
+__device__ __forceinline__ uint64_t sdesc_mn16(uint32_t saddr, uint32_t mn_block_bytes) {
+  return sdesc(saddr, mn_block_bytes, 1024);
+}
+
 // Byte offset of K step k (8 tf32 = 32 bytes) in a K-major operand stored as
 // 32-column (128-byte) regions of region_bytes each.
 __host__ __device__ constexpr uint32_t kstep_off(int k, int region_bytes) {
@@ -272,8 +303,24 @@ __host__ __device__ constexpr uint32_t idesc_tf32(int M, int N, bool a_mn_major,
          | ((uint32_t)(M >> 4) << 24);
 }
 
+// Instruction descriptor for kind::f16 with f32 accumulation; bf16 or fp16 operands.
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool bf16, bool a_mn_major, bool b_mn_major) {
+  return (1u << 4)                        // D format f32
+         | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10)
+         | ((a_mn_major ? 1u : 0u) << 15)
+         | ((b_mn_major ? 1u : 0u) << 16)
+         | ((uint32_t)(N >> 3) << 17)
+         | ((uint32_t)(M >> 4) << 24);
+}
+
 }  // namespace tc
 
+// Host: a map of a 16-bit (batch, heads, rows, dim) tensor with element
+// strides over batch, head and row: boxes of box_rows rows x 64 elements in
+// the 128-byte swizzle; what lies outside the tensor reads as zero.
+// AMC_ERR_UNSUPPORTED (no message) when such a map cannot hold it.
+int make_tmap_4d_16(CUtensorMap* map, const void* base, bool bf16, int64_t batch, int64_t heads, int64_t rows,
+                    int64_t dim, const int64_t strides[3], uint32_t box_rows);
 // Host: encode a 2-D f32 tensor map (rows x cols, row pitch in elements) with
 // a (32 x box_rows) box and 128-byte swizzle, through the driver entry point.
 int make_tmap_2d_f32(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch_elems,
