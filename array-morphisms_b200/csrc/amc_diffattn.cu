@@ -216,43 +216,46 @@ __global__ void __launch_bounds__(256, 1) k_diff_fwd_simt(const __grid_constant_
   if (p.o2) store_rows<T, R, DV / 16>((T*)p.o2 + b * p.o2s[0] + h * p.o2s[1], p.o2s[2], o[1], 1.f, r0, p.nq, p.dv, ty, tx);
 }
 
-// One warp per row: DiffRow from lse, o, o2 and dO.
+// One warp per row: lse2 and dsum from lse, o, o2 and dO; lam of every head.
 template <typename T>
 __global__ void __launch_bounds__(256) k_diff_bwd_rows(const __grid_constant__ amc_diff_attention p,
-                                                       DiffRow* __restrict__ rows) {
+                                                       const __grid_constant__ DiffBwdWork w) {
   const int lane = threadIdx.x & 31;
   const int i = blockIdx.x * 8 + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
   if (i >= p.nq) return;
+  const float lam = lam_of<T>(p, h);
+  if (i == 0 && b == 0 && lane == 0) w.lam[h] = lam;
   const DiffLens len = diff_lens(p, b);
-  DiffRow r{INFINITY, 0.f, INFINITY, 0.f};
+  float2 e = make_float2(INFINITY, INFINITY), r = make_float2(0.f, 0.f);
   if (diff_limit(len, p.causal, i) > 0) {
     const T* o = (const T*)p.o + b * p.os[0] + h * p.os[1] + (int64_t)i * p.os[2];
     const T* o2 = (const T*)p.o2 + b * p.o2s[0] + h * p.o2s[1] + (int64_t)i * p.o2s[2];
     const T* go = (const T*)p.d_o + b * p.dos[0] + h * p.dos[1] + (int64_t)i * p.dos[2];
-    const float lam = lam_of<T>(p, h);
     float d = 0.f, d2 = 0.f;
     for (int c = lane; c < p.dv; c += 32) {
       const float x = to_f32(go[c]);
       d = fmaf(x, to_f32(o[c]), d);
       d2 = fmaf(x, to_f32(o2[c]), d2);
     }
-    for (int w = 16; w > 0; w >>= 1) {
-      d += __shfl_xor_sync(0xffffffffu, d, w);
-      d2 += __shfl_xor_sync(0xffffffffu, d2, w);
+    for (int s = 16; s > 0; s >>= 1) {
+      d += __shfl_xor_sync(0xffffffffu, d, s);
+      d2 += __shfl_xor_sync(0xffffffffu, d2, s);
     }
     const float* lse = p.lse + ((int64_t)b * 2 * p.heads + 2 * h) * p.nq + i;
-    r.lse1 = lse[0] * kLog2e;
-    r.lse2 = lse[p.nq] * kLog2e;
-    r.d1 = fmaf(lam, d2, d);   // dO . O_1 = dO . (O + lam O_2)
-    r.d2 = d2;
+    e = make_float2(lse[0] * kLog2e, lse[p.nq] * kLog2e);
+    r = make_float2(fmaf(lam, d2, d), d2);   // dO . O_1 = dO . (O + lam O_2)
   }
-  if (lane == 0) rows[((int64_t)b * p.heads + h) * p.nq + i] = r;
+  if (lane == 0) {
+    const int64_t at = ((int64_t)b * p.heads + h) * w.pitch + i;
+    w.lse2[at] = e;
+    w.dsum[at] = r;
+  }
 }
 
 // dK, dV of TT keys of one key head: streams the rows of its query heads.
 template <typename T, int TT, int DM, int DV>
 __global__ void __launch_bounds__(256, 1) k_diff_dkv_simt(const __grid_constant__ amc_diff_attention p,
-                                                          const DiffRow* __restrict__ rows) {
+                                                          const __grid_constant__ DiffBwdWork wk) {
   using L = Tile<TT, DM, DV>;
   constexpr int R = L::R;
   extern __shared__ float diff_sm[];
@@ -270,7 +273,7 @@ __global__ void __launch_bounds__(256, 1) k_diff_dkv_simt(const __grid_constant_
   float dk[2][R][DM / 16] = {}, dv[R][DV / 16] = {};
   const int first = diff_first_row(len, p.causal, k0) / TT * TT;
   for (int h = g * group; h < (g + 1) * group; ++h) {
-    const float lam = lam_of<T>(p, h);
+    const float lam = wk.lam[h];
     for (int r0 = first; r0 < len.nq; r0 += TT) {
       __syncthreads();
       for (int m = 0; m < 2; ++m)
@@ -288,13 +291,15 @@ __global__ void __launch_bounds__(256, 1) k_diff_dkv_simt(const __grid_constant_
         for (int i = 0; i < R; ++i) {
           const int r = r0 + ty + 16 * i;
           const int lim = diff_limit(len, p.causal, r);
-          const DiffRow e = lim > 0 ? rows[((int64_t)b * p.heads + h) * p.nq + r] : DiffRow{INFINITY, 0.f, INFINITY, 0.f};
+          const int64_t at = ((int64_t)b * p.heads + h) * wk.pitch + r;
+          const float2 e = lim > 0 ? wk.lse2[at] : make_float2(INFINITY, INFINITY);
+          const float2 ds = lim > 0 ? wk.dsum[at] : make_float2(0.f, 0.f);
 #pragma unroll
           for (int j = 0; j < R; ++j) {
-            const float pr = k0 + tx + 16 * j < lim ? exp2f(fmaf(s[i][j], c2, -(m ? e.lse2 : e.lse1))) : 0.f;
+            const float pr = k0 + tx + 16 * j < lim ? exp2f(fmaf(s[i][j], c2, -(m ? e.y : e.x))) : 0.f;
             const float w = m ? -lam * pr : pr;
             both[i][j] = m ? both[i][j] + w : w;
-            sS[m * TT * L::PP + (ty + 16 * i) * L::PP + tx + 16 * j] = w * (gv[i][j] - (m ? e.d2 : e.d1));
+            sS[m * TT * L::PP + (ty + 16 * i) * L::PP + tx + 16 * j] = w * (gv[i][j] - (m ? ds.y : ds.x));
           }
         }
       }
@@ -318,8 +323,7 @@ __global__ void __launch_bounds__(256, 1) k_diff_dkv_simt(const __grid_constant_
 // dQ of TT rows, and this tile's part of sum P_2 G.
 template <typename T, int TT, int DM, int DV>
 __global__ void __launch_bounds__(256, 1) k_diff_dq_simt(const __grid_constant__ amc_diff_attention p,
-                                                         const DiffRow* __restrict__ rows,
-                                                         float* __restrict__ partials) {
+                                                         const __grid_constant__ DiffBwdWork wk) {
   using L = Tile<TT, DM, DV>;
   constexpr int R = L::R;
   extern __shared__ float diff_sm[];
@@ -329,7 +333,7 @@ __global__ void __launch_bounds__(256, 1) k_diff_dq_simt(const __grid_constant__
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int r0 = blockIdx.x * TT, h = blockIdx.y, b = blockIdx.z, g = h / (p.heads / p.kv_heads);
   const DiffLens len = diff_lens(p, b);
-  const float lam = lam_of<T>(p, h);
+  const float lam = wk.lam[h];
   const float c2 = p.scale * kLog2e;
   const int dim4 = (p.d + 3) & ~3, dimv4 = (p.dv + 3) & ~3;
   for (int m = 0; m < 2; ++m)
@@ -337,12 +341,14 @@ __global__ void __launch_bounds__(256, 1) k_diff_dq_simt(const __grid_constant__
                                 len.nq, p.d);
   load_tile<T, TT, DV, L::PV>(sG, (const T*)p.d_o + b * p.dos[0] + h * p.dos[1], p.dos[2], r0, len.nq, p.dv);
   int lim[R];
-  DiffRow e[R];
+  float2 e[R], ds[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int r = r0 + ty + 16 * i;
     lim[i] = diff_limit(len, p.causal, r);
-    e[i] = lim[i] > 0 ? rows[((int64_t)b * p.heads + h) * p.nq + r] : DiffRow{INFINITY, 0.f, INFINITY, 0.f};
+    const int64_t at = ((int64_t)b * p.heads + h) * wk.pitch + r;
+    e[i] = lim[i] > 0 ? wk.lse2[at] : make_float2(INFINITY, INFINITY);
+    ds[i] = lim[i] > 0 ? wk.dsum[at] : make_float2(0.f, 0.f);
   }
   float dq[2][R][DM / 16] = {}, pg = 0.f;
   const int last = min(r0 + TT, len.nq) - 1;
@@ -364,10 +370,10 @@ __global__ void __launch_bounds__(256, 1) k_diff_dq_simt(const __grid_constant__
       for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-          const float pr = k0 + tx + 16 * j < lim[i] ? exp2f(fmaf(s[i][j], c2, -(m ? e[i].lse2 : e[i].lse1))) : 0.f;
+          const float pr = k0 + tx + 16 * j < lim[i] ? exp2f(fmaf(s[i][j], c2, -(m ? e[i].y : e[i].x))) : 0.f;
           if (m) part = fmaf(pr, gv[i][j], part);
           sS[m * TT * L::PP + (ty + 16 * i) * L::PP + tx + 16 * j] =
-              (m ? -lam * pr : pr) * (gv[i][j] - (m ? e[i].d2 : e[i].d1));
+              (m ? -lam * pr : pr) * (gv[i][j] - (m ? ds[i].y : ds[i].x));
         }
     }
     pg += part;
@@ -385,7 +391,7 @@ __global__ void __launch_bounds__(256, 1) k_diff_dq_simt(const __grid_constant__
   if (threadIdx.x == 0) {
     float t = 0.f;
     for (int w = 0; w < 8; ++w) t += red[w];
-    partials[((int64_t)h * p.batch + b) * gridDim.x + blockIdx.x] = t;
+    wk.partials[((int64_t)h * p.batch + b) * gridDim.x + blockIdx.x] = t;
   }
 }
 
@@ -436,21 +442,21 @@ int fwd_simt(const amc_diff_attention& p, cudaStream_t s) {
 }
 
 template <typename T, int TT, int DM, int DV>
-int bwd_simt(const amc_diff_attention& p, DiffRow* rows, float* partials, cudaStream_t s) {
+int bwd_simt(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s) {
   static std::atomic<uint64_t> attr_dkv{0}, attr_dq{0};
   using L = Tile<TT, DM, DV>;
   if (int rc = smem_attr_once(k_diff_dkv_simt<T, TT, DM, DV>, L::dkv, attr_dkv)) return rc;
   if (int rc = smem_attr_once(k_diff_dq_simt<T, TT, DM, DV>, L::dq, attr_dq)) return rc;
   if (p.nk) {
-    k_diff_dkv_simt<T, TT, DM, DV><<<dim3((p.nk + TT - 1) / TT, p.kv_heads, p.batch), 256, L::dkv, s>>>(p, rows);
+    k_diff_dkv_simt<T, TT, DM, DV><<<dim3((p.nk + TT - 1) / TT, p.kv_heads, p.batch), 256, L::dkv, s>>>(p, w);
     AMC_CUDA(cudaGetLastError());
   }
   const int tiles = (p.nq + TT - 1) / TT;
   if (p.nq) {
-    k_diff_dq_simt<T, TT, DM, DV><<<dim3(tiles, p.heads, p.batch), 256, L::dq, s>>>(p, rows, partials);
+    k_diff_dq_simt<T, TT, DM, DV><<<dim3(tiles, p.heads, p.batch), 256, L::dq, s>>>(p, w);
     AMC_CUDA(cudaGetLastError());
   }
-  return launch_diff_dlam(p, partials, tiles, s);
+  return launch_diff_dlam(p, w, tiles, s);
 }
 
 }  // namespace
@@ -462,26 +468,25 @@ int launch_diff_fwd_simt(const amc_diff_attention& p, cudaStream_t s) {
   });
 }
 
-int launch_diff_bwd_rows(const amc_diff_attention& p, DiffRow* rows, cudaStream_t s) {
+int launch_diff_bwd_rows(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s) {
   if (!p.nq) return AMC_OK;
   return by_type(p.dtype, [&](auto t) {
-    k_diff_bwd_rows<decltype(t)><<<dim3((p.nq + 7) / 8, p.heads, p.batch), 256, 0, s>>>(p, rows);
+    k_diff_bwd_rows<decltype(t)><<<dim3((p.nq + 7) / 8, p.heads, p.batch), 256, 0, s>>>(p, w);
     AMC_CUDA(cudaGetLastError());
     return AMC_OK;
   });
 }
 
-int launch_diff_bwd_simt(const amc_diff_attention& p, DiffRow* rows, float* partials, cudaStream_t s) {
+int launch_diff_bwd_simt(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s) {
   return by_type(p.dtype, [&](auto t) {
     using T = decltype(t);
-    return p.d <= 64 && p.dv <= 128 ? bwd_simt<T, 64, 64, 128>(p, rows, partials, s)
-                                    : bwd_simt<T, 32, 128, 256>(p, rows, partials, s);
+    return p.d <= 64 && p.dv <= 128 ? bwd_simt<T, 64, 64, 128>(p, w, s) : bwd_simt<T, 32, 128, 256>(p, w, s);
   });
 }
 
-int launch_diff_dlam(const amc_diff_attention& p, const float* partials, int tiles, cudaStream_t s) {
+int launch_diff_dlam(const amc_diff_attention& p, const DiffBwdWork& w, int tiles, cudaStream_t s) {
   return by_type(p.dtype, [&](auto t) {
-    k_diff_dlam<decltype(t)><<<p.lam_rows, 256, 0, s>>>(p, partials, (int64_t)p.batch * tiles);
+    k_diff_dlam<decltype(t)><<<p.lam_rows, 256, 0, s>>>(p, w.partials, (int64_t)p.batch * tiles);
     AMC_CUDA(cudaGetLastError());
     return AMC_OK;
   });
@@ -507,7 +512,6 @@ int check_sizes(const amc_diff_attention* p, const char* who) {
 }
 
 size_t fwd_bytes(const amc_diff_attention&) { return 0; }
-size_t bwd_bytes(const amc_diff_attention& p) { return diff_rows_bytes(p) + diff_partials(p) * sizeof(float); }
 
 int check_workspace(const amc_diff_attention* p, size_t need, const char* who) {
   if (!need) return AMC_OK;
@@ -529,7 +533,7 @@ int amc_diff_attention_workspace(const amc_diff_attention* p, int32_t backward, 
   if (!bytes) return fail(AMC_ERR_INVALID, "amc_diff_attention_workspace: null out");
   if (int rc = check_sizes(p, "amc_diff_attention_workspace")) return rc;
   size_t n = fwd_bytes(*p);
-  if (backward && bwd_bytes(*p) > n) n = bwd_bytes(*p);
+  if (backward && diff_bwd_bytes(*p) > n) n = diff_bwd_bytes(*p);
   *bytes = (int64_t)n;
   return AMC_OK;
 }
@@ -554,14 +558,16 @@ int amc_diff_attention_bwd(const amc_diff_attention* p, void* stream) {
   if (p->batch && ((p->nq && (!p->q || !p->o || !p->o2 || !p->lse || !p->d_o || !p->dq)) ||
                    (p->nk && (!p->k || !p->v || !p->dk || !p->dv_))))
     return fail(AMC_ERR_INVALID, "amc_diff_attention_bwd: null tensor");
-  if (int rc = check_workspace(p, bwd_bytes(*p), "amc_diff_attention_bwd")) return rc;
+  if (int rc = check_workspace(p, diff_bwd_bytes(*p), "amc_diff_attention_bwd")) return rc;
   if (fault_injected("launch")) return fail(AMC_ERR_INJECTED, "diff_attention: injected launch failure (AMC_FAULT=launch)");
   cudaStream_t s = pick_stream(stream);
-  DiffRow* rows = (DiffRow*)p->workspace;
-  float* partials = (float*)((char*)p->workspace + diff_rows_bytes(*p));
-  if (!p->batch) return launch_diff_dlam(*p, partials, 0, s);
-  if (int rc = launch_diff_bwd_rows(*p, rows, s)) return rc;
-  return launch_diff_bwd_simt(*p, rows, partials, s);
+  const DiffBwdWork w = diff_bwd_work(*p);
+  if (!p->batch) return launch_diff_dlam(*p, w, 0, s);
+  if (int rc = launch_diff_bwd_rows(*p, w, s)) return rc;
+  bool handled = false;
+  if (int rc = diff_bwd_tc(*p, w, s, &handled)) return rc;
+  if (handled) return AMC_OK;
+  return launch_diff_bwd_simt(*p, w, s);
 }
 
 }  // extern "C"

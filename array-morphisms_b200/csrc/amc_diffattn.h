@@ -26,20 +26,36 @@ __device__ __forceinline__ int diff_first_row(const DiffLens& l, int causal, int
   return causal ? min(l.nq, max(0, j - (l.nk - l.nq))) : 0;
 }
 
-// Per (batch, head, row) of the backward: both maps' lse * log2 e (+inf where
-// the row is empty, so that exp2(s - lse) is 0) and D = rowsum(dO * O_m).
-struct DiffRow {
-  float lse1, d1, lse2, d2;
-};
-
-// Workspace of the backward: DiffRow rows, then one partial of dlam per
-// (head, batch, row tile of kDiffTile).
+// Workspace of the backward.  Per (batch, head, row) the pairs
+//   lse2 = both maps' lse * log2 e, +inf where the row is empty, so that
+//          exp2(s - lse) is 0
+//   dsum = D_m = rowsum(dO * O_m) of both maps
+// (rows padded to a multiple of 4, so that a tile of them is a bulk copy),
+// then lam of every head, then one partial of sum P_2 G for every (head,
+// batch, row tile).
 constexpr int kDiffTile = 32;
-inline size_t diff_rows_bytes(const amc_diff_attention& p) {
-  return (size_t)p.batch * p.heads * p.nq * sizeof(DiffRow);
+struct DiffBwdWork {
+  float2* lse2;
+  float2* dsum;
+  float* lam;
+  float* partials;
+  int pitch;
+};
+inline int diff_row_pitch(const amc_diff_attention& p) { return (p.nq + 3) & ~3; }
+inline size_t diff_bwd_bytes(const amc_diff_attention& p) {
+  const size_t rows = (size_t)p.batch * p.heads * diff_row_pitch(p);
+  const size_t partials = (size_t)p.batch * p.heads * ((p.nq + kDiffTile - 1) / kDiffTile);
+  return 2 * rows * sizeof(float2) + (size_t)p.heads * sizeof(float) + partials * sizeof(float);
 }
-inline size_t diff_partials(const amc_diff_attention& p) {
-  return (size_t)p.batch * p.heads * ((p.nq + kDiffTile - 1) / kDiffTile);
+inline DiffBwdWork diff_bwd_work(const amc_diff_attention& p) {
+  const size_t rows = (size_t)p.batch * p.heads * diff_row_pitch(p);
+  DiffBwdWork w;
+  w.lse2 = (float2*)p.workspace;
+  w.dsum = w.lse2 + rows;
+  w.lam = (float*)(w.dsum + rows);
+  w.partials = w.lam + p.heads;
+  w.pitch = diff_row_pitch(p);
+  return w;
 }
 
 // Tensor-core forward; *handled = false (and nothing launched) for other
@@ -47,9 +63,11 @@ inline size_t diff_partials(const amc_diff_attention& p) {
 bool diff_tc_shape(const amc_diff_attention& p);
 int diff_fwd_tc(const amc_diff_attention& p, cudaStream_t s, bool* handled);
 int launch_diff_fwd_simt(const amc_diff_attention& p, cudaStream_t s);
-int launch_diff_bwd_simt(const amc_diff_attention& p, DiffRow* rows, float* partials, cudaStream_t s);
-int launch_diff_bwd_rows(const amc_diff_attention& p, DiffRow* rows, cudaStream_t s);
+int launch_diff_bwd_rows(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s);
+int launch_diff_bwd_simt(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s);
+// Tensor-core gradients (after the rows), likewise.
+int diff_bwd_tc(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s, bool* handled);
 // tiles: partials per (head, batch)
-int launch_diff_dlam(const amc_diff_attention& p, const float* partials, int tiles, cudaStream_t s);
+int launch_diff_dlam(const amc_diff_attention& p, const DiffBwdWork& w, int tiles, cudaStream_t s);
 
 }  // namespace amc

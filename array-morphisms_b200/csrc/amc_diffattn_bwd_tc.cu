@@ -1,0 +1,630 @@
+// Differential attention gradients on the tensor cores (sm_100a, tcgen05
+// kind::f16), 16-bit tensors with d <= 64 and dv <= 128, both multiples of 8:
+//   P_m = 2^(scale log2e Q_m K_m^T - lse2_m)      G = dO V^T
+//   dS_1 = P_1 (G - D_1)                          dS_2 = lam P_2 (D_2 - G)
+//   dV = (P_1 - lam P_2)^T dO   dK_m = scale dS_m^T Q_m   dQ_m = scale dS_m K_m
+// Both maps share G, and the difference of the maps is taken before dV's
+// product, so a (row, key) pair costs 16 d + 12 d operations in two kernels
+// against 20 d were dQ added up across CTAs; without atomics the results are
+// the same at every call.
+//   k_diff_dkv_tc  one CTA per 128 keys of a key head; streams 64-row tiles of
+//                  every query head that shares it;
+//   k_diff_dq_tc   one CTA per 128 rows of a query head; streams 64-key tiles,
+//                  and sums P_2 G (dlam) in f32 on the way.
+// The operands that the threads make (the difference of the maps, dS_1, dS_2)
+// are rounded to the tensors' type and stay in tensor memory, written over
+// the scores they came from; a thread writes only columns it has read.  A
+// 16-bit tile in the 128-byte swizzle serves K-major (its rows as N) and
+// MN-major (its rows as K) alike, so one copy of Q, K and dO feeds both
+// products.  Two warpgroups share a tile, 32 of its 64 columns each.
+// Every wait is bounded; on expiry the kernel records AMC_ERR_TIMEOUT, drains
+// and returns.
+#include <cmath>
+#include <type_traits>
+
+#include "amc_diffattn.h"
+#include "amc_half.cuh"
+#include "amc_tc.cuh"
+
+namespace amc {
+
+using namespace tc;
+
+namespace {
+
+constexpr int kThreadsB = 384;       // warps 0-7 rows (two warpgroups), 8 loads, 9 issues
+constexpr int kRowThreads = 256;
+constexpr int kStages = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// dK/dV kernel (bytes from a 1024-aligned base)
+template <int NV>
+struct KvSmem {
+  static constexpr int k = 0;                                 // 2 maps x 128 keys
+  static constexpr int v = 32768;
+  static constexpr int f = v + NV / 64 * 16384;               // stages: Q_1, Q_2 (8 KB each), dO, pairs
+  static constexpr int stage = 16384 + NV / 64 * 8192;
+  static constexpr int r = f + kStages * stage;               // stages: 64 lse2 pairs, 64 dsum pairs
+  static constexpr int bar = r + kStages * 1024;
+  static constexpr int bytes = bar + 256 + 1024;
+};
+// dQ kernel
+template <int NV>
+struct QSmem {
+  static constexpr int q = 0;
+  static constexpr int g = 32768;                             // dO
+  static constexpr int f = g + NV / 64 * 16384;               // stages: K_1, K_2 (8 KB each), V
+  static constexpr int stage = 16384 + NV / 64 * 8192;
+  static constexpr int bar = f + kStages * stage;
+  static constexpr int bytes = bar + 256 + 1024;
+};
+static_assert(KvSmem<128>::bytes <= 232448 && QSmem<128>::bytes <= 232448, "shared memory");
+
+__device__ int g_diff_bwd_error;
+
+template <typename T>
+__device__ __forceinline__ void store16(T* dst, const float (&v)[16], float f, int cols) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack2<T>(v[2 * i] * f, v[2 * i + 1] * f);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (8 * i < cols)
+      *reinterpret_cast<uint4*>(dst + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+}
+
+// Zero the 128-byte row of a swizzled tile region.
+__device__ __forceinline__ void zero_row(unsigned char* row) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) *reinterpret_cast<int4*>(row + 16 * i) = make_int4(0, 0, 0, 0);
+}
+
+}  // namespace
+
+// ------------------------------------------------------------------ dK, dV
+// Tensor memory: four 64-column buffers in two pairs, dV at 256, dK_1, dK_2 at
+// 384 and 448.  Tile i has S_1, S_2 in pair X = i & 1 and G in the first
+// buffer of the other pair Y.  The threads take the exponentials of S(i) as
+// soon as S(i) is there, then read G(i); that frees Y's first buffer (Y's
+// second held dS_2(i-1), whose product was issued before), so S(i+1) goes to
+// Y while the threads write the operands of tile i over X; their products and
+// then G(i+1), into X's first buffer, run while the threads take the
+// exponentials of tile i+1.  One thread issues everything, so a buffer that
+// an earlier product reads may be the target of a later one.
+template <typename T, int NV>
+__global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
+    const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mK,
+    const __grid_constant__ CUtensorMap mV, const __grid_constant__ CUtensorMap mG,
+    const __grid_constant__ amc_diff_attention p, const __grid_constant__ DiffBwdWork wk) {
+  using L = KvSmem<NV>;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ unsigned char diff_sm_raw[];
+  unsigned char* sm = (unsigned char*)(((uintptr_t)diff_sm_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* kv_full = (uint64_t*)(sm + L::bar);
+  uint64_t* f_full = kv_full + 1;            // [kStages] Q, dO and row pairs landed
+  uint64_t* f_empty = f_full + kStages;      // [kStages] their products are done and the pairs read
+  uint64_t* s_full = f_empty + kStages;      // S(i) complete
+  uint64_t* g_full = s_full + 1;             // G(i) complete
+  uint64_t* g_read = s_full + 2;             // the threads have read G(i) (count 256)
+  uint64_t* p_full = s_full + 3;             // operands of tile i written (count 256)
+  uint64_t* acc_full = s_full + 4;
+  uint32_t* tslot = (uint32_t*)(sm + L::bar + 192);
+  volatile int* abort_flag = (volatile int*)(sm + L::bar + 196);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // key tiles of one head are launched first tile first: with a causal mask
+  // those have the most rows
+  const int per = p.kv_heads * p.batch, group = p.heads / p.kv_heads;
+  const int k0 = (int)(blockIdx.x / per) * 128, g = blockIdx.x % per % p.kv_heads, b = blockIdx.x % per / p.kv_heads;
+  const DiffLens len = diff_lens(p, b);
+  const int first = diff_first_row(len, p.causal, k0) / 64 * 64;
+  const int nth = first < len.nq ? (len.nq - first + 63) / 64 : 0;   // tiles a head
+  const int nt = nth * group;
+  if (tid == 0) {
+    mbar_init(kv_full, 1);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&f_full[i], 1);
+      mbar_init(&f_empty[i], 1 + kRowThreads);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(g_full, 1);
+    mbar_init(g_read, kRowThreads);
+    mbar_init(p_full, kRowThreads);
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  __syncthreads();
+  if (warp == 0) tmem_alloc(tslot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tslot;
+  const uint32_t t_dv = tmem + 256, t_dk = tmem + 384;
+
+  if (warp == 8) {
+    if (lane == 0 && nt > 0) {
+      mbar_expect_tx(kv_full, 32768 + NV / 64 * 16384);
+      for (int m = 0; m < 2; ++m) tma_load_4d(sm + L::k + m * 16384, &mK, 0, k0, 2 * g + m, b, kv_full);
+      for (int c = 0; c < NV / 64; ++c) tma_load_4d(sm + L::v + c * 16384, &mV, 64 * c, k0, g, b, kv_full);
+      int h = g * group, r0 = first;
+      for (int i = 0; i < nt; ++i) {
+        const int s = i % kStages;
+        if (i >= kStages && !mbar_wait(&f_empty[s], (uint32_t)(i / kStages - 1) & 1u)) { *abort_flag = 1; break; }
+        if (*abort_flag) break;
+        const int rows = min(64, wk.pitch - r0);
+        unsigned char* st = sm + L::f + s * L::stage;
+        mbar_expect_tx(&f_full[s], L::stage + rows * 16);
+        for (int m = 0; m < 2; ++m) tma_load_4d(st + m * 8192, &mQ, 0, r0, 2 * h + m, b, &f_full[s]);
+        for (int c = 0; c < NV / 64; ++c) tma_load_4d(st + 16384 + c * 8192, &mG, 64 * c, r0, h, b, &f_full[s]);
+        const int64_t at = ((int64_t)b * p.heads + h) * wk.pitch + r0;
+        bulk_load_1d(sm + L::r + s * 1024, wk.lse2 + at, rows * 8, &f_full[s]);
+        bulk_load_1d(sm + L::r + s * 1024 + 512, wk.dsum + at, rows * 8, &f_full[s]);
+        r0 += 64;
+        if (r0 >= len.nq) {
+          r0 = first;
+          ++h;
+        }
+      }
+    }
+  } else if (warp == 9) {
+    if (lane == 0 && nt > 0) {
+      const uint32_t id = idesc_f16(128, 64, kBf16, false, false);
+      const uint32_t id_dk = idesc_f16(128, 64, kBf16, false, true);
+      const uint32_t id_dv = idesc_f16(128, NV, kBf16, false, true);
+      const uint64_t kd = sdesc(smem_addr(sm + L::k), 16, 1024), vd = sdesc(smem_addr(sm + L::v), 16, 1024);
+      const uint64_t fd = sdesc(smem_addr(sm + L::f), 16, 1024), fmn = sdesc_mn16(smem_addr(sm + L::f), 8192);
+      const int ksteps = (p.d + 15) / 16, vsteps = (p.dv + 15) / 16;
+      auto issue_s = [&](int i) {
+        const uint64_t st = desc_add(fd, (i % kStages) * L::stage);
+        for (int m = 0; m < 2; ++m)
+          for (int k = 0; k < ksteps; ++k)
+            mma_f16(tmem + (i & 1) * 128 + m * 64, desc_add(kd, m * 16384 + k * 32), desc_add(st, m * 8192 + k * 32), id,
+                    k > 0);
+        mma_commit(s_full);
+      };
+      auto issue_g = [&](int i) {
+        const uint64_t st = desc_add(fd, (i % kStages) * L::stage + 16384);
+        for (int k = 0; k < vsteps; ++k)
+          mma_f16(tmem + (~i & 1) * 128, desc_add(vd, (k >> 2) * 16384 + (k & 3) * 32),
+                  desc_add(st, (k >> 2) * 8192 + (k & 3) * 32), id, k > 0);
+        mma_commit(g_full);
+      };
+      // A operands: warpgroup w wrote rows 32 w .. 32 w + 31 of the tile (K
+      // steps 2 w and 2 w + 1) at columns 32 w (+16 for dS_1) of the buffers
+      auto issue_acc = [&](int i) {
+        const uint64_t st = desc_add(fmn, (i % kStages) * L::stage);
+        const uint32_t x = tmem + (i & 1) * 128;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t a = x + (k >> 1) * 32 + (k & 1) * 8;
+          mma_f16_ts(t_dv, a, desc_add(st, 16384 + k * 2048), id_dv, i > 0 || k > 0);
+          mma_f16_ts(t_dk, a + 16, desc_add(st, k * 2048), id_dk, i > 0 || k > 0);
+          mma_f16_ts(t_dk + 64, a + 64, desc_add(st, 8192 + k * 2048), id_dk, i > 0 || k > 0);
+        }
+        mma_commit(&f_empty[i % kStages]);
+      };
+      bool ok = mbar_wait(kv_full, 0) && mbar_wait(&f_full[0], 0);
+      if (ok) {
+        tc_fence_after();
+        issue_s(0);
+        issue_g(0);
+      }
+      for (int i = 0; i < nt && ok; ++i) {
+        const bool more = i + 1 < nt;
+        if (more) {
+          if (!mbar_wait(&f_full[(i + 1) % kStages], (uint32_t)((i + 1) / kStages) & 1u) ||
+              !mbar_wait(g_read, (uint32_t)i & 1u)) { ok = false; break; }
+          tc_fence_after();
+          issue_s(i + 1);
+        }
+        if (!mbar_wait(p_full, (uint32_t)i & 1u) || *abort_flag) { ok = false; break; }
+        tc_fence_after();
+        issue_acc(i);
+        if (more) issue_g(i + 1);
+      }
+      if (ok) mma_commit(acc_full);
+      else *abort_flag = 1;
+    }
+  } else if (warp < 8) {
+    // one thread per key; warpgroup w takes rows 32 w .. 32 w + 31 of a tile
+    const int w = warp >> 2, t = tid & 127;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const float c2 = p.scale * kLog2e;
+    const int fr = diff_first_row(len, p.causal, k0 + t);
+    const int fr_all = diff_first_row(len, p.causal, k0 + 127);   // from here on every key of the tile is seen
+    bool ok = true;
+    int h = g * group, r0 = first;
+    float lam = nt > 0 ? wk.lam[h] : 0.f;
+    for (int i = 0; i < nt; ++i) {
+      const int s = i % kStages;
+      const uint32_t x = tmem + (i & 1) * 128 + lane_base + 32 * w;
+      ok = __all_sync(0xffffffffu, mbar_wait(&f_full[s], (uint32_t)(i / kStages) & 1u) &&
+                                       mbar_wait(s_full, (uint32_t)i & 1u) && !*abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      const float4* le = reinterpret_cast<const float4*>(sm + L::r + s * 1024 + 256 * w);
+      uint32_t s1[32], s2[32];
+      tmem_ld32_nowait(x, s1);
+      tmem_ld32_nowait(x + 64, s2);
+      tmem_ld_wait();
+      float p1[32], p2[32];
+#pragma unroll
+      for (int j = 0; j < 32; j += 2) {
+        const float4 e = le[j >> 1];
+        p1[j] = ex2_approx(fmaf(__uint_as_float(s1[j]), c2, -e.x));
+        p2[j] = lam * ex2_approx(fmaf(__uint_as_float(s2[j]), c2, -e.y));
+        p1[j + 1] = ex2_approx(fmaf(__uint_as_float(s1[j + 1]), c2, -e.z));
+        p2[j + 1] = lam * ex2_approx(fmaf(__uint_as_float(s2[j + 1]), c2, -e.w));
+      }
+      const bool masked = r0 < fr_all || r0 + 64 > len.nq;
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const int r = r0 + 32 * w + j;
+          if (r < fr || r >= len.nq) p1[j] = p2[j] = 0.f;
+        }
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(g_full, (uint32_t)i & 1u));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t gv[32];
+      tmem_ld32_nowait(tmem + (~i & 1) * 128 + lane_base + 32 * w, gv);
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive(g_read);
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const int r = r0 + 32 * w + j;
+          if (r < fr || r >= len.nq) gv[j] = 0u;
+        }
+        if (r0 + 64 > len.nq && t < 64 && r0 + t >= len.nq) {
+          // rows behind the length may hold anything, and 0 times it is not
+          // 0: clear them (the scores have been read) before the products
+          unsigned char* row = sm + L::f + s * L::stage + t * 128;
+          zero_row(row + (w ? 8192 : 0));
+          if (NV == 128 || !w) zero_row(row + 16384 + (w ? 8192 : 0));
+        }
+        fence_proxy_async();
+      }
+      float v[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        v[j] = __uint_as_float(pack2<T>(p1[2 * j] - p2[2 * j], p1[2 * j + 1] - p2[2 * j + 1]));
+      tmem_st16(x, v);
+      float v2[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        float4 d = le[32 + j];
+        const float g0 = __uint_as_float(gv[2 * j]), g1 = __uint_as_float(gv[2 * j + 1]);
+        if (masked) {   // the pairs of rows that see nothing may be unwritten
+          const int r = r0 + 32 * w + 2 * j;
+          if (r < fr || r >= len.nq) d.x = d.y = 0.f;
+          if (r + 1 < fr || r + 1 >= len.nq) d.z = d.w = 0.f;
+        }
+        v[j] = __uint_as_float(pack2<T>(p1[2 * j] * (g0 - d.x), p1[2 * j + 1] * (g1 - d.z)));
+        v2[j] = __uint_as_float(pack2<T>(p2[2 * j] * (d.y - g0), p2[2 * j + 1] * (d.w - g1)));
+      }
+      tmem_st16(x + 16, v);
+      tmem_st16(x + 64, v2);
+      tmem_st_wait();
+      mbar_arrive(&f_empty[s]);
+      tc_fence_before();
+      mbar_arrive(p_full);
+      r0 += 64;
+      if (r0 >= len.nq) {
+        r0 = first;
+        ++h;
+        if (i + 1 < nt) lam = wk.lam[h];
+      }
+    }
+    if (nt > 0) ok = ok && mbar_wait(acc_full, 0);
+    ok = named_bar_and(1, kRowThreads, ok && !*abort_flag);
+    if (ok) {
+      // warpgroup w writes dK_{w+1} and columns 64 w .. of dV
+      tc_fence_after();
+      const int key = k0 + t;
+      T* dk = (T*)p.dk + b * p.dks[0] + (2 * g + w) * p.dks[1] + (int64_t)key * p.dks[2];
+      T* dv = (T*)p.dv_ + b * p.dvs[0] + g * p.dvs[1] + (int64_t)key * p.dvs[2] + 64 * w;
+#pragma unroll 1
+      for (int c = 0; c < 64; c += 16) {
+        float v[16];
+        if (nt > 0) tmem_ld16(t_dk + 64 * w + lane_base + c, v);
+        else
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = 0.f;
+        if (key < p.nk && c < p.d) store16<T>(dk + c, v, p.scale, p.d - c);
+        if (64 * w < NV) {
+          if (nt > 0) tmem_ld16(t_dv + 64 * w + lane_base + c, v);
+          if (key < p.nk && 64 * w + c < p.dv) store16<T>(dv + c, v, 1.f, p.dv - 64 * w - c);
+        }
+      }
+    } else if (tid == 0) {
+      *abort_flag = 1;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    if (tid == 0) atomicExch(&g_diff_bwd_error, AMC_ERR_TIMEOUT);
+    // bounded drain of copies and products still in flight
+    mbar_wait(kv_full, 0, 1 << 14);
+    for (int i = 0; i < kStages; ++i) mbar_wait(&f_full[i], 0, 1 << 14);
+    mbar_wait(s_full, 0, 1 << 14);
+    mbar_wait(g_full, 0, 1 << 14);
+    mbar_wait(acc_full, 0, 1 << 14);
+  }
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------------ dQ, dlam
+// Tensor memory: two buffers of S_1, S_2, G (64 columns each) at 0 and 192,
+// dQ_1, dQ_2 at 384 and 448.  Tile j+2 is computed into the buffer of tile j
+// right after the products that read dS(j) from it, while the threads work on
+// tile j+1.
+template <typename T, int NV>
+__global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
+    const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mK,
+    const __grid_constant__ CUtensorMap mV, const __grid_constant__ CUtensorMap mG,
+    const __grid_constant__ amc_diff_attention p, const __grid_constant__ DiffBwdWork wk) {
+  using L = QSmem<NV>;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ unsigned char diff_sm_raw[];
+  unsigned char* sm = (unsigned char*)(((uintptr_t)diff_sm_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* q_full = (uint64_t*)(sm + L::bar);
+  uint64_t* f_full = q_full + 1;             // [kStages]
+  uint64_t* f_empty = f_full + kStages;      // [kStages]
+  uint64_t* s_full = f_empty + kStages;      // [2] S_1, S_2, G of a buffer
+  uint64_t* p_full = s_full + 2;             // [2] dS written (count 256)
+  uint64_t* acc_full = p_full + 2;
+  uint32_t* tslot = (uint32_t*)(sm + L::bar + 192);
+  volatile int* abort_flag = (volatile int*)(sm + L::bar + 196);
+  float* red = (float*)(sm + L::bar + 208);  // [8]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int per = p.heads * p.batch, tiles = (p.nq + 127) / 128;
+  const int tile = tiles - 1 - (int)(blockIdx.x / per), h = blockIdx.x % per % p.heads, b = blockIdx.x % per / p.heads;
+  const int g = h / (p.heads / p.kv_heads), r0 = tile * 128;
+  const DiffLens len = diff_lens(p, b);
+  const int last = min(r0 + 128, len.nq) - 1;
+  const int kend = last >= r0 ? diff_limit(len, p.causal, last) : 0;
+  const int nt = (kend + 63) / 64;
+  if (tid == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&f_full[i], 1);
+      mbar_init(&f_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], kRowThreads);
+    }
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  __syncthreads();
+  if (warp == 0) tmem_alloc(tslot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tslot;
+  const uint32_t t_dq = tmem + 384;
+
+  if (warp == 8) {
+    if (lane == 0 && nt > 0) {
+      mbar_expect_tx(q_full, 32768 + NV / 64 * 16384);
+      for (int m = 0; m < 2; ++m) tma_load_4d(sm + L::q + m * 16384, &mQ, 0, r0, 2 * h + m, b, q_full);
+      for (int c = 0; c < NV / 64; ++c) tma_load_4d(sm + L::g + c * 16384, &mG, 64 * c, r0, h, b, q_full);
+      for (int j = 0; j < nt; ++j) {
+        const int s = j % kStages;
+        if (j >= kStages && !mbar_wait(&f_empty[s], (uint32_t)(j / kStages - 1) & 1u)) { *abort_flag = 1; break; }
+        if (*abort_flag) break;
+        unsigned char* st = sm + L::f + s * L::stage;
+        mbar_expect_tx(&f_full[s], L::stage);
+        for (int m = 0; m < 2; ++m) tma_load_4d(st + m * 8192, &mK, 0, j * 64, 2 * g + m, b, &f_full[s]);
+        for (int c = 0; c < NV / 64; ++c) tma_load_4d(st + 16384 + c * 8192, &mV, 64 * c, j * 64, g, b, &f_full[s]);
+      }
+    }
+  } else if (warp == 9) {
+    if (lane == 0 && nt > 0) {
+      const uint32_t id = idesc_f16(128, 64, kBf16, false, false);
+      const uint32_t id_dq = idesc_f16(128, 64, kBf16, false, true);
+      const uint64_t qd = sdesc(smem_addr(sm + L::q), 16, 1024), gd = sdesc(smem_addr(sm + L::g), 16, 1024);
+      const uint64_t fd = sdesc(smem_addr(sm + L::f), 16, 1024), fmn = sdesc_mn16(smem_addr(sm + L::f), 8192);
+      const int ksteps = (p.d + 15) / 16, vsteps = (p.dv + 15) / 16;
+      auto issue_s = [&](int j) -> bool {
+        if (!mbar_wait(&f_full[j % kStages], (uint32_t)(j / kStages) & 1u)) return false;
+        tc_fence_after();
+        const uint64_t st = desc_add(fd, (j % kStages) * L::stage);
+        const uint32_t x = tmem + (j & 1) * 192;
+        for (int m = 0; m < 2; ++m)
+          for (int k = 0; k < ksteps; ++k)
+            mma_f16(x + m * 64, desc_add(qd, m * 16384 + k * 32), desc_add(st, m * 8192 + k * 32), id, k > 0);
+        for (int k = 0; k < vsteps; ++k)
+          mma_f16(x + 128, desc_add(gd, (k >> 2) * 16384 + (k & 3) * 32),
+                  desc_add(st, 16384 + (k >> 2) * 8192 + (k & 3) * 32), id, k > 0);
+        mma_commit(&s_full[j & 1]);
+        return true;
+      };
+      bool ok = mbar_wait(q_full, 0);
+      for (int j = 0; j < 2 && j < nt && ok; ++j) ok = issue_s(j);
+      for (int j = 0; j < nt && ok; ++j) {
+        if (!mbar_wait(&p_full[j & 1], (uint32_t)(j >> 1) & 1u) || *abort_flag) { ok = false; break; }
+        tc_fence_after();
+        const uint64_t st = desc_add(fmn, (j % kStages) * L::stage);
+        const uint32_t x = tmem + (j & 1) * 192;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t a = x + (k >> 1) * 32 + (k & 1) * 8;   // warpgroup k / 2 wrote keys 16 k .. of the tile
+          mma_f16_ts(t_dq, a, desc_add(st, k * 2048), id_dq, j > 0 || k > 0);
+          mma_f16_ts(t_dq + 64, a + 64, desc_add(st, 8192 + k * 2048), id_dq, j > 0 || k > 0);
+        }
+        mma_commit(&f_empty[j % kStages]);
+        if (j + 2 < nt) ok = issue_s(j + 2);
+      }
+      if (ok) mma_commit(acc_full);
+      else *abort_flag = 1;
+    }
+  } else if (warp < 8) {
+    // one thread per row; warpgroup w takes keys 32 w .. 32 w + 31 of a tile
+    const int w = warp >> 2, t = tid & 127, row = r0 + t;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const float c2 = p.scale * kLog2e, lam = wk.lam[h];
+    const int lim = diff_limit(len, p.causal, row);
+    const int all_see = r0 + 127 < len.nq ? diff_limit(len, p.causal, r0) : 0;
+    float2 e = make_float2(INFINITY, INFINITY), ds = make_float2(0.f, 0.f);
+    if (lim > 0) {
+      const int64_t at = ((int64_t)b * p.heads + h) * wk.pitch + row;
+      e = wk.lse2[at];
+      ds = wk.dsum[at];
+    }
+    float pg = 0.f;
+    bool ok = true;
+    for (int j = 0; j < nt; ++j) {
+      const uint32_t x = tmem + (j & 1) * 192 + lane_base + 32 * w;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[j & 1], (uint32_t)(j >> 1) & 1u) && !*abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s1[32], s2[32], gv[32];
+      tmem_ld32_nowait(x, s1);
+      tmem_ld32_nowait(x + 64, s2);
+      tmem_ld32_nowait(x + 128, gv);
+      tmem_ld_wait();
+      if (j * 64 + 64 > all_see) {
+        const int n = lim - j * 64 - 32 * w;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i >= n) {
+            s1[i] = s2[i] = 0xff800000u;
+            gv[i] = 0u;
+          }
+        if (j * 64 + 64 > len.nk && len.nk < p.nk && t < 64 && j * 64 + t >= len.nk) {
+          // K behind the length may hold anything, and 0 times it is not 0
+          zero_row(sm + L::f + (j % kStages) * L::stage + w * 8192 + t * 128);
+        }
+        fence_proxy_async();
+      }
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      float v1[16], v2[16];
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        float a[2], c[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float gk = __uint_as_float(gv[i + k]);
+          const float p1 = ex2_approx(fmaf(__uint_as_float(s1[i + k]), c2, -e.x));
+          const float p2 = ex2_approx(fmaf(__uint_as_float(s2[i + k]), c2, -e.y));
+          part[(i + k) & 3] = fmaf(p2, gk, part[(i + k) & 3]);
+          a[k] = p1 * (gk - ds.x);
+          c[k] = (lam * p2) * (ds.y - gk);
+        }
+        v1[i >> 1] = __uint_as_float(pack2<T>(a[0], a[1]));
+        v2[i >> 1] = __uint_as_float(pack2<T>(c[0], c[1]));
+      }
+      tmem_st16(x, v1);
+      tmem_st16(x + 64, v2);
+      tmem_st_wait();
+      pg += (part[0] + part[1]) + (part[2] + part[3]);
+      tc_fence_before();
+      mbar_arrive(&p_full[j & 1]);
+    }
+    if (nt > 0) ok = ok && mbar_wait(acc_full, 0);
+    for (int o = 16; o > 0; o >>= 1) pg += __shfl_xor_sync(0xffffffffu, pg, o);
+    if (lane == 0) red[warp] = pg;
+    ok = named_bar_and(1, kRowThreads, ok && !*abort_flag);
+    if (ok) {
+      tc_fence_after();
+      // warpgroup w writes dQ_{w+1}
+      T* dq = (T*)p.dq + b * p.dqs[0] + (2 * h + w) * p.dqs[1] + (int64_t)row * p.dqs[2];
+#pragma unroll 1
+      for (int c = 0; c < 64; c += 16) {
+        float v[16];
+        if (nt > 0) tmem_ld16(t_dq + 64 * w + lane_base + c, v);
+        else
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = 0.f;
+        if (row < p.nq && c < p.d) store16<T>(dq + c, v, p.scale, p.d - c);
+      }
+      if (tid == 0)
+        wk.partials[((int64_t)h * p.batch + b) * tiles + tile] =
+            ((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7]));
+    } else if (tid == 0) {
+      *abort_flag = 1;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    if (tid == 0) atomicExch(&g_diff_bwd_error, AMC_ERR_TIMEOUT);
+    mbar_wait(q_full, 0, 1 << 14);
+    for (int i = 0; i < kStages; ++i) mbar_wait(&f_full[i], 0, 1 << 14);
+    for (int i = 0; i < 2; ++i) mbar_wait(&s_full[i], 0, 1 << 14);
+    mbar_wait(acc_full, 0, 1 << 14);
+  }
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+namespace {
+
+bool aligned_out(const void* x, const int64_t s[3], int64_t heads, int64_t rows, int64_t batch) {
+  return !((uintptr_t)x & 15) && (batch == 1 || s[0] % 8 == 0) && (heads == 1 || s[1] % 8 == 0) &&
+         (rows == 1 || s[2] % 8 == 0);
+}
+
+template <typename T, int NV>
+int bwd_tc(const amc_diff_attention& p, const DiffBwdWork& w, const CUtensorMap (&kv)[4], const CUtensorMap (&q)[4],
+           cudaStream_t s) {
+  static std::atomic<uint64_t> attr_kv{0}, attr_q{0};
+  if (int rc = smem_attr_once(k_diff_dkv_tc<T, NV>, KvSmem<NV>::bytes, attr_kv)) return rc;
+  if (int rc = smem_attr_once(k_diff_dq_tc<T, NV>, QSmem<NV>::bytes, attr_q)) return rc;
+  const unsigned gk = (unsigned)((int64_t)((p.nk + 127) / 128) * p.kv_heads * p.batch);
+  const int tiles = (p.nq + 127) / 128;
+  k_diff_dkv_tc<T, NV><<<gk, kThreadsB, KvSmem<NV>::bytes, s>>>(kv[0], kv[1], kv[2], kv[3], p, w);
+  AMC_CUDA(cudaGetLastError());
+  const unsigned gq = (unsigned)((int64_t)tiles * p.heads * p.batch);
+  k_diff_dq_tc<T, NV><<<gq, kThreadsB, QSmem<NV>::bytes, s>>>(q[0], q[1], q[2], q[3], p, w);
+  AMC_CUDA(cudaGetLastError());
+  return launch_diff_dlam(p, w, tiles, s);
+}
+
+}  // namespace
+
+int diff_bwd_tc(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s, bool* handled) {
+  *handled = false;
+  if (!diff_tc_shape(p) || p.nq <= 0) return AMC_OK;
+  if (!aligned_out(p.dq, p.dqs, 2 * p.heads, p.nq, p.batch) || !aligned_out(p.dk, p.dks, 2 * p.kv_heads, p.nk, p.batch) ||
+      !aligned_out(p.dv_, p.dvs, p.kv_heads, p.nk, p.batch))
+    return AMC_OK;
+  if ((int64_t)((p.nq + 127) / 128) * p.heads * p.batch > 0x7fffffff ||
+      (int64_t)((p.nk + 127) / 128) * p.kv_heads * p.batch > 0x7fffffff)
+    return AMC_OK;
+  const bool bf16 = p.dtype == AMC_BF16;
+  CUtensorMap kv[4], q[4];   // Q, K, V, dO: boxes of 128 rows for the resident side, 64 for the streamed one
+  int rc = AMC_OK;
+  for (int side = 0; side < 2 && !rc; ++side) {
+    CUtensorMap* m = side ? q : kv;
+    const uint32_t rq = side ? 128 : 64, rk = side ? 64 : 128;
+    rc = make_tmap_4d_16(&m[0], p.q, bf16, p.batch, 2 * p.heads, p.nq, p.d, p.qs, rq);
+    if (!rc) rc = make_tmap_4d_16(&m[1], p.k, bf16, p.batch, 2 * p.kv_heads, p.nk, p.d, p.ks, rk);
+    if (!rc) rc = make_tmap_4d_16(&m[2], p.v, bf16, p.batch, p.kv_heads, p.nk, p.dv, p.vs, rk);
+    if (!rc) rc = make_tmap_4d_16(&m[3], p.d_o, bf16, p.batch, p.heads, p.nq, p.dv, p.dos, rq);
+  }
+  if (rc == AMC_ERR_UNSUPPORTED) return AMC_OK;
+  if (rc) return rc;
+  *handled = true;
+  if (bf16) return p.dv <= 64 ? bwd_tc<__nv_bfloat16, 64>(p, w, kv, q, s) : bwd_tc<__nv_bfloat16, 128>(p, w, kv, q, s);
+  return p.dv <= 64 ? bwd_tc<__half, 64>(p, w, kv, q, s) : bwd_tc<__half, 128>(p, w, kv, q, s);
+}
+
+int diff_bwd_check_error() {
+  int e = 0;
+  AMC_CUDA(cudaMemcpyFromSymbol(&e, g_diff_bwd_error, sizeof(int)));
+  if (e) {
+    int z = 0;
+    AMC_CUDA(cudaMemcpyToSymbol(g_diff_bwd_error, &z, sizeof(int)));
+    return fail(e, "diff_attention backward: a bounded wait on the tensor-core pipeline gave up");
+  }
+  return AMC_OK;
+}
+
+}  // namespace amc
