@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(256) k_adamw(const __grid_constant__ AdamArgs 
       top_m = warp_max(top_m);
       top_u = warp_max(top_u);
       const bool some_m = top_m >= 7.888609052210118e-31f, some_u = top_u >= 7.888609052210118e-31f;   // 2^-100
-      const float im = some_m ? kE4m3Max / top_m : 0.f, iu = some_u ? kE4m3Max / top_u : 0.f;
+      const float im = some_m ? 1.f / top_m * kE4m3Max : 0.f, iu = some_u ? 1.f / top_u * kE4m3Max : 0.f;
       if (lane == 0) {
         t.m_scale[e0 / kAdamBlock] = some_m ? top_m * (1.f / kE4m3Max) : 0.f;
         t.v_scale[e0 / kAdamBlock] = some_u ? top_u * (1.f / kE4m3Max) : 0.f;

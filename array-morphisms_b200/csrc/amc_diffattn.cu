@@ -511,7 +511,6 @@ int check_sizes(const amc_diff_attention* p, const char* who) {
   return AMC_OK;
 }
 
-size_t fwd_bytes(const amc_diff_attention&) { return 0; }
 
 int check_workspace(const amc_diff_attention* p, size_t need, const char* who) {
   if (!need) return AMC_OK;
@@ -532,7 +531,7 @@ extern "C" {
 int amc_diff_attention_workspace(const amc_diff_attention* p, int32_t backward, int64_t* bytes) {
   if (!bytes) return fail(AMC_ERR_INVALID, "amc_diff_attention_workspace: null out");
   if (int rc = check_sizes(p, "amc_diff_attention_workspace")) return rc;
-  size_t n = fwd_bytes(*p);
+  size_t n = diff_split_bytes(*p);
   if (backward && diff_bwd_bytes(*p) > n) n = diff_bwd_bytes(*p);
   *bytes = (int64_t)n;
   return AMC_OK;
@@ -543,10 +542,12 @@ int amc_diff_attention_fwd(const amc_diff_attention* p, void* stream) {
   if (!p->batch || !p->nq) return AMC_OK;
   if (!p->q || !p->o || !p->lam || (p->nk && (!p->k || !p->v)))
     return fail(AMC_ERR_INVALID, "amc_diff_attention_fwd: null tensor");
-  if (int rc = check_workspace(p, fwd_bytes(*p), "amc_diff_attention_fwd")) return rc;
+  if (int rc = check_workspace(p, diff_split_bytes(*p), "amc_diff_attention_fwd")) return rc;
   if (fault_injected("launch")) return fail(AMC_ERR_INJECTED, "diff_attention: injected launch failure (AMC_FAULT=launch)");
   cudaStream_t s = pick_stream(stream);
   bool handled = false;
+  if (int rc = diff_fwd_split(*p, s, &handled)) return rc;
+  if (handled) return AMC_OK;
   if (int rc = diff_fwd_tc(*p, s, &handled)) return rc;
   if (handled) return AMC_OK;
   return launch_diff_fwd_simt(*p, s);

@@ -62,6 +62,9 @@ inline DiffBwdWork diff_bwd_work(const amc_diff_attention& p) {
 // types, shapes and alignments.
 bool diff_tc_shape(const amc_diff_attention& p);
 int diff_fwd_tc(const amc_diff_attention& p, cudaStream_t s, bool* handled);
+// The form for few rows and many keys, likewise, and its workspace.
+size_t diff_split_bytes(const amc_diff_attention& p);
+int diff_fwd_split(const amc_diff_attention& p, cudaStream_t s, bool* handled);
 int launch_diff_fwd_simt(const amc_diff_attention& p, cudaStream_t s);
 int launch_diff_bwd_rows(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s);
 int launch_diff_bwd_simt(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s);

@@ -359,12 +359,13 @@ int fwd_tc(const amc_diff_attention& p, const CUtensorMap (&map)[3], cudaStream_
 }  // namespace
 
 bool diff_tc_shape(const amc_diff_attention& p) {
-  return p.dtype != AMC_F32 && p.d <= 64 && p.dv <= 128 && p.d % 8 == 0 && p.dv % 8 == 0 && p.scale > 0.f && p.nk > 0;
+  return p.dtype != AMC_F32 && p.d <= 64 && p.dv <= 128 && p.d % 8 == 0 && p.dv % 8 == 0 && p.nk > 0;
 }
 
 int diff_fwd_tc(const amc_diff_attention& p, cudaStream_t s, bool* handled) {
   *handled = false;
-  if (!diff_tc_shape(p) || !aligned_rows(p.o, p.os, p) || (p.o2 && !aligned_rows(p.o2, p.o2s, p))) return AMC_OK;
+  // the running maximum is taken before the scale
+  if (!diff_tc_shape(p) || !(p.scale > 0.f) || !aligned_rows(p.o, p.os, p) || (p.o2 && !aligned_rows(p.o2, p.o2s, p))) return AMC_OK;
   if ((int64_t)((p.nq + 127) / 128) * p.heads * p.batch > 0x7fffffff) return AMC_OK;
   CUtensorMap map[3];
   const bool bf16 = p.dtype == AMC_BF16;

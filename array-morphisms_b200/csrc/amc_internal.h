@@ -300,6 +300,7 @@ int colfold_check_error();
 int dist_check_error();
 int diff_check_error();
 int diff_bwd_check_error();
+int diff_split_check_error();
 int device_check_errors();  // all kernels' bounded-wait flags
 
 }  // namespace amc

@@ -159,6 +159,8 @@ int device_check_errors() {
   if (rc) return rc;
   rc = diff_bwd_check_error();
   if (rc) return rc;
+  rc = diff_split_check_error();
+  if (rc) return rc;
   rc = colfold_check_error();
   if (rc) return rc;
   return conv_check_error();

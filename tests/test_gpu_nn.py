@@ -243,6 +243,11 @@ FWD = [
     dict(B=4, H=2, K=1, nq=150, nk=150, d=64, causal=True, q_lens=[150, 0, 1, 77], kv_lens=[150, 0, 1, 77]),
     dict(B=4, H=2, K=2, nq=130, nk=260, d=64, q_lens=[130, 20, 1, 128], kv_lens=[0, 260, 129, 128]),
     dict(B=3, H=2, K=1, nq=40, nk=300, d=64, causal=True, q_lens=[40, 3, 40], kv_lens=[300, 256, 20]),
+    dict(B=3, H=4, K=1, nq=1, nk=1500, d=64, causal=True, q_lens=[1, 1, 0], kv_lens=[1500, 257, 9]),   # one token
+    dict(B=2, H=4, K=2, nq=4, nk=1030, d=64, causal=True, kv_lens=[1029, 2]),    # a few; rows that see no key
+    dict(B=1, H=16, K=1, nq=1, nk=700, d=32),
+    dict(B=1, H=2, K=2, nq=16, nk=530, d=40, dv=72),
+    dict(B=2, H=3, K=3, nq=2, nk=137, d=64, heads_inner=False),
     dict(B=1, H=2, K=1, nq=70, nk=70, d=100, dv=200, causal=True),    # wide head
     dict(B=1, H=1, K=1, nq=33, nk=65, d=13, dv=7),                    # odd dims
     dict(B=1, H=2, K=1, nq=33, nk=65, d=64, heads_inner=False, lam_rows=1),
