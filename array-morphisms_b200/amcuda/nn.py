@@ -55,12 +55,29 @@ def _run(name: str, device, stream, *args) -> None:
         stream = torch.cuda.current_stream(device)
     # handle 0, torch's default stream, is the legacy stream (1 in the C ABI's
     # terms: NULL would mean the library's own stream)
-    ptr = C.c_void_p(stream.cuda_stream or 1)
+    ptr = stream.cuda_stream or 1
     if device.index == torch.cuda.current_device():
         A.call(name, *args, ptr)
     else:
         with torch.cuda.device(device):
             A.call(name, *args, ptr)
+
+
+# What a call checks depends on its tensors' layouts alone, so a layout that
+# passed is remembered with what was derived from it; addresses and contents
+# are read at every call.
+_LAYOUTS: dict = {}
+
+
+def _layout(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _remember(key, value):
+    if len(_LAYOUTS) >= 4096:
+        _LAYOUTS.clear()
+    _LAYOUTS[key] = value
+    return value
 
 
 def _same(who: str, first, *tensors) -> None:
@@ -111,27 +128,43 @@ def rope(x, pos, freqs, out, x2=None, out2=None, mscale: float = 1.0, interleave
     same batch, n and d goes along in the same launch.  `pos` is int64 (n,) or
     (batch, n).  Pairs are the halves of the rotated dims, or neighbours when
     `interleaved`.  `inverse` turns back: the gradient.  out may be x."""
+    key = ("rope", _layout(x), _layout(out), _layout(x2), _layout(out2), _layout(pos), _layout(freqs))
+    known = _LAYOUTS.get(key)
+    if known is None:
+        known = _remember(key, _rope_layout(x, pos, freqs, out, x2, out2))
+    first, second, sizes, pos_stride = known
+    tensors = _ROPE.pack(x.data_ptr(), out.data_ptr(), *first)
+    if second is not None:
+        tensors += _ROPE.pack(x2.data_ptr(), out2.data_ptr(), *second)
+    _run("amc_rope", x.device, stream, tensors, *sizes, pos.data_ptr(), pos_stride, freqs.data_ptr(), mscale,
+         int(interleaved), int(inverse))
+
+
+_ROPE = struct.Struct("=2Q7q")
+assert _ROPE.size == C.sizeof(A.RopeTensor)
+
+
+def _rope_layout(x, pos, freqs, out, x2, out2):
+    """Checks rope's tensors; (heads and strides of each tensor, the entry point's sizes, the stride of pos)."""
     import torch
     B, _, n, d = x.shape if x.dim() == 4 else (0, 0, 0, 0)
     pairs = [(x, out)] if x2 is None else [(x, out), (x2, out2)]
     if x2 is not None and out2 is None:
         raise ValueError("rope: x2 needs out2")
-    tensors = (A.RopeTensor * 2)()
-    for t, (a, o) in zip(tensors, pairs):
+    rows = []
+    for a, o in pairs:
         xs, os = _rows(a, "rope", (B, a.shape[1], n, d) if a.dim() == 4 else None), _rows(o, "rope", a.shape)
         _same("rope", x, a, o)
         _written(o, os, "rope")
-        t.x, t.out, t.heads = a.data_ptr(), o.data_ptr(), a.shape[1]
-        t.xs[:], t.os[:] = xs, os
+        rows.append((a.shape[1], *xs, *os))
     if pos.dtype != torch.int64 or tuple(pos.shape) not in ((n,), (B, n)) or (n > 1 and pos.stride(-1) != 1):
         raise ValueError("rope: positions are int64 (n,) or (batch, n) with unit stride along n")
     if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
         raise ValueError("rope: freqs is a contiguous float64 vector")
     if pos.device != x.device or freqs.device != x.device:
         raise ValueError("rope: positions and freqs live on the tensors' device")
-    _run("amc_rope", x.device, stream, tensors, len(pairs), _dtype(x, "rope"), B, n, d, 2 * freqs.shape[0],
-         pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0, freqs.data_ptr(), mscale, int(interleaved),
-         int(inverse))
+    return (rows[0], rows[1] if x2 is not None else None,
+            (len(pairs), _dtype(x, "rope"), B, n, d, 2 * freqs.shape[0]), pos.stride(0) if pos.dim() == 2 else 0)
 
 
 # ---------------------------------------------------------------------------- differential attention
@@ -157,41 +190,63 @@ def _diff_sizes(q, k, v, who: str):
     return (B, H2 // 2, K2 // 2, nq, nk, d, dv), qs, ks, vs
 
 
-def _lens(t, B: int, device, who: str) -> int:
+def _check_lens(t, B: int, device, who: str) -> None:
     import torch
-    if t is None:
-        return 0
-    if t.dtype != torch.int32 or tuple(t.shape) != (B,) or t.device != device or (B > 1 and t.stride(0) != 1):
+    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (B,) or t.device != device or
+                          (B > 1 and t.stride(0) != 1)):
         raise ValueError(f"{who}: lengths are int32 (batch,) on the tensors' device")
-    return t.data_ptr()
 
 
-def _workspace(t, device, who: str):
-    if t is None:
-        return 0, 0
-    if t.device != device or not t.is_contiguous():
-        raise ValueError(f"{who}: the workspace is contiguous, on the tensors' device")
-    return t.data_ptr(), t.numel() * t.element_size()
-
-
-def _diff_common(q, k, v, lam, q_lens, kv_lens, causal, scale, lam_init, who: str):
+def _diff_layout(q, k, v, lam, o, lse, o2, q_lens, kv_lens, workspace, grads, who: str):
+    """Checks the tensors of a call; (sizes, strides, workspace bytes) as the C
+    struct holds them.  grads: None, or (do, dq, dk, dv, dlam)."""
+    import torch
     (B, H, K, nq, nk, d, dv), qs, ks, vs = _diff_sizes(q, k, v, who)
     _same(who, q, lam)
     if lam.dim() != 3 or lam.shape[0] not in (1, H) or tuple(lam.shape[1:]) != (4, d) or not lam.is_contiguous():
         raise ValueError(f"{who}: lam is a contiguous (1 or H, 4, d) tensor")
-    head = (_dtype(q, who), int(bool(causal)), B, H, K, nq, nk, d, dv, lam.shape[0], scale, lam_init, q.data_ptr(),
-            k.data_ptr(), v.data_ptr(), lam.data_ptr(), _lens(q_lens, B, q.device, who),
-            _lens(kv_lens, B, q.device, who))
-    return head, (B, H, K, nq, nk, d, dv), (*qs, *ks, *vs)
-
-
-def _lse(lse, B, H, nq, device, who: str) -> int:
-    import torch
-    if lse is None:
-        return 0
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (B, 2 * H, nq) or not lse.is_contiguous() or lse.device != device:
+    _check_lens(q_lens, B, q.device, who)
+    _check_lens(kv_lens, B, q.device, who)
+    shape = (B, H, nq, dv)
+    os = _rows(o, who, shape)
+    o2s = _NONE3 if o2 is None else _rows(o2, who, shape)
+    _same(who, q, o, o2)
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (B, 2 * H, nq) or
+                            not lse.is_contiguous() or lse.device != q.device):
         raise ValueError(f"{who}: lse is a contiguous float32 (B, 2H, nq) tensor")
-    return lse.data_ptr()
+    if workspace is not None and (workspace.device != q.device or not workspace.is_contiguous()):
+        raise ValueError(f"{who}: the workspace is contiguous, on the tensors' device")
+    if grads is None:
+        written, more = ((o, os), (o2, o2s)), _NONE3 * 4
+    else:
+        do, dq, dk, dv_, dlam = grads
+        if lse is None or o2 is None:
+            raise ValueError(f"{who}: lse and o2 of the forward are needed")
+        dos = _rows(do, who, shape)
+        dqs, dks, dvs = _rows(dq, who, q.shape), _rows(dk, who, k.shape), _rows(dv_, who, v.shape)
+        _same(who, q, do, dq, dk, dv_, dlam)
+        if tuple(dlam.shape) != tuple(lam.shape) or not dlam.is_contiguous():
+            raise ValueError(f"{who}: dlam is contiguous and shaped like lam")
+        written, more = ((dq, dqs), (dk, dks), (dv_, dvs)), (*dos, *dqs, *dks, *dvs)
+    for t, s in written:
+        if t is not None:
+            _written(t, s, who)
+    return ((B, H, K, nq, nk, d, dv, lam.shape[0]), (*qs, *ks, *vs, *os, *o2s, *more),
+            0 if workspace is None else workspace.numel() * workspace.element_size(), _dtype(q, who))
+
+
+def _diff_call(who: str, q, k, v, lam, o, lse, o2, q_lens, kv_lens, workspace, grads, causal, scale, lam_init, stream):
+    key = (who, _layout(q), _layout(k), _layout(v), _layout(lam), _layout(o), _layout(lse), _layout(o2),
+           _layout(q_lens), _layout(kv_lens), _layout(workspace), None if grads is None else tuple(map(_layout, grads)))
+    known = _LAYOUTS.get(key)
+    if known is None:
+        known = _remember(key, _diff_layout(q, k, v, lam, o, lse, o2, q_lens, kv_lens, workspace, grads, who))
+    sizes, strides, ws_bytes, dtype = known
+    args = _DIFF.pack(dtype, int(bool(causal)), *sizes, scale, lam_init, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                      lam.data_ptr(), _ptr(q_lens), _ptr(kv_lens), o.data_ptr(), _ptr(o2), _ptr(lse),
+                      *((0, 0, 0, 0, 0) if grads is None else [t.data_ptr() for t in grads]), _ptr(workspace), ws_bytes,
+                      *strides)
+    _run("amc_" + who, q.device, stream, args)
 
 
 def diff_attention_workspace(q, k, v, backward: bool = False) -> int:
@@ -219,18 +274,8 @@ def diff_attention_fwd(q, k, v, lam, o, lse, lam_init: float, scale: float, caus
     float32 (or None) receives the row log-sum-exps; o2 (like o) the second
     map's part, which the backward needs.  One query row (or few) a head runs
     the single-token form, split over the keys."""
-    who = "diff_attention_fwd"
-    head, (B, H, K, nq, nk, d, dv), strides = _diff_common(q, k, v, lam, q_lens, kv_lens, causal, scale, lam_init, who)
-    os = _rows(o, who, (B, H, nq, dv))
-    o2s = _NONE3 if o2 is None else _rows(o2, who, o.shape)
-    _same(who, q, o, o2)
-    _written(o, os, who)
-    if o2 is not None:
-        _written(o2, o2s, who)
-    ws, ws_bytes = _workspace(workspace, q.device, who)
-    args = _DIFF.pack(*head, o.data_ptr(), _ptr(o2), _lse(lse, B, H, nq, q.device, who), 0, 0, 0, 0, 0, ws, ws_bytes,
-                      *strides, *os, *o2s, *_NONE3 * 4)
-    _run("amc_diff_attention_fwd", q.device, stream, args)
+    _diff_call("diff_attention_fwd", q, k, v, lam, o, lse, o2, q_lens, kv_lens, workspace, None, causal, scale,
+               lam_init, stream)
 
 
 def diff_attention_bwd(q, k, v, lam, o, o2, lse, do, dq, dk, dv, dlam, lam_init: float, scale: float,
@@ -239,23 +284,8 @@ def diff_attention_bwd(q, k, v, lam, o, o2, lse, do, dq, dk, dv, dlam, lam_init:
     o2 and lse: dq, dk, dv and dlam, shaped like their tensors, gradients of
     shared heads summed, zero behind the lengths.  No atomics: repeated calls
     give identical bits."""
-    who = "diff_attention_bwd"
-    head, (B, H, K, nq, nk, d, w), strides = _diff_common(q, k, v, lam, q_lens, kv_lens, causal, scale, lam_init, who)
-    shape = (B, H, nq, w)
-    os, o2s, dos = _rows(o, who, shape), _rows(o2, who, shape), _rows(do, who, shape)
-    dqs, dks, dvs = _rows(dq, who, q.shape), _rows(dk, who, k.shape), _rows(dv, who, v.shape)
-    _same(who, q, o, o2, do, dq, dk, dv, dlam)
-    for t, s in ((dq, dqs), (dk, dks), (dv, dvs)):
-        _written(t, s, who)
-    if tuple(dlam.shape) != tuple(lam.shape) or not dlam.is_contiguous():
-        raise ValueError(f"{who}: dlam is contiguous and shaped like lam")
-    if lse is None:
-        raise ValueError(f"{who}: lse of the forward is needed")
-    ws, ws_bytes = _workspace(workspace, q.device, who)
-    args = _DIFF.pack(*head, o.data_ptr(), o2.data_ptr(), _lse(lse, B, H, nq, q.device, who), do.data_ptr(),
-                      dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), ws, ws_bytes, *strides, *os, *o2s,
-                      *dos, *dqs, *dks, *dvs)
-    _run("amc_diff_attention_bwd", q.device, stream, args)
+    _diff_call("diff_attention_bwd", q, k, v, lam, o, lse, o2, q_lens, kv_lens, workspace, (do, dq, dk, dv, dlam),
+               causal, scale, lam_init, stream)
 
 
 # ---------------------------------------------------------------------------- AdamW

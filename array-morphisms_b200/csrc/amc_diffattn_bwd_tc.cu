@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
   uint64_t* acc_full = s_full + 4;
   uint32_t* tslot = (uint32_t*)(sm + L::bar + 192);
   volatile int* abort_flag = (volatile int*)(sm + L::bar + 196);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = (int)warp_uniform(tid >> 5), lane = tid & 31;
   // key tiles of one head are launched first tile first: with a causal mask
   // those have the most rows
   const int per = p.kv_heads * p.batch, group = p.heads / p.kv_heads;
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
   const DiffLens len = diff_lens(p, b);
   const int first = diff_first_row(len, p.causal, k0) / 64 * 64;
   const int nth = first < len.nq ? (len.nq - first + 63) / 64 : 0;   // tiles a head
-  const int nt = nth * group;
+  const int nt = (int)warp_uniform(nth * group);
   if (tid == 0) {
     mbar_init(kv_full, 1);
     for (int i = 0; i < kStages; ++i) {
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tslot;
+  const uint32_t tmem = warp_uniform(*tslot);
   const uint32_t t_dv = tmem + 256, t_dk = tmem + 384;
 
   if (warp == 8) {
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
       }
     }
   } else if (warp == 9) {
-    if (lane == 0 && nt > 0) {
+    if (nt > 0) {
       const uint32_t id = idesc_f16(128, 64, kBf16, false, false);
       const uint32_t id_dk = idesc_f16(128, 64, kBf16, false, true);
       const uint32_t id_dv = idesc_f16(128, NV, kBf16, false, true);
@@ -176,18 +176,23 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
       const int ksteps = (p.d + 15) / 16, vsteps = (p.dv + 15) / 16;
       auto issue_s = [&](int i) {
         const uint64_t st = desc_add(fd, (i % kStages) * L::stage);
+#pragma unroll
         for (int m = 0; m < 2; ++m)
-          for (int k = 0; k < ksteps; ++k)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < ksteps)
             mma_f16(tmem + (i & 1) * 128 + m * 64, desc_add(kd, m * 16384 + k * 32), desc_add(st, m * 8192 + k * 32), id,
                     k > 0);
-        mma_commit(s_full);
+        mma_commit_warp(s_full);
       };
       auto issue_g = [&](int i) {
         const uint64_t st = desc_add(fd, (i % kStages) * L::stage + 16384);
-        for (int k = 0; k < vsteps; ++k)
+#pragma unroll
+        for (int k = 0; k < NV / 16; ++k)
+          if (k < vsteps)
           mma_f16(tmem + (~i & 1) * 128, desc_add(vd, (k >> 2) * 16384 + (k & 3) * 32),
                   desc_add(st, (k >> 2) * 8192 + (k & 3) * 32), id, k > 0);
-        mma_commit(g_full);
+        mma_commit_warp(g_full);
       };
       // A operands: warpgroup w wrote rows 32 w .. 32 w + 31 of the tile (K
       // steps 2 w and 2 w + 1) at columns 32 w (+16 for dS_1) of the buffers
@@ -201,9 +206,9 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
           mma_f16_ts(t_dk, a + 16, desc_add(st, k * 2048), id_dk, i > 0 || k > 0);
           mma_f16_ts(t_dk + 64, a + 64, desc_add(st, 8192 + k * 2048), id_dk, i > 0 || k > 0);
         }
-        mma_commit(&f_empty[i % kStages]);
+        mma_commit_warp(&f_empty[i % kStages]);
       };
-      bool ok = mbar_wait(kv_full, 0) && mbar_wait(&f_full[0], 0);
+      bool ok = warp_wait(kv_full, 0) && warp_wait(&f_full[0], 0);
       if (ok) {
         tc_fence_after();
         issue_s(0);
@@ -212,17 +217,17 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
       for (int i = 0; i < nt && ok; ++i) {
         const bool more = i + 1 < nt;
         if (more) {
-          if (!mbar_wait(&f_full[(i + 1) % kStages], (uint32_t)((i + 1) / kStages) & 1u) ||
-              !mbar_wait(g_read, (uint32_t)i & 1u)) { ok = false; break; }
+          if (!warp_wait(&f_full[(i + 1) % kStages], (uint32_t)((i + 1) / kStages) & 1u) ||
+              !warp_wait(g_read, (uint32_t)i & 1u)) { ok = false; break; }
           tc_fence_after();
           issue_s(i + 1);
         }
-        if (!mbar_wait(p_full, (uint32_t)i & 1u) || *abort_flag) { ok = false; break; }
+        if (!warp_wait(p_full, (uint32_t)i & 1u) || warp_uniform(*abort_flag)) { ok = false; break; }
         tc_fence_after();
         issue_acc(i);
         if (more) issue_g(i + 1);
       }
-      if (ok) mma_commit(acc_full);
+      if (ok) mma_commit_warp(acc_full);
       else *abort_flag = 1;
     }
   } else if (warp < 8) {
@@ -380,14 +385,14 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
   uint32_t* tslot = (uint32_t*)(sm + L::bar + 192);
   volatile int* abort_flag = (volatile int*)(sm + L::bar + 196);
   float* red = (float*)(sm + L::bar + 208);  // [8]
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = (int)warp_uniform(tid >> 5), lane = tid & 31;
   const int per = p.heads * p.batch, tiles = (p.nq + 127) / 128;
   const int tile = tiles - 1 - (int)(blockIdx.x / per), h = blockIdx.x % per % p.heads, b = blockIdx.x % per / p.heads;
   const int g = h / (p.heads / p.kv_heads), r0 = tile * 128;
   const DiffLens len = diff_lens(p, b);
   const int last = min(r0 + 128, len.nq) - 1;
   const int kend = last >= r0 ? diff_limit(len, p.causal, last) : 0;
-  const int nt = (kend + 63) / 64;
+  const int nt = (int)warp_uniform((kend + 63) / 64);
   if (tid == 0) {
     mbar_init(q_full, 1);
     for (int i = 0; i < kStages; ++i) {
@@ -407,7 +412,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tslot;
+  const uint32_t tmem = warp_uniform(*tslot);
   const uint32_t t_dq = tmem + 384;
 
   if (warp == 8) {
@@ -426,30 +431,35 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
       }
     }
   } else if (warp == 9) {
-    if (lane == 0 && nt > 0) {
+    if (nt > 0) {
       const uint32_t id = idesc_f16(128, 64, kBf16, false, false);
       const uint32_t id_dq = idesc_f16(128, 64, kBf16, false, true);
       const uint64_t qd = sdesc(smem_addr(sm + L::q), 16, 1024), gd = sdesc(smem_addr(sm + L::g), 16, 1024);
       const uint64_t fd = sdesc(smem_addr(sm + L::f), 16, 1024), fmn = sdesc_mn16(smem_addr(sm + L::f), 8192);
       const int ksteps = (p.d + 15) / 16, vsteps = (p.dv + 15) / 16;
       auto issue_s = [&](int j) -> bool {
-        if (!mbar_wait(&f_full[j % kStages], (uint32_t)(j / kStages) & 1u)) return false;
+        if (!warp_wait(&f_full[j % kStages], (uint32_t)(j / kStages) & 1u)) return false;
         tc_fence_after();
         const uint64_t st = desc_add(fd, (j % kStages) * L::stage);
         const uint32_t x = tmem + (j & 1) * 192;
+#pragma unroll
         for (int m = 0; m < 2; ++m)
-          for (int k = 0; k < ksteps; ++k)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < ksteps)
             mma_f16(x + m * 64, desc_add(qd, m * 16384 + k * 32), desc_add(st, m * 8192 + k * 32), id, k > 0);
-        for (int k = 0; k < vsteps; ++k)
+#pragma unroll
+        for (int k = 0; k < NV / 16; ++k)
+          if (k < vsteps)
           mma_f16(x + 128, desc_add(gd, (k >> 2) * 16384 + (k & 3) * 32),
                   desc_add(st, 16384 + (k >> 2) * 8192 + (k & 3) * 32), id, k > 0);
-        mma_commit(&s_full[j & 1]);
+        mma_commit_warp(&s_full[j & 1]);
         return true;
       };
-      bool ok = mbar_wait(q_full, 0);
+      bool ok = warp_wait(q_full, 0);
       for (int j = 0; j < 2 && j < nt && ok; ++j) ok = issue_s(j);
       for (int j = 0; j < nt && ok; ++j) {
-        if (!mbar_wait(&p_full[j & 1], (uint32_t)(j >> 1) & 1u) || *abort_flag) { ok = false; break; }
+        if (!warp_wait(&p_full[j & 1], (uint32_t)(j >> 1) & 1u) || warp_uniform(*abort_flag)) { ok = false; break; }
         tc_fence_after();
         const uint64_t st = desc_add(fmn, (j % kStages) * L::stage);
         const uint32_t x = tmem + (j & 1) * 192;
@@ -459,10 +469,10 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
           mma_f16_ts(t_dq, a, desc_add(st, k * 2048), id_dq, j > 0 || k > 0);
           mma_f16_ts(t_dq + 64, a + 64, desc_add(st, 8192 + k * 2048), id_dq, j > 0 || k > 0);
         }
-        mma_commit(&f_empty[j % kStages]);
+        mma_commit_warp(&f_empty[j % kStages]);
         if (j + 2 < nt) ok = issue_s(j + 2);
       }
-      if (ok) mma_commit(acc_full);
+      if (ok) mma_commit_warp(acc_full);
       else *abort_flag = 1;
     }
   } else if (warp < 8) {
