@@ -216,39 +216,57 @@ __global__ void __launch_bounds__(256, 1) k_diff_fwd_simt(const __grid_constant_
   if (p.o2) store_rows<T, R, DV / 16>((T*)p.o2 + b * p.o2s[0] + h * p.o2s[1], p.o2s[2], o[1], 1.f, r0, p.nq, p.dv, ty, tx);
 }
 
-// One warp per row: lse2 and dsum from lse, o, o2 and dO; lam of every head.
-template <typename T>
+// nlse and nsum from lse, o, o2 and dO, and lam of every head.  A row is
+// shared by LANES lanes of V elements a load (16 bytes where every row is
+// aligned): the pass reads three output-sized tensors once and is bound by
+// that.
+template <typename T, int V, int LANES>
 __global__ void __launch_bounds__(256) k_diff_bwd_rows(const __grid_constant__ amc_diff_attention p,
                                                        const __grid_constant__ DiffBwdWork w) {
-  const int lane = threadIdx.x & 31;
-  const int i = blockIdx.x * 8 + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
-  if (i >= p.nq) return;
+  constexpr int kRowsPerCta = 256 / LANES;
+  const int sub = threadIdx.x % LANES, h = blockIdx.y, b = blockIdx.z;
+  const int i = blockIdx.x * kRowsPerCta + threadIdx.x / LANES;
   const float lam = lam_of<T>(p, h);
-  if (i == 0 && b == 0 && lane == 0) w.lam[h] = lam;
+  if (blockIdx.x == 0 && b == 0 && threadIdx.x == 0) w.lam[h] = lam;
   const DiffLens len = diff_lens(p, b);
-  float2 e = make_float2(INFINITY, INFINITY), r = make_float2(0.f, 0.f);
-  if (diff_limit(len, p.causal, i) > 0) {
+  const bool live = i < p.nq && diff_limit(len, p.causal, i) > 0;
+  float d = 0.f, d2 = 0.f;
+  if (live) {
     const T* o = (const T*)p.o + b * p.os[0] + h * p.os[1] + (int64_t)i * p.os[2];
     const T* o2 = (const T*)p.o2 + b * p.o2s[0] + h * p.o2s[1] + (int64_t)i * p.o2s[2];
     const T* go = (const T*)p.d_o + b * p.dos[0] + h * p.dos[1] + (int64_t)i * p.dos[2];
-    float d = 0.f, d2 = 0.f;
-    for (int c = lane; c < p.dv; c += 32) {
-      const float x = to_f32(go[c]);
-      d = fmaf(x, to_f32(o[c]), d);
-      d2 = fmaf(x, to_f32(o2[c]), d2);
+    for (int c = sub * V; c < p.dv; c += LANES * V) {
+      if constexpr (V == 8) {
+        const uint4 x = *reinterpret_cast<const uint4*>(go + c), y = *reinterpret_cast<const uint4*>(o + c),
+                    z = *reinterpret_cast<const uint4*>(o2 + c);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 a = unpack2<T>(xs[k]), e = unpack2<T>(ys[k]), f = unpack2<T>(zs[k]);
+          d = fmaf(a.x, e.x, fmaf(a.y, e.y, d));
+          d2 = fmaf(a.x, f.x, fmaf(a.y, f.y, d2));
+        }
+      } else {
+        const float x = to_f32(go[c]);
+        d = fmaf(x, to_f32(o[c]), d);
+        d2 = fmaf(x, to_f32(o2[c]), d2);
+      }
     }
-    for (int s = 16; s > 0; s >>= 1) {
-      d += __shfl_xor_sync(0xffffffffu, d, s);
-      d2 += __shfl_xor_sync(0xffffffffu, d2, s);
-    }
-    const float* lse = p.lse + ((int64_t)b * 2 * p.heads + 2 * h) * p.nq + i;
-    e = make_float2(lse[0] * kLog2e, lse[p.nq] * kLog2e);
-    r = make_float2(fmaf(lam, d2, d), d2);   // dO . O_1 = dO . (O + lam O_2)
   }
-  if (lane == 0) {
+#pragma unroll
+  for (int s = LANES / 2; s > 0; s >>= 1) {
+    d += __shfl_xor_sync(0xffffffffu, d, s);
+    d2 += __shfl_xor_sync(0xffffffffu, d2, s);
+  }
+  if (sub == 0 && i < w.pitch) {   // the padding too: the gradients multiply it by 0
+    const float* lse = p.lse + ((int64_t)b * 2 * p.heads + 2 * h) * p.nq + i;
     const int64_t at = ((int64_t)b * p.heads + h) * w.pitch + i;
-    w.lse2[at] = e;
-    w.dsum[at] = r;
+    float* e = reinterpret_cast<float*>(w.nlse + at / 2) + (at & 1);
+    float* r = reinterpret_cast<float*>(w.nsum + at / 2) + (at & 1);
+    e[0] = live ? -lse[0] * kLog2e : -INFINITY;
+    e[2] = live ? -lse[p.nq] * kLog2e : -INFINITY;
+    r[0] = -fmaf(lam, d2, d);   // dO . O_1 = dO . (O + lam O_2)
+    r[2] = -d2;
   }
 }
 
@@ -291,15 +309,15 @@ __global__ void __launch_bounds__(256, 1) k_diff_dkv_simt(const __grid_constant_
         for (int i = 0; i < R; ++i) {
           const int r = r0 + ty + 16 * i;
           const int lim = diff_limit(len, p.causal, r);
-          const int64_t at = ((int64_t)b * p.heads + h) * wk.pitch + r;
-          const float2 e = lim > 0 ? wk.lse2[at] : make_float2(INFINITY, INFINITY);
-          const float2 ds = lim > 0 ? wk.dsum[at] : make_float2(0.f, 0.f);
+          const int64_t at = ((int64_t)b * p.heads + h) * wk.pitch;
+          const float e = lim > 0 ? diff_row(wk.nlse, at, r, m) : -INFINITY;
+          const float ds = lim > 0 ? diff_row(wk.nsum, at, r, m) : 0.f;
 #pragma unroll
           for (int j = 0; j < R; ++j) {
-            const float pr = k0 + tx + 16 * j < lim ? exp2f(fmaf(s[i][j], c2, -(m ? e.y : e.x))) : 0.f;
+            const float pr = k0 + tx + 16 * j < lim ? exp2f(fmaf(s[i][j], c2, e)) : 0.f;
             const float w = m ? -lam * pr : pr;
             both[i][j] = m ? both[i][j] + w : w;
-            sS[m * TT * L::PP + (ty + 16 * i) * L::PP + tx + 16 * j] = w * (gv[i][j] - (m ? ds.y : ds.x));
+            sS[m * TT * L::PP + (ty + 16 * i) * L::PP + tx + 16 * j] = w * (gv[i][j] + ds);
           }
         }
       }
@@ -346,9 +364,13 @@ __global__ void __launch_bounds__(256, 1) k_diff_dq_simt(const __grid_constant__
   for (int i = 0; i < R; ++i) {
     const int r = r0 + ty + 16 * i;
     lim[i] = diff_limit(len, p.causal, r);
-    const int64_t at = ((int64_t)b * p.heads + h) * wk.pitch + r;
-    e[i] = lim[i] > 0 ? wk.lse2[at] : make_float2(INFINITY, INFINITY);
-    ds[i] = lim[i] > 0 ? wk.dsum[at] : make_float2(0.f, 0.f);
+    const int64_t at = ((int64_t)b * p.heads + h) * wk.pitch;
+    e[i] = make_float2(-INFINITY, -INFINITY);
+    ds[i] = make_float2(0.f, 0.f);
+    if (lim[i] > 0) {
+      e[i] = make_float2(diff_row(wk.nlse, at, r, 0), diff_row(wk.nlse, at, r, 1));
+      ds[i] = make_float2(diff_row(wk.nsum, at, r, 0), diff_row(wk.nsum, at, r, 1));
+    }
   }
   float dq[2][R][DM / 16] = {}, pg = 0.f;
   const int last = min(r0 + TT, len.nq) - 1;
@@ -370,10 +392,10 @@ __global__ void __launch_bounds__(256, 1) k_diff_dq_simt(const __grid_constant__
       for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-          const float pr = k0 + tx + 16 * j < lim[i] ? exp2f(fmaf(s[i][j], c2, -(m ? e[i].y : e[i].x))) : 0.f;
+          const float pr = k0 + tx + 16 * j < lim[i] ? exp2f(fmaf(s[i][j], c2, m ? e[i].y : e[i].x)) : 0.f;
           if (m) part = fmaf(pr, gv[i][j], part);
           sS[m * TT * L::PP + (ty + 16 * i) * L::PP + tx + 16 * j] =
-              (m ? -lam * pr : pr) * (gv[i][j] - (m ? ds[i].y : ds[i].x));
+              (m ? -lam * pr : pr) * (gv[i][j] + (m ? ds[i].y : ds[i].x));
         }
     }
     pg += part;
@@ -470,11 +492,17 @@ int launch_diff_fwd_simt(const amc_diff_attention& p, cudaStream_t s) {
 
 int launch_diff_bwd_rows(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s) {
   if (!p.nq) return AMC_OK;
-  return by_type(p.dtype, [&](auto t) {
-    k_diff_bwd_rows<decltype(t)><<<dim3((p.nq + 7) / 8, p.heads, p.batch), 256, 0, s>>>(p, w);
-    AMC_CUDA(cudaGetLastError());
-    return AMC_OK;
-  });
+  bool wide = p.dtype != AMC_F32 && p.dv % 8 == 0 && !(((uintptr_t)p.o | (uintptr_t)p.o2 | (uintptr_t)p.d_o) & 15);
+  const int64_t extent[3] = {p.batch, p.heads, p.nq};
+  for (int j = 0; j < 3; ++j) wide = wide && (extent[j] == 1 || (p.os[j] % 8 == 0 && p.o2s[j] % 8 == 0 && p.dos[j] % 8 == 0));
+  const dim3 grid16((w.pitch + 15) / 16, p.heads, p.batch), grid8((w.pitch + 7) / 8, p.heads, p.batch);
+  if (wide && p.dtype == AMC_BF16) k_diff_bwd_rows<__nv_bfloat16, 8, 16><<<grid16, 256, 0, s>>>(p, w);
+  else if (wide) k_diff_bwd_rows<__half, 8, 16><<<grid16, 256, 0, s>>>(p, w);
+  else if (p.dtype == AMC_F32) k_diff_bwd_rows<float, 1, 32><<<grid8, 256, 0, s>>>(p, w);
+  else if (p.dtype == AMC_BF16) k_diff_bwd_rows<__nv_bfloat16, 1, 32><<<grid8, 256, 0, s>>>(p, w);
+  else k_diff_bwd_rows<__half, 1, 32><<<grid8, 256, 0, s>>>(p, w);
+  AMC_CUDA(cudaGetLastError());
+  return AMC_OK;
 }
 
 int launch_diff_bwd_simt(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s) {

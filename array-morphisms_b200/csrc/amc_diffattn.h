@@ -26,33 +26,39 @@ __device__ __forceinline__ int diff_first_row(const DiffLens& l, int causal, int
   return causal ? min(l.nq, max(0, j - (l.nk - l.nq))) : 0;
 }
 
-// Workspace of the backward.  Per (batch, head, row) the pairs
-//   lse2 = both maps' lse * log2 e, +inf where the row is empty, so that
-//          exp2(s - lse) is 0
-//   dsum = D_m = rowsum(dO * O_m) of both maps
+// Workspace of the backward.  For every two rows (2 r, 2 r + 1) of a (batch,
+// head) one float4 of each kind, negated for the fused operations that use
+// them, both rows of map 1 and then both of map 2:
+//   nlse = -lse * log2 e, -inf where the row is empty, so that
+//          exp2(s + nlse) is 0
+//   nsum = -D_m, D_m = rowsum(dO * O_m)
 // (rows padded to a multiple of 4, so that a tile of them is a bulk copy),
 // then lam of every head, then one partial of sum P_2 G for every (head,
 // batch, row tile).
 constexpr int kDiffTile = 32;
 struct DiffBwdWork {
-  float2* lse2;
-  float2* dsum;
+  float4* nlse;
+  float4* nsum;
   float* lam;
   float* partials;
-  int pitch;
+  int pitch;   // rows of a (batch, head)
 };
+// The value of row r of map m in such an array.
+__device__ __forceinline__ float diff_row(const float4* x, int64_t first_row, int r, int m) {
+  return reinterpret_cast<const float*>(x + (first_row + r) / 2)[2 * m + (r & 1)];
+}
 inline int diff_row_pitch(const amc_diff_attention& p) { return (p.nq + 3) & ~3; }
 inline size_t diff_bwd_bytes(const amc_diff_attention& p) {
   const size_t rows = (size_t)p.batch * p.heads * diff_row_pitch(p);
   const size_t partials = (size_t)p.batch * p.heads * ((p.nq + kDiffTile - 1) / kDiffTile);
-  return 2 * rows * sizeof(float2) + (size_t)p.heads * sizeof(float) + partials * sizeof(float);
+  return rows * sizeof(float4) + (size_t)p.heads * sizeof(float) + partials * sizeof(float);
 }
 inline DiffBwdWork diff_bwd_work(const amc_diff_attention& p) {
   const size_t rows = (size_t)p.batch * p.heads * diff_row_pitch(p);
   DiffBwdWork w;
-  w.lse2 = (float2*)p.workspace;
-  w.dsum = w.lse2 + rows;
-  w.lam = (float*)(w.dsum + rows);
+  w.nlse = (float4*)p.workspace;
+  w.nsum = w.nlse + rows / 2;
+  w.lam = (float*)(w.nsum + rows / 2);
   w.partials = w.lam + p.heads;
   w.pitch = diff_row_pitch(p);
   return w;

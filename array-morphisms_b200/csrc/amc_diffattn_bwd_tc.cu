@@ -1,6 +1,6 @@
 // Differential attention gradients on the tensor cores (sm_100a, tcgen05
 // kind::f16), 16-bit tensors with d <= 64 and dv <= 128, both multiples of 8:
-//   P_m = 2^(scale log2e Q_m K_m^T - lse2_m)      G = dO V^T
+//   P_m = 2^(scale log2e Q_m K_m^T + nlse_m)      G = dO V^T
 //   dS_1 = P_1 (G - D_1)                          dS_2 = lam P_2 (D_2 - G)
 //   dV = (P_1 - lam P_2)^T dO   dK_m = scale dS_m^T Q_m   dQ_m = scale dS_m K_m
 // Both maps share G, and the difference of the maps is taken before dV's
@@ -16,7 +16,9 @@
 // the scores they came from; a thread writes only columns it has read.  A
 // 16-bit tile in the 128-byte swizzle serves K-major (its rows as N) and
 // MN-major (its rows as K) alike, so one copy of Q, K and dO feeds both
-// products.  Two warpgroups share a tile, 32 of its 64 columns each.
+// products.  Four warpgroups share a tile, 16 of its 64 columns each: with two
+// of them, 32 columns a thread, the two warps of a scheduler could not cover
+// each other's latencies.
 // Every wait is bounded; on expiry the kernel records AMC_ERR_TIMEOUT, drains
 // and returns.
 #include <cmath>
@@ -32,8 +34,8 @@ using namespace tc;
 
 namespace {
 
-constexpr int kThreadsB = 384;       // warps 0-7 rows (two warpgroups), 8 loads, 9 issues
-constexpr int kRowThreads = 256;
+constexpr int kThreadsB = 576;       // warps 0-15 rows (four warpgroups), 16 loads, 17 issues
+constexpr int kRowThreads = 512, kRowWarps = 16;
 constexpr int kStages = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -44,7 +46,7 @@ struct KvSmem {
   static constexpr int v = 32768;
   static constexpr int f = v + NV / 64 * 16384;               // stages: Q_1, Q_2 (8 KB each), dO, pairs
   static constexpr int stage = 16384 + NV / 64 * 8192;
-  static constexpr int r = f + kStages * stage;               // stages: 64 lse2 pairs, 64 dsum pairs
+  static constexpr int r = f + kStages * stage;               // stages: 32 nlse, 32 nsum (two rows each)
   static constexpr int bar = r + kStages * 1024;
   static constexpr int bytes = bar + 256 + 1024;
 };
@@ -56,7 +58,7 @@ struct QSmem {
   static constexpr int f = g + NV / 64 * 16384;               // stages: K_1, K_2 (8 KB each), V
   static constexpr int stage = 16384 + NV / 64 * 8192;
   static constexpr int bar = f + kStages * stage;
-  static constexpr int bytes = bar + 256 + 1024;
+  static constexpr int bytes = bar + 320 + 1024;
 };
 static_assert(KvSmem<128>::bytes <= 232448 && QSmem<128>::bytes <= 232448, "shared memory");
 
@@ -105,8 +107,8 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
   uint64_t* f_empty = f_full + kStages;      // [kStages] their products are done and the pairs read
   uint64_t* s_full = f_empty + kStages;      // S(i) complete
   uint64_t* g_full = s_full + 1;             // G(i) complete
-  uint64_t* g_read = s_full + 2;             // the threads have read G(i) (count 256)
-  uint64_t* p_full = s_full + 3;             // operands of tile i written (count 256)
+  uint64_t* g_read = s_full + 2;             // the threads have read G(i) (16 warps)
+  uint64_t* p_full = s_full + 3;             // operands of tile i written (16 warps)
   uint64_t* acc_full = s_full + 4;
   uint32_t* tslot = (uint32_t*)(sm + L::bar + 192);
   volatile int* abort_flag = (volatile int*)(sm + L::bar + 196);
@@ -119,16 +121,20 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
   const int first = diff_first_row(len, p.causal, k0) / 64 * 64;
   const int nth = first < len.nq ? (len.nq - first + 63) / 64 : 0;   // tiles a head
   const int nt = (int)warp_uniform(nth * group);
+  // pairs behind the tensor's rows are never loaded: they count as zeros
+  for (int i = tid; i < kStages * 64; i += kThreadsB)
+    reinterpret_cast<float4*>(sm + L::r)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  fence_proxy_async();
   if (tid == 0) {
     mbar_init(kv_full, 1);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&f_full[i], 1);
-      mbar_init(&f_empty[i], 1 + kRowThreads);
+      mbar_init(&f_empty[i], 1 + kRowWarps);
     }
     mbar_init(s_full, 1);
     mbar_init(g_full, 1);
-    mbar_init(g_read, kRowThreads);
-    mbar_init(p_full, kRowThreads);
+    mbar_init(g_read, kRowWarps);
+    mbar_init(p_full, kRowWarps);
     mbar_init(acc_full, 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -141,7 +147,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
   const uint32_t tmem = warp_uniform(*tslot);
   const uint32_t t_dv = tmem + 256, t_dk = tmem + 384;
 
-  if (warp == 8) {
+  if (warp == 16) {
     if (lane == 0 && nt > 0) {
       mbar_expect_tx(kv_full, 32768 + NV / 64 * 16384);
       for (int m = 0; m < 2; ++m) tma_load_4d(sm + L::k + m * 16384, &mK, 0, k0, 2 * g + m, b, kv_full);
@@ -156,9 +162,9 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
         mbar_expect_tx(&f_full[s], L::stage + rows * 16);
         for (int m = 0; m < 2; ++m) tma_load_4d(st + m * 8192, &mQ, 0, r0, 2 * h + m, b, &f_full[s]);
         for (int c = 0; c < NV / 64; ++c) tma_load_4d(st + 16384 + c * 8192, &mG, 64 * c, r0, h, b, &f_full[s]);
-        const int64_t at = ((int64_t)b * p.heads + h) * wk.pitch + r0;
-        bulk_load_1d(sm + L::r + s * 1024, wk.lse2 + at, rows * 8, &f_full[s]);
-        bulk_load_1d(sm + L::r + s * 1024 + 512, wk.dsum + at, rows * 8, &f_full[s]);
+        const int64_t at = (((int64_t)b * p.heads + h) * wk.pitch + r0) / 2;
+        bulk_load_1d(sm + L::r + s * 1024, wk.nlse + at, rows * 8, &f_full[s]);
+        bulk_load_1d(sm + L::r + s * 1024 + 512, wk.nsum + at, rows * 8, &f_full[s]);
         r0 += 64;
         if (r0 >= len.nq) {
           r0 = first;
@@ -166,21 +172,19 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
         }
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == 17) {
     if (nt > 0) {
       const uint32_t id = idesc_f16(128, 64, kBf16, false, false);
       const uint32_t id_dk = idesc_f16(128, 64, kBf16, false, true);
       const uint32_t id_dv = idesc_f16(128, NV, kBf16, false, true);
       const uint64_t kd = sdesc(smem_addr(sm + L::k), 16, 1024), vd = sdesc(smem_addr(sm + L::v), 16, 1024);
       const uint64_t fd = sdesc(smem_addr(sm + L::f), 16, 1024), fmn = sdesc_mn16(smem_addr(sm + L::f), 8192);
-      const int ksteps = (p.d + 15) / 16, vsteps = (p.dv + 15) / 16;
       auto issue_s = [&](int i) {
         const uint64_t st = desc_add(fd, (i % kStages) * L::stage);
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (k < ksteps)
             mma_f16(tmem + (i & 1) * 128 + m * 64, desc_add(kd, m * 16384 + k * 32), desc_add(st, m * 8192 + k * 32), id,
                     k > 0);
         mma_commit_warp(s_full);
@@ -189,23 +193,28 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
         const uint64_t st = desc_add(fd, (i % kStages) * L::stage + 16384);
 #pragma unroll
         for (int k = 0; k < NV / 16; ++k)
-          if (k < vsteps)
           mma_f16(tmem + (~i & 1) * 128, desc_add(vd, (k >> 2) * 16384 + (k & 3) * 32),
                   desc_add(st, (k >> 2) * 8192 + (k & 3) * 32), id, k > 0);
         mma_commit_warp(g_full);
       };
-      // A operands: warpgroup w wrote rows 32 w .. 32 w + 31 of the tile (K
-      // steps 2 w and 2 w + 1) at columns 32 w (+16 for dS_1) of the buffers
+      // A operands: warpgroup k wrote rows 16 k .. 16 k + 15 of the tile (K
+      // step k) at columns 16 k (+8 for dS_1) of the buffers
       auto issue_acc = [&](int i) {
         const uint64_t st = desc_add(fmn, (i % kStages) * L::stage);
         const uint32_t x = tmem + (i & 1) * 128;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t a = x + (k >> 1) * 32 + (k & 1) * 8;
+          const uint32_t a = x + k * 16;
           mma_f16_ts(t_dv, a, desc_add(st, 16384 + k * 2048), id_dv, i > 0 || k > 0);
-          mma_f16_ts(t_dk, a + 16, desc_add(st, k * 2048), id_dk, i > 0 || k > 0);
-          mma_f16_ts(t_dk + 64, a + 64, desc_add(st, 8192 + k * 2048), id_dk, i > 0 || k > 0);
+          mma_f16_ts(t_dk, a + 8, desc_add(st, k * 2048), id_dk, i > 0 || k > 0);
         }
+      };
+      auto issue_acc2 = [&](int i) {
+        const uint64_t st = desc_add(fmn, (i % kStages) * L::stage);
+        const uint32_t x = tmem + (i & 1) * 128;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_f16_ts(t_dk + 64, x + 64 + k * 16, desc_add(st, 8192 + k * 2048), id_dk, i > 0 || k > 0);
         mma_commit_warp(&f_empty[i % kStages]);
       };
       bool ok = warp_wait(kv_full, 0) && warp_wait(&f_full[0], 0);
@@ -225,123 +234,130 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
         if (!warp_wait(p_full, (uint32_t)i & 1u) || warp_uniform(*abort_flag)) { ok = false; break; }
         tc_fence_after();
         issue_acc(i);
-        if (more) issue_g(i + 1);
+        if (more) issue_g(i + 1);   // into the buffer that dV and dK_1 have read; dK_2 reads the other
+        issue_acc2(i);
       }
       if (ok) mma_commit_warp(acc_full);
       else *abort_flag = 1;
     }
-  } else if (warp < 8) {
-    // one thread per key; warpgroup w takes rows 32 w .. 32 w + 31 of a tile
+  } else {
+    // one thread per key; warpgroup w takes rows 16 w .. 16 w + 15 of a tile
     const int w = warp >> 2, t = tid & 127;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const float c2 = p.scale * kLog2e;
     const int fr = diff_first_row(len, p.causal, k0 + t);
     const int fr_all = diff_first_row(len, p.causal, k0 + 127);   // from here on every key of the tile is seen
+    const float2 cc = make_float2(c2, c2);
     bool ok = true;
     int h = g * group, r0 = first;
-    float lam = nt > 0 ? wk.lam[h] : 0.f;
-    for (int i = 0; i < nt; ++i) {
+    float nlam = nt > 0 ? -wk.lam[h] : 0.f;
+    if (nt > 0) ok = __all_sync(0xffffffffu, mbar_wait(&f_full[0], 0));
+    for (int i = 0; i < nt && ok; ++i) {
       const int s = i % kStages;
-      const uint32_t x = tmem + (i & 1) * 128 + lane_base + 32 * w;
-      ok = __all_sync(0xffffffffu, mbar_wait(&f_full[s], (uint32_t)(i / kStages) & 1u) &&
-                                       mbar_wait(s_full, (uint32_t)i & 1u) && !*abort_flag);
+      const uint32_t x = tmem + (i & 1) * 128 + lane_base + 16 * w;
+      // The row pairs come from shared memory, whose port the products'
+      // operands keep busy: they are read before each wait, not after it.
+      const float4* le = reinterpret_cast<const float4*>(sm + L::r + s * 1024 + 128 * w);
+      float4 rp[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) rp[j] = le[j];
+      ok = __all_sync(0xffffffffu, mbar_wait(s_full, (uint32_t)i & 1u));
       if (!ok) break;
       tc_fence_after();
-      const float4* le = reinterpret_cast<const float4*>(sm + L::r + s * 1024 + 256 * w);
-      uint32_t s1[32], s2[32];
-      tmem_ld32_nowait(x, s1);
-      tmem_ld32_nowait(x + 64, s2);
+      uint32_t s1[16], s2[16];
+      tmem_ld16_nowait(x, s1);
+      tmem_ld16_nowait(x + 64, s2);
       tmem_ld_wait();
-      float p1[32], p2[32];
+      // P_1 and -lam P_2, two rows at a time
+      float2 p1[8], p2[8];
 #pragma unroll
-      for (int j = 0; j < 32; j += 2) {
-        const float4 e = le[j >> 1];
-        p1[j] = ex2_approx(fmaf(__uint_as_float(s1[j]), c2, -e.x));
-        p2[j] = lam * ex2_approx(fmaf(__uint_as_float(s2[j]), c2, -e.y));
-        p1[j + 1] = ex2_approx(fmaf(__uint_as_float(s1[j + 1]), c2, -e.z));
-        p2[j + 1] = lam * ex2_approx(fmaf(__uint_as_float(s2[j + 1]), c2, -e.w));
+      for (int j = 0; j < 8; ++j) {
+        const float4 e = rp[j];
+        const float2 a = fma2(make_float2(__uint_as_float(s1[2 * j]), __uint_as_float(s1[2 * j + 1])), cc, make_float2(e.x, e.y));
+        const float2 c = fma2(make_float2(__uint_as_float(s2[2 * j]), __uint_as_float(s2[2 * j + 1])), cc, make_float2(e.z, e.w));
+        p1[j] = make_float2(ex2_approx(a.x), ex2_approx(a.y));
+        p2[j] = mul2(make_float2(ex2_approx(c.x), ex2_approx(c.y)), make_float2(nlam, nlam));
       }
       const bool masked = r0 < fr_all || r0 + 64 > len.nq;
       if (masked) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const int r = r0 + 32 * w + j;
-          if (r < fr || r >= len.nq) p1[j] = p2[j] = 0.f;
+        for (int j = 0; j < 8; ++j) {
+          const int r = r0 + 16 * w + 2 * j;
+          if (r < fr || r >= len.nq) p1[j].x = p2[j].x = 0.f;
+          if (r + 1 < fr || r + 1 >= len.nq) p1[j].y = p2[j].y = 0.f;
         }
       }
-      ok = __all_sync(0xffffffffu, mbar_wait(g_full, (uint32_t)i & 1u));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) rp[j] = le[32 + j];
+      // the next tile's row pairs, off the path from its scores to its products
+      const int sn = (i + 1) % kStages;
+      ok = __all_sync(0xffffffffu, (i + 1 == nt || mbar_wait(&f_full[sn], (uint32_t)((i + 1) / kStages) & 1u)) &&
+                                       mbar_wait(g_full, (uint32_t)i & 1u));
       if (!ok) break;
       tc_fence_after();
-      uint32_t gv[32];
-      tmem_ld32_nowait(tmem + (~i & 1) * 128 + lane_base + 32 * w, gv);
+      uint32_t gv[16];
+      tmem_ld16_nowait(tmem + (~i & 1) * 128 + lane_base + 16 * w, gv);
       tmem_ld_wait();
       tc_fence_before();
-      mbar_arrive(g_read);
+      warp_arrive(g_read);
       if (masked) {
+        // the values of rows that see nothing may be anything, and 0 times
+        // that is not 0
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const int r = r0 + 32 * w + j;
+        for (int j = 0; j < 16; ++j) {
+          const int r = r0 + 16 * w + j;
           if (r < fr || r >= len.nq) gv[j] = 0u;
         }
-        if (r0 + 64 > len.nq && t < 64 && r0 + t >= len.nq) {
-          // rows behind the length may hold anything, and 0 times it is not
-          // 0: clear them (the scores have been read) before the products
-          unsigned char* row = sm + L::f + s * L::stage + t * 128;
-          zero_row(row + (w ? 8192 : 0));
-          if (NV == 128 || !w) zero_row(row + 16384 + (w ? 8192 : 0));
-        }
+        // Q_1, Q_2 and the halves of dO: 8 KB each
+        if (r0 + 64 > len.nq && t < 64 && r0 + t >= len.nq && (NV == 128 || w < 3))
+          zero_row(sm + L::f + s * L::stage + w * 8192 + t * 128);
         fence_proxy_async();
       }
-      float v[16];
+      float v[8], v1[8], v2[8];
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        v[j] = __uint_as_float(pack2<T>(p1[2 * j] - p2[2 * j], p1[2 * j + 1] - p2[2 * j + 1]));
-      tmem_st16(x, v);
-      float v2[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        float4 d = le[32 + j];
-        const float g0 = __uint_as_float(gv[2 * j]), g1 = __uint_as_float(gv[2 * j + 1]);
-        if (masked) {   // the pairs of rows that see nothing may be unwritten
-          const int r = r0 + 32 * w + 2 * j;
-          if (r < fr || r >= len.nq) d.x = d.y = 0.f;
-          if (r + 1 < fr || r + 1 >= len.nq) d.z = d.w = 0.f;
-        }
-        v[j] = __uint_as_float(pack2<T>(p1[2 * j] * (g0 - d.x), p1[2 * j + 1] * (g1 - d.z)));
-        v2[j] = __uint_as_float(pack2<T>(p2[2 * j] * (d.y - g0), p2[2 * j + 1] * (d.w - g1)));
+      for (int j = 0; j < 8; ++j) {
+        const float4 d = rp[j];
+        const float2 gg = make_float2(__uint_as_float(gv[2 * j]), __uint_as_float(gv[2 * j + 1]));
+        const float2 both = add2(p1[j], p2[j]);
+        const float2 a = mul2(p1[j], add2(gg, make_float2(d.x, d.y))), c = mul2(p2[j], add2(gg, make_float2(d.z, d.w)));
+        v[j] = __uint_as_float(pack2<T>(both.x, both.y));
+        v1[j] = __uint_as_float(pack2<T>(a.x, a.y));
+        v2[j] = __uint_as_float(pack2<T>(c.x, c.y));
       }
-      tmem_st16(x + 16, v);
-      tmem_st16(x + 64, v2);
+      tmem_st8(x, v);
+      tmem_st8(x + 8, v1);
+      tmem_st8(x + 64, v2);
       tmem_st_wait();
-      mbar_arrive(&f_empty[s]);
       tc_fence_before();
-      mbar_arrive(p_full);
+      warp_arrive(p_full);
+      warp_arrive(&f_empty[s]);
       r0 += 64;
       if (r0 >= len.nq) {
         r0 = first;
         ++h;
-        if (i + 1 < nt) lam = wk.lam[h];
+        if (i + 1 < nt) nlam = -wk.lam[h];
       }
     }
     if (nt > 0) ok = ok && mbar_wait(acc_full, 0);
     ok = named_bar_and(1, kRowThreads, ok && !*abort_flag);
     if (ok) {
-      // warpgroup w writes dK_{w+1} and columns 64 w .. of dV
+      // warpgroups 0 and 1 write dK_1 and dK_2, 2 and 3 the halves of dV
       tc_fence_after();
       const int key = k0 + t;
-      T* dk = (T*)p.dk + b * p.dks[0] + (2 * g + w) * p.dks[1] + (int64_t)key * p.dks[2];
-      T* dv = (T*)p.dv_ + b * p.dvs[0] + g * p.dvs[1] + (int64_t)key * p.dvs[2] + 64 * w;
+      T* dst = w < 2 ? (T*)p.dk + b * p.dks[0] + (2 * g + w) * p.dks[1] + (int64_t)key * p.dks[2]
+                     : (T*)p.dv_ + b * p.dvs[0] + g * p.dvs[1] + (int64_t)key * p.dvs[2] + 64 * (w - 2);
+      const uint32_t src = (w < 2 ? t_dk + 64 * w : t_dv + 64 * (w - 2)) + lane_base;
+      const int cols = w < 2 ? p.d : p.dv - 64 * (w - 2);
+      const float f = w < 2 ? p.scale : 1.f;
+      if (NV == 128 || w < 3) {
 #pragma unroll 1
-      for (int c = 0; c < 64; c += 16) {
-        float v[16];
-        if (nt > 0) tmem_ld16(t_dk + 64 * w + lane_base + c, v);
-        else
+        for (int c = 0; c < 64; c += 16) {
+          float v[16];
+          if (nt > 0) tmem_ld16(src + c, v);
+          else
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = 0.f;
-        if (key < p.nk && c < p.d) store16<T>(dk + c, v, p.scale, p.d - c);
-        if (64 * w < NV) {
-          if (nt > 0) tmem_ld16(t_dv + 64 * w + lane_base + c, v);
-          if (key < p.nk && 64 * w + c < p.dv) store16<T>(dv + c, v, 1.f, p.dv - 64 * w - c);
+            for (int j = 0; j < 16; ++j) v[j] = 0.f;
+          if (key < p.nk && c < cols) store16<T>(dst + c, v, f, cols - c);
         }
       }
     } else if (tid == 0) {
@@ -380,11 +396,11 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
   uint64_t* f_full = q_full + 1;             // [kStages]
   uint64_t* f_empty = f_full + kStages;      // [kStages]
   uint64_t* s_full = f_empty + kStages;      // [2] S_1, S_2, G of a buffer
-  uint64_t* p_full = s_full + 2;             // [2] dS written (count 256)
+  uint64_t* p_full = s_full + 2;             // [2] dS written (16 warps)
   uint64_t* acc_full = p_full + 2;
   uint32_t* tslot = (uint32_t*)(sm + L::bar + 192);
   volatile int* abort_flag = (volatile int*)(sm + L::bar + 196);
-  float* red = (float*)(sm + L::bar + 208);  // [8]
+  float* red = (float*)(sm + L::bar + 256);  // [16]
   const int tid = threadIdx.x, warp = (int)warp_uniform(tid >> 5), lane = tid & 31;
   const int per = p.heads * p.batch, tiles = (p.nq + 127) / 128;
   const int tile = tiles - 1 - (int)(blockIdx.x / per), h = blockIdx.x % per % p.heads, b = blockIdx.x % per / p.heads;
@@ -401,7 +417,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], kRowThreads);
+      mbar_init(&p_full[i], kRowWarps);
     }
     mbar_init(acc_full, 1);
     *abort_flag = 0;
@@ -415,7 +431,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
   const uint32_t tmem = warp_uniform(*tslot);
   const uint32_t t_dq = tmem + 384;
 
-  if (warp == 8) {
+  if (warp == 16) {
     if (lane == 0 && nt > 0) {
       mbar_expect_tx(q_full, 32768 + NV / 64 * 16384);
       for (int m = 0; m < 2; ++m) tma_load_4d(sm + L::q + m * 16384, &mQ, 0, r0, 2 * h + m, b, q_full);
@@ -430,13 +446,12 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
         for (int c = 0; c < NV / 64; ++c) tma_load_4d(st + 16384 + c * 8192, &mV, 64 * c, j * 64, g, b, &f_full[s]);
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == 17) {
     if (nt > 0) {
       const uint32_t id = idesc_f16(128, 64, kBf16, false, false);
       const uint32_t id_dq = idesc_f16(128, 64, kBf16, false, true);
       const uint64_t qd = sdesc(smem_addr(sm + L::q), 16, 1024), gd = sdesc(smem_addr(sm + L::g), 16, 1024);
       const uint64_t fd = sdesc(smem_addr(sm + L::f), 16, 1024), fmn = sdesc_mn16(smem_addr(sm + L::f), 8192);
-      const int ksteps = (p.d + 15) / 16, vsteps = (p.dv + 15) / 16;
       auto issue_s = [&](int j) -> bool {
         if (!warp_wait(&f_full[j % kStages], (uint32_t)(j / kStages) & 1u)) return false;
         tc_fence_after();
@@ -446,11 +461,9 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
         for (int m = 0; m < 2; ++m)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (k < ksteps)
             mma_f16(x + m * 64, desc_add(qd, m * 16384 + k * 32), desc_add(st, m * 8192 + k * 32), id, k > 0);
 #pragma unroll
         for (int k = 0; k < NV / 16; ++k)
-          if (k < vsteps)
           mma_f16(x + 128, desc_add(gd, (k >> 2) * 16384 + (k & 3) * 32),
                   desc_add(st, 16384 + (k >> 2) * 8192 + (k & 3) * 32), id, k > 0);
         mma_commit_warp(&s_full[j & 1]);
@@ -465,7 +478,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
         const uint32_t x = tmem + (j & 1) * 192;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t a = x + (k >> 1) * 32 + (k & 1) * 8;   // warpgroup k / 2 wrote keys 16 k .. of the tile
+          const uint32_t a = x + k * 16;   // warpgroup k wrote keys 16 k .. of the tile
           mma_f16_ts(t_dq, a, desc_add(st, k * 2048), id_dq, j > 0 || k > 0);
           mma_f16_ts(t_dq + 64, a + 64, desc_add(st, 8192 + k * 2048), id_dq, j > 0 || k > 0);
         }
@@ -475,68 +488,65 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
       if (ok) mma_commit_warp(acc_full);
       else *abort_flag = 1;
     }
-  } else if (warp < 8) {
-    // one thread per row; warpgroup w takes keys 32 w .. 32 w + 31 of a tile
+  } else {
+    // one thread per row; warpgroup w takes keys 16 w .. 16 w + 15 of a tile
     const int w = warp >> 2, t = tid & 127, row = r0 + t;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const float c2 = p.scale * kLog2e, lam = wk.lam[h];
     const int lim = diff_limit(len, p.causal, row);
     const int all_see = r0 + 127 < len.nq ? diff_limit(len, p.causal, r0) : 0;
-    float2 e = make_float2(INFINITY, INFINITY), ds = make_float2(0.f, 0.f);
+    float2 e = make_float2(-INFINITY, -INFINITY), ds = make_float2(0.f, 0.f);
     if (lim > 0) {
-      const int64_t at = ((int64_t)b * p.heads + h) * wk.pitch + row;
-      e = wk.lse2[at];
-      ds = wk.dsum[at];
+      const int64_t at = ((int64_t)b * p.heads + h) * wk.pitch;
+      e = make_float2(diff_row(wk.nlse, at, row, 0), diff_row(wk.nlse, at, row, 1));
+      ds = make_float2(diff_row(wk.nsum, at, row, 0), diff_row(wk.nsum, at, row, 1));
     }
+    const float2 cc = make_float2(c2, c2), e1 = make_float2(e.x, e.x), e2 = make_float2(e.y, e.y);
+    const float2 d1 = make_float2(ds.x, ds.x), d2 = make_float2(ds.y, ds.y), nl = make_float2(-lam, -lam);
     float pg = 0.f;
     bool ok = true;
     for (int j = 0; j < nt; ++j) {
-      const uint32_t x = tmem + (j & 1) * 192 + lane_base + 32 * w;
-      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[j & 1], (uint32_t)(j >> 1) & 1u) && !*abort_flag);
+      const uint32_t x = tmem + (j & 1) * 192 + lane_base + 16 * w;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[j & 1], (uint32_t)(j >> 1) & 1u));
       if (!ok) break;
       tc_fence_after();
-      uint32_t s1[32], s2[32], gv[32];
-      tmem_ld32_nowait(x, s1);
-      tmem_ld32_nowait(x + 64, s2);
-      tmem_ld32_nowait(x + 128, gv);
+      uint32_t s1[16], s2[16], gv[16];
+      tmem_ld16_nowait(x, s1);
+      tmem_ld16_nowait(x + 64, s2);
+      tmem_ld16_nowait(x + 128, gv);
       tmem_ld_wait();
       if (j * 64 + 64 > all_see) {
-        const int n = lim - j * 64 - 32 * w;
+        const int n = lim - j * 64 - 16 * w;
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
+        for (int i = 0; i < 16; ++i)
           if (i >= n) {
             s1[i] = s2[i] = 0xff800000u;
             gv[i] = 0u;
           }
-        if (j * 64 + 64 > len.nk && len.nk < p.nk && t < 64 && j * 64 + t >= len.nk) {
-          // K behind the length may hold anything, and 0 times it is not 0
+        // K behind the length may hold anything, and 0 times it is not 0
+        if (j * 64 + 64 > len.nk && len.nk < p.nk && w < 2 && t < 64 && j * 64 + t >= len.nk)
           zero_row(sm + L::f + (j % kStages) * L::stage + w * 8192 + t * 128);
-        }
         fence_proxy_async();
       }
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
-      float v1[16], v2[16];
+      float2 part[2] = {};
+      float v1[8], v2[8];
 #pragma unroll
-      for (int i = 0; i < 32; i += 2) {
-        float a[2], c[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float gk = __uint_as_float(gv[i + k]);
-          const float p1 = ex2_approx(fmaf(__uint_as_float(s1[i + k]), c2, -e.x));
-          const float p2 = ex2_approx(fmaf(__uint_as_float(s2[i + k]), c2, -e.y));
-          part[(i + k) & 3] = fmaf(p2, gk, part[(i + k) & 3]);
-          a[k] = p1 * (gk - ds.x);
-          c[k] = (lam * p2) * (ds.y - gk);
-        }
-        v1[i >> 1] = __uint_as_float(pack2<T>(a[0], a[1]));
-        v2[i >> 1] = __uint_as_float(pack2<T>(c[0], c[1]));
+      for (int i = 0; i < 8; ++i) {
+        const float2 gg = make_float2(__uint_as_float(gv[2 * i]), __uint_as_float(gv[2 * i + 1]));
+        const float2 a = fma2(make_float2(__uint_as_float(s1[2 * i]), __uint_as_float(s1[2 * i + 1])), cc, e1);
+        const float2 c = fma2(make_float2(__uint_as_float(s2[2 * i]), __uint_as_float(s2[2 * i + 1])), cc, e2);
+        const float2 p1 = make_float2(ex2_approx(a.x), ex2_approx(a.y)), p2 = make_float2(ex2_approx(c.x), ex2_approx(c.y));
+        part[i & 1] = fma2(p2, gg, part[i & 1]);
+        const float2 q1 = mul2(p1, add2(gg, d1)), q2 = mul2(mul2(p2, nl), add2(gg, d2));
+        v1[i] = __uint_as_float(pack2<T>(q1.x, q1.y));
+        v2[i] = __uint_as_float(pack2<T>(q2.x, q2.y));
       }
-      tmem_st16(x, v1);
-      tmem_st16(x + 64, v2);
+      tmem_st8(x, v1);
+      tmem_st8(x + 64, v2);
       tmem_st_wait();
-      pg += (part[0] + part[1]) + (part[2] + part[3]);
+      pg += (part[0].x + part[0].y) + (part[1].x + part[1].y);
       tc_fence_before();
-      mbar_arrive(&p_full[j & 1]);
+      warp_arrive(&p_full[j & 1]);
     }
     if (nt > 0) ok = ok && mbar_wait(acc_full, 0);
     for (int o = 16; o > 0; o >>= 1) pg += __shfl_xor_sync(0xffffffffu, pg, o);
@@ -544,20 +554,23 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
     ok = named_bar_and(1, kRowThreads, ok && !*abort_flag);
     if (ok) {
       tc_fence_after();
-      // warpgroup w writes dQ_{w+1}
-      T* dq = (T*)p.dq + b * p.dqs[0] + (2 * h + w) * p.dqs[1] + (int64_t)row * p.dqs[2];
+      // warpgroup w writes 32 columns of dQ_1 (w = 0, 1) or dQ_2
+      const int m = w >> 1, c0 = 32 * (w & 1);
+      T* dq = (T*)p.dq + b * p.dqs[0] + (2 * h + m) * p.dqs[1] + (int64_t)row * p.dqs[2];
 #pragma unroll 1
-      for (int c = 0; c < 64; c += 16) {
+      for (int c = c0; c < c0 + 32; c += 16) {
         float v[16];
-        if (nt > 0) tmem_ld16(t_dq + 64 * w + lane_base + c, v);
+        if (nt > 0) tmem_ld16(t_dq + 64 * m + lane_base + c, v);
         else
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[i] = 0.f;
         if (row < p.nq && c < p.d) store16<T>(dq + c, v, p.scale, p.d - c);
       }
-      if (tid == 0)
-        wk.partials[((int64_t)h * p.batch + b) * tiles + tile] =
-            ((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7]));
+      if (tid == 0) {
+        float sum = 0.f;
+        for (int i = 0; i < kRowWarps; ++i) sum += red[i];
+        wk.partials[((int64_t)h * p.batch + b) * tiles + tile] = sum;
+      }
     } else if (tid == 0) {
       *abort_flag = 1;
     }

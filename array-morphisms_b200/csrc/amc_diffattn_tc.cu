@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kThreadsF, 1) k_diff_fwd_tc(const __grid_const
   uint64_t* v_full = k_empty + kKStages;          // [kVStages]
   uint64_t* v_empty = v_full + kVStages;
   uint64_t* s_full = v_empty + kVStages;          // [map][buffer] S(j) complete
-  uint64_t* p_full = s_full + 4;                  // [map][buffer] P(j) written (count 128)
+  uint64_t* p_full = s_full + 4;                  // [map][buffer] P(j) written (4 warps)
   uint64_t* o_done = p_full + 4;                  // [map] P V of a step complete
   uint64_t* all_done = o_done + 2;
   uint32_t* tslot = (uint32_t*)(sm + L::bar + 192);
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kThreadsF, 1) k_diff_fwd_tc(const __grid_const
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[i], 4);
     }
     mbar_init(&o_done[0], 1);
     mbar_init(&o_done[1], 1);
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(kThreadsF, 1) k_diff_fwd_tc(const __grid_const
       tmem_st_wait();
       l2 = add2(l2, add2(add2(s4[0], s4[1]), add2(s4[2], s4[3])));
       tc_fence_before();
-      mbar_arrive(&p_full[2 * m + (j & 1)]);
+      warp_arrive(&p_full[2 * m + (j & 1)]);
     }
     const float l = l2.x + l2.y;
     if (ns > 0) ok = ok && mbar_wait(all_done, 0);
