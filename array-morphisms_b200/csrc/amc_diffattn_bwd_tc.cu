@@ -8,7 +8,10 @@
 // against 20 d were dQ added up across CTAs; without atomics the results are
 // the same at every call.
 //   k_diff_dkv_tc  one CTA per 128 keys of a key head; streams 64-row tiles of
-//                  every query head that shares it;
+//                  every query head that shares it, or, where such CTAs would
+//                  not fill the GPU, one cluster of CTAs that take a share of
+//                  those heads each and add up through distributed shared
+//                  memory, in order of rank;
 //   k_diff_dq_tc   one CTA per 128 rows of a query head; streams 64-key tiles,
 //                  and sums P_2 G (dlam) in f32 on the way.
 // The operands that the threads make (the difference of the maps, dS_1, dS_2)
@@ -60,6 +63,8 @@ struct QSmem {
   static constexpr int bar = f + kStages * stage;
   static constexpr int bytes = bar + 320 + 1024;
 };
+constexpr int kPartPitch = 260;      // floats: dK_1, dK_2, dV, and a shift of banks from row to row
+static_assert(128 * kPartPitch * 4 <= KvSmem<64>::r, "a cluster's parts fit the tiles' memory");
 static_assert(KvSmem<128>::bytes <= 232448 && QSmem<128>::bytes <= 232448, "shared memory");
 
 __device__ int g_diff_bwd_error;
@@ -97,7 +102,7 @@ template <typename T, int NV>
 __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
     const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mK,
     const __grid_constant__ CUtensorMap mV, const __grid_constant__ CUtensorMap mG,
-    const __grid_constant__ amc_diff_attention p, const __grid_constant__ DiffBwdWork wk) {
+    const __grid_constant__ amc_diff_attention p, const __grid_constant__ DiffBwdWork wk, int share) {
   using L = KvSmem<NV>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ unsigned char diff_sm_raw[];
@@ -116,11 +121,13 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
   // key tiles of one head are launched first tile first: with a causal mask
   // those have the most rows
   const int per = p.kv_heads * p.batch, group = p.heads / p.kv_heads;
-  const int k0 = (int)(blockIdx.x / per) * 128, g = blockIdx.x % per % p.kv_heads, b = blockIdx.x % per / p.kv_heads;
+  const int unit = blockIdx.x / share, rank = blockIdx.x % share;   // share: CTAs of a cluster
+  const int k0 = unit / per * 128, g = unit % per % p.kv_heads, b = unit % per / p.kv_heads;
+  const int head0 = g * group + rank * (group / share);
   const DiffLens len = diff_lens(p, b);
   const int first = diff_first_row(len, p.causal, k0) / 64 * 64;
   const int nth = first < len.nq ? (len.nq - first + 63) / 64 : 0;   // tiles a head
-  const int nt = (int)warp_uniform(nth * group);
+  const int nt = (int)warp_uniform(nth * (group / share));
   // pairs behind the tensor's rows are never loaded: they count as zeros
   for (int i = tid; i < kStages * 64; i += kThreadsB)
     reinterpret_cast<float4*>(sm + L::r)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -146,13 +153,14 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
   tc_fence_after();
   const uint32_t tmem = warp_uniform(*tslot);
   const uint32_t t_dv = tmem + 256, t_dk = tmem + 384;
+  float* part = (float*)sm;   // [128 keys][kPartPitch] once all products are done
 
   if (warp == 16) {
     if (lane == 0 && nt > 0) {
       mbar_expect_tx(kv_full, 32768 + NV / 64 * 16384);
       for (int m = 0; m < 2; ++m) tma_load_4d(sm + L::k + m * 16384, &mK, 0, k0, 2 * g + m, b, kv_full);
       for (int c = 0; c < NV / 64; ++c) tma_load_4d(sm + L::v + c * 16384, &mV, 64 * c, k0, g, b, kv_full);
-      int h = g * group, r0 = first;
+      int h = head0, r0 = first;
       for (int i = 0; i < nt; ++i) {
         const int s = i % kStages;
         if (i >= kStages && !mbar_wait(&f_empty[s], (uint32_t)(i / kStages - 1) & 1u)) { *abort_flag = 1; break; }
@@ -249,7 +257,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
     const int fr_all = diff_first_row(len, p.causal, k0 + 127);   // from here on every key of the tile is seen
     const float2 cc = make_float2(c2, c2);
     bool ok = true;
-    int h = g * group, r0 = first;
+    int h = head0, r0 = first;
     float nlam = nt > 0 ? -wk.lam[h] : 0.f;
     if (nt > 0) ok = __all_sync(0xffffffffu, mbar_wait(&f_full[0], 0));
     for (int i = 0; i < nt && ok; ++i) {
@@ -357,7 +365,13 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
           else
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] = 0.f;
-          if (key < p.nk && c < cols) store16<T>(dst + c, v, f, cols - c);
+          if (share > 1) {   // all products are done: the tiles' memory is free
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<float4*>(part + t * kPartPitch + 64 * w + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          } else if (key < p.nk && c < cols) {
+            store16<T>(dst + c, v, f, cols - c);
+          }
         }
       }
     } else if (tid == 0) {
@@ -374,8 +388,31 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
     mbar_wait(s_full, 0, 1 << 14);
     mbar_wait(g_full, 0, 1 << 14);
     mbar_wait(acc_full, 0, 1 << 14);
+    __syncthreads();
   }
   if (warp == 0) tmem_dealloc(tmem, 512);
+  if (share > 1) {
+    // every CTA of the cluster adds up its part of the 128 keys: 4 columns of
+    // dK_1, dK_2 and dV a thread, ranks in order
+    cluster_sync();
+    const int keys = (128 + share - 1) / share;
+    for (int i = tid; i < keys * 64; i += kThreadsB) {
+      const int row = rank * keys + i / 64, c = i % 64 * 4, key = k0 + row;
+      if (row >= 128 || key >= p.nk || (NV == 64 && c >= 192)) continue;
+      float4 sum = ld_cluster(part + row * kPartPitch + c, 0);
+      for (int r = 1; r < share; ++r) {
+        const float4 v = ld_cluster(part + row * kPartPitch + c, r);
+        sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+      }
+      const int m = c / 64, cc = m < 2 ? c % 64 : c - 128;
+      if (cc >= (m < 2 ? p.d : p.dv)) continue;
+      const float f = m < 2 ? p.scale : 1.f;
+      T* dst = m < 2 ? (T*)p.dk + b * p.dks[0] + (2 * g + m) * p.dks[1] + (int64_t)key * p.dks[2]
+                     : (T*)p.dv_ + b * p.dvs[0] + g * p.dvs[1] + (int64_t)key * p.dvs[2];
+      *reinterpret_cast<uint2*>(dst + cc) = make_uint2(pack2<T>(sum.x * f, sum.y * f), pack2<T>(sum.z * f, sum.w * f));
+    }
+    cluster_sync();   // the others have read this CTA's part
+  }
 }
 
 // ------------------------------------------------------------------ dQ, dlam
@@ -602,8 +639,23 @@ int bwd_tc(const amc_diff_attention& p, const DiffBwdWork& w, const CUtensorMap 
   if (int rc = smem_attr_once(k_diff_dq_tc<T, NV>, QSmem<NV>::bytes, attr_q)) return rc;
   const unsigned gk = (unsigned)((int64_t)((p.nk + 127) / 128) * p.kv_heads * p.batch);
   const int tiles = (p.nq + 127) / 128;
-  k_diff_dkv_tc<T, NV><<<gk, kThreadsB, KvSmem<NV>::bytes, s>>>(kv[0], kv[1], kv[2], kv[3], p, w);
-  AMC_CUDA(cudaGetLastError());
+  // Heads that share a key head go to a cluster of CTAs while one CTA for all
+  // of them leaves SMs idle: 6 heads over 2 at 5 x 1000 rows take 80 CTAs.
+  const int group = p.heads / p.kv_heads;
+  int share = 1;
+  for (int c = 2; c <= 8 && c <= group && (int64_t)gk * share < num_sms(); ++c)
+    if (group % c == 0) share = c;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(gk * share);
+  cfg.blockDim = dim3(kThreadsB);
+  cfg.dynamicSmemBytes = KvSmem<NV>::bytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)share, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = share > 1 ? 1 : 0;
+  AMC_CUDA(cudaLaunchKernelEx(&cfg, k_diff_dkv_tc<T, NV>, kv[0], kv[1], kv[2], kv[3], p, w, share));
   const unsigned gq = (unsigned)((int64_t)tiles * p.heads * p.batch);
   k_diff_dq_tc<T, NV><<<gq, kThreadsB, QSmem<NV>::bytes, s>>>(q[0], q[1], q[2], q[3], p, w);
   AMC_CUDA(cudaGetLastError());

@@ -338,6 +338,14 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Four floats at `p` (this CTA's address) in the CTA of rank `rank`.
+__device__ __forceinline__ float4 ld_cluster(const float* p, uint32_t rank) {
+  float4 v;
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem_addr(p)), "r"(rank) : "memory");
+  return v;
+}
 // Arrive at `bar` (this CTA's address) in the CTA of rank `rank`.  Without a
 // cluster-wide release: what such an arrival announces is in tensor memory or
 // shared memory read by the products (tcgen05 and proxy fences order those),
