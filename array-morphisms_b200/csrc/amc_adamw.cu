@@ -4,35 +4,46 @@
 // The bound is HBM: 28 bytes an element for f32 parameters and states, 16 and
 // a bit with 8-bit states.  One launch covers up to 256 tensors, whose
 // descriptors travel as kernel parameters (no copy to the device, nothing to
-// keep between calls); a CTA owns 4096 elements of one tensor and finds it by
-// bisection.  A warp owns blocks of 256 elements, 8 a lane in two groups of 4
+// keep between calls).  CTAs are persistent: the step's scalars (two powers in
+// double) are formed once, and each CTA goes over chunks of 2048 elements of
+// one tensor.  A warp owns blocks of 256 elements, 8 a lane in two groups of 4
 // neighbours, so f32 data moves in coalesced 16-byte accesses and an 8-bit
 // state's scale is one warp reduction.
 //
-// The sums are made in the order written above with every operation rounded
-// (the file is compiled without multiply-add contraction), so the step is the
-// same as the elementary f32 operations one after the other.  8-bit states
+// The states' sums are made in the order written above with every operation
+// rounded (the file is compiled without multiply-add contraction), so they are
+// the same as the elementary f32 operations one after the other; p's quotient
+// is a product with an approximate reciprocal, 2^-22 of the step.  8-bit states
 // hold m and sqrt(v) as e4m3 (4 significant bits, 2^-9 .. 448) of the value
 // over its block's largest.  Their rounding is random, up with the
 // probability of the remainder: with b2 = 0.999 a step changes v by about
 // 0.1 %, nearest rounding to a code 6 % away would never move it.  The bits
 // come from the lowbias32 mixer (C. Wellons, "Prospecting for Hash
 // Functions") of element, tensor and step.
+#include <cuda_fp8.h>
+
 #include "amc_half.cuh"
 #include "amc_internal.h"
+#include "amc_tc.cuh"
 
 namespace amc {
+
+using tc::add2;
+using tc::max3;
+using tc::min3;
+using tc::mul2;
 
 namespace {
 
 constexpr int kAdamTensors = 256;    // descriptors per launch
-constexpr int kAdamChunk = 4096;     // elements per CTA
+constexpr int kAdamChunk = 2048;     // elements of a CTA's pass: a block a warp
+constexpr int kAdamCtas = 4;         // a SM, at 64 registers a thread
 constexpr int kAdamBlock = 256;      // elements per scale
 constexpr float kE4m3Max = 448.f;
 
 struct AdamTensor {
   amc_adamw_tensor t;
-  int64_t chunk0;     // first CTA of this tensor
+  int64_t chunk0;     // its first chunk
 };
 
 struct AdamArgs {
@@ -41,6 +52,7 @@ struct AdamArgs {
   double lr, b1, b2;
   float eps;
   double wd;
+  int64_t chunks;
   int count, base, last;   // tensors here, index of the first, whether this launch ends the step
   AdamTensor t[kAdamTensors];
 };
@@ -63,17 +75,34 @@ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
   return x ^ (x >> 16);
 }
 
-// a in [0, 448] (a hair above from rounding): to e4m3 with 20 random bits.
-// Returns the 7-bit code.
-__device__ __forceinline__ uint32_t e4m3_random(float a, uint32_t rnd) {
-  if (a < 0.015625f) return (uint32_t)floorf(a * 512.f + (float)rnd * 9.5367431640625e-07f);   // steps of 2^-9
-  const uint32_t c = ((__float_as_uint(a) + rnd) >> 20) - (120u << 3);
-  return c > 126u ? 126u : c;
+// A value in [0, 448] (a hair above from rounding) to its 7-bit e4m3 code with
+// 20 random bits.  From 2^-6 up the bits are added below the third bit of the
+// mantissa and cut off; below, the codes are steps of 2^-9, and
+// floor(512 a + bits 2^-20) comes out of the low bits of a sum with 2^23 that
+// is rounded down.  No conversion instruction (16 a clock) is needed.
+constexpr float kE4m3Fine = 0.015625f;
+__device__ __forceinline__ uint32_t e4m3_coarse(uint32_t bits, uint32_t rnd) {
+  return min(((bits + rnd) >> 20) - (120u << 3), 126u);
 }
-__device__ __forceinline__ float e4m3_value(uint32_t c) {
-  const uint32_t m = c & 127u;
-  const float v = m < 8u ? (float)m * 0.001953125f : __uint_as_float((m + (120u << 3)) << 20);
-  return c & 128u ? -v : v;
+__device__ __forceinline__ uint32_t e4m3_fine(float a, uint32_t rnd) {
+  const float part = __uint_as_float(0x3F800000u | rnd << 3) - 1.f;   // rnd 2^-20
+  return __float_as_uint(__fadd_rd(a * 512.f + part, 8388608.f)) & 15u;
+}
+__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 get2(const float (&v)[4], int k) { return make_float2(v[k], v[k + 1]); }
+__device__ __forceinline__ void put2(float (&v)[4], int k, float2 x) {
+  v[k] = x.x;
+  v[k + 1] = x.y;
+}
+// Four codes to their values (the 8-bit pairs convert through fp16, which holds them exactly).
+__device__ __forceinline__ void e4m3_values(float (&v)[4], uint32_t w) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * k) & 0xFFFFu), __NV_E4M3);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    v[2 * k] = f.x;
+    v[2 * k + 1] = f.y;
+  }
 }
 
 // 4 neighbours, as one access where the block is whole and aligned.
@@ -121,6 +150,28 @@ __device__ __forceinline__ void store_codes(uint8_t* p, uint32_t w, int64_t e, i
       if (e + k < n) p[e + k] = (uint8_t)(w >> (8 * k));
   }
 }
+// A sum of two products, each rounded: written as a packed sum, the assembler
+// contracts it with one of them.
+__device__ __forceinline__ float2 sum2(float2 a, float2 b) {
+  return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y));
+}
+// The square root of x >= 0, rounded to nearest: one Newton step (Heron's
+// method) from the approximate reciprocal root, with the residual x - s^2
+// formed exactly by one fused operation; the library's root where that
+// residual could underflow, and for infinities and NaN.
+__device__ __forceinline__ float root_nearest(float x) {
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  const float s = x * y;
+  float r = __fmaf_rn(__fmaf_rn(-s, s, x), 0.5f * y, s);
+  if (!(x >= 7.888609052210118e-31f && x <= 3e38f)) r = sqrtf(x);   // 2^-100
+  return r;
+}
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float warp_max(float x) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
@@ -130,39 +181,39 @@ __device__ __forceinline__ float warp_max(float x) {
 }  // namespace
 
 template <typename P, typename G, bool MASTER, bool BITS8>
-__global__ void __launch_bounds__(256) k_adamw(const __grid_constant__ AdamArgs a) {
+__global__ void __launch_bounds__(256, kAdamCtas) k_adamw(const __grid_constant__ AdamArgs a) {
   __shared__ float sh[3];
   __shared__ uint32_t sh_t;
-  int lo = 0, hi = a.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.t[mid].chunk0 <= (int64_t)blockIdx.x) lo = mid;
-    else hi = mid - 1;
-  }
-  const amc_adamw_tensor& t = a.t[lo].t;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t n = t.n, c0 = ((int64_t)blockIdx.x - a.t[lo].chunk0) * kAdamChunk;
   if (threadIdx.x == 0) {
     const int64_t step = a.state[0] + 1;
     const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
     sh[0] = (float)(lr / (1.0 - int_pow(a.b1, step)));
-    sh[1] = (float)sqrt(1.0 - int_pow(a.b2, step));
+    sh[1] = (float)(1.0 / sqrt(1.0 - int_pow(a.b2, step)));
     sh[2] = (float)(1.0 - lr * a.wd);
     sh_t = (uint32_t)step;
   }
-  // aligned for 4-element accesses of every array (chunks start on multiples of 4096)
-  const uintptr_t al = (uintptr_t)t.m | (uintptr_t)t.v;
-  bool aligned = !(al & (BITS8 ? 3 : 15)) && !((uintptr_t)t.p & (4 * sizeof(P) - 1)) && !((uintptr_t)t.g & (4 * sizeof(G) - 1));
-  if (MASTER) aligned = aligned && !((uintptr_t)t.master & 15);
   const float b1 = (float)a.b1, b2 = (float)a.b2, r1 = (float)(1.0 - a.b1), r2 = (float)(1.0 - a.b2);
   __syncthreads();
   const float rate = sh[0], root = sh[1], keep = sh[2];
-  const uint32_t seed = sh_t * 0x85EBCA77u + (uint32_t)(a.base + lo) * 0xC2B2AE3Du;
-#pragma unroll
-  for (int r = 0; r < kAdamChunk / (8 * kAdamBlock); ++r) {
-    const int64_t e0 = c0 + (r * 8 + warp) * kAdamBlock;
+  int lo = 0;
+  for (int64_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
+    // the last tensor that starts at or before this chunk, by bisection of those still ahead
+    int hi = a.count - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (a.t[mid].chunk0 <= chunk) lo = mid;
+      else hi = mid - 1;
+    }
+    const amc_adamw_tensor& t = a.t[lo].t;
+    const int64_t n = t.n, e0 = (chunk - a.t[lo].chunk0) * kAdamChunk + warp * kAdamBlock;
     if (e0 >= n) continue;
-    const bool vec = aligned && e0 + kAdamBlock <= n;
+    // aligned for 4-element accesses of every array (blocks start on multiples of 256)
+    const uintptr_t al = (uintptr_t)t.m | (uintptr_t)t.v;
+    bool vec = e0 + kAdamBlock <= n && !(al & (BITS8 ? 3 : 15)) && !((uintptr_t)t.p & (4 * sizeof(P) - 1)) &&
+               !((uintptr_t)t.g & (4 * sizeof(G) - 1));
+    if (MASTER) vec = vec && !((uintptr_t)t.master & 15);
+    const uint32_t seed = sh_t * 0x85EBCA77u + (uint32_t)(a.base + lo) * 0xC2B2AE3Du;
     float p[2][4], g[2][4], m[2][4], v[2][4];
     uint32_t cm[2], cv[2];
 #pragma unroll
@@ -182,27 +233,34 @@ __global__ void __launch_bounds__(256) k_adamw(const __grid_constant__ AdamArgs 
     if (BITS8) {
       const float sm = t.m_scale[e0 / kAdamBlock], sv = t.v_scale[e0 / kAdamBlock];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j) {
+        e4m3_values(m[j], cm[j]);
+        e4m3_values(v[j], cv[j]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          m[j][k] = e4m3_value(cm[j] >> (8 * k) & 255u) * sm;
-          const float u = e4m3_value(cv[j] >> (8 * k) & 255u) * sv;
-          v[j][k] = u * u;
+        for (int k = 0; k < 4; k += 2) {
+          put2(m[j], k, mul2(get2(m[j], k), twice(sm)));
+          const float2 u = mul2(get2(v[j], k), twice(sv));
+          put2(v[j], k, mul2(u, u));
         }
+      }
     }
     float top_m = 0.f, top_u = 0.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        m[j][k] = m[j][k] * b1 + g[j][k] * r1;
-        v[j][k] = v[j][k] * b2 + (g[j][k] * g[j][k]) * r2;
-        const float u = sqrtf(v[j][k]);
-        p[j][k] = p[j][k] * keep - rate * (m[j][k] / (u / root + a.eps));
+      for (int k = 0; k < 4; k += 2) {
+        const float2 gg = get2(g[j], k);
+        const float2 mm = sum2(mul2(get2(m[j], k), twice(b1)), mul2(gg, twice(r1)));
+        const float2 vv = sum2(mul2(get2(v[j], k), twice(b2)), mul2(mul2(gg, gg), twice(r2)));
+        const float2 u = make_float2(root_nearest(vv.x), root_nearest(vv.y));
+        const float2 den = add2(mul2(u, twice(root)), twice(a.eps));
+        const float2 step = mul2(mm, make_float2(reciprocal(den.x), reciprocal(den.y)));
+        put2(p[j], k, add2(mul2(get2(p[j], k), twice(keep)), mul2(twice(-rate), step)));
+        put2(m[j], k, mm);
+        put2(v[j], k, BITS8 ? u : vv);
         if (BITS8) {
-          v[j][k] = u;
-          top_m = fmaxf(top_m, fabsf(m[j][k]));
-          top_u = fmaxf(top_u, u);
+          top_m = max3(top_m, fabsf(mm.x), fabsf(mm.y));
+          top_u = max3(top_u, u.x, u.y);
         }
       }
     if (BITS8) {
@@ -214,18 +272,35 @@ __global__ void __launch_bounds__(256) k_adamw(const __grid_constant__ AdamArgs 
         t.m_scale[e0 / kAdamBlock] = some_m ? top_m * (1.f / kE4m3Max) : 0.f;
         t.v_scale[e0 / kAdamBlock] = some_u ? top_u * (1.f / kE4m3Max) : 0.f;
       }
+      // values over their scale; m keeps its sign
+      float least = 448.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+          const float2 x = mul2(get2(m[j], k), twice(im)), u = mul2(get2(v[j], k), twice(iu));
+          put2(m[j], k, x);
+          put2(v[j], k, u);
+          least = min3(least, fabsf(x.x), fabsf(x.y));
+          least = min3(least, u.x, u.y);
+        }
+      // below 2^-6 of 448 the codes are even steps: about one block in forty
+      // of normally distributed values has any, and takes the longer way
+      const bool fine = __any_sync(0xffffffffu, !(least >= kE4m3Fine));
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
+        uint32_t x = (uint32_t)(e0 + 128 * j + 4 * lane) * 0x9E3779B1u + seed;
         cm[j] = cv[j] = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t rnd = mix32((uint32_t)(e0 + 128 * j + 4 * lane + k) * 0x9E3779B1u + seed);
-          const uint32_t neg = __float_as_uint(m[j][k]) >> 31 << 7;
-          cm[j] |= (e4m3_random(fabsf(m[j][k]) * im, rnd & 0xFFFFFu) | neg) << (8 * k);
-          const float u = v[j][k] * iu;
-          uint32_t c = e4m3_random(u, rnd >> 12);
-          if (c == 0 && u > 0.f) c = 1;
-          cv[j] |= c << (8 * k);
+        for (int k = 0; k < 4; ++k, x += 0x9E3779B1u) {
+          const uint32_t rnd = mix32(x), bits = __float_as_uint(m[j][k]);
+          uint32_t c = e4m3_coarse(bits & 0x7FFFFFFFu, rnd & 0xFFFFFu), d = e4m3_coarse(__float_as_uint(v[j][k]), rnd >> 12);
+          if (fine) {
+            if (fabsf(m[j][k]) < kE4m3Fine) c = e4m3_fine(fabsf(m[j][k]), rnd & 0xFFFFFu);
+            if (v[j][k] < kE4m3Fine) d = max(e4m3_fine(v[j][k], rnd >> 12), v[j][k] > 0.f ? 1u : 0u);
+          }
+          cm[j] |= (c | bits >> 31 << 7) << (8 * k);
+          cv[j] |= d << (8 * k);
         }
       }
     }
@@ -327,7 +402,9 @@ int amc_adamw(const amc_adamw_tensor* t, int32_t count, int32_t p_dtype, int32_t
     }
     if (chunks > 0x7fffffff) return fail(AMC_ERR_INVALID, "amc_adamw: too many elements");
     if (!chunks && !a.last) continue;
-    const unsigned grid = chunks ? (unsigned)chunks : 1u;
+    a.chunks = chunks;
+    const int64_t most = (int64_t)num_sms() * kAdamCtas;
+    const unsigned grid = (unsigned)(chunks < 1 ? 1 : chunks < most ? chunks : most);
     int rc = p_dtype == AMC_F32    ? adamw_grad<float>(a, g_dtype, grid, master, bits8, s)
              : p_dtype == AMC_BF16 ? adamw_grad<__nv_bfloat16>(a, g_dtype, grid, master, bits8, s)
                                    : adamw_grad<__half>(a, g_dtype, grid, master, bits8, s);

@@ -260,6 +260,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // 2^x on the FMA pipe for finite x in [-126, 127], to relieve the
 // special-function unit (16 a clock and SM): x = n + f with n the nearest
 // integer (added 1.5 * 2^23 leaves it in the low bits), the minimax polynomial
