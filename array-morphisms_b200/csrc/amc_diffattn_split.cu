@@ -3,17 +3,19 @@
 //
 // The bound is HBM: every key and value is read once, for all rows (query
 // heads that share the key head, times their rows) of a 16-row block.  The
-// keys of one sequence and key head are cut into chunks, one CTA each, and
-// within a chunk its four warps take every fourth block of 16 keys.  Warps do
+// keys of all sequences and key heads, in blocks of 64, are one line of work
+// that the CTAs, two a SM, share evenly, so sequences of different lengths
+// leave none idle; a CTA's share may end one sequence and begin another.
+// Within a CTA the four warps take a block's four boxes of 16 keys.  Warps do
 // not wait for each other: each has its own ring of TMA boxes (K_1, K_2 and V
 // rows of 16 keys, 8 KB), its own running maximum, sum and output, and they
-// meet at the end of the chunk in shared memory.  The products are
+// meet at the end of a sequence's part in shared memory.  The products are
 // mma.sync m16n8k16: 16 rows fill a legacy tile, where a tcgen05 tile of 128
 // would be an eighth full, and at 16 rows they take less than half the time
 // of the loads.  P is taken into P V as the sum of two 16-bit values (the
 // rounded one and the rounding's remainder), which the loads hide: the result
-// carries no rounding of P.  A second kernel joins the chunks' outputs by
-// their maxima and sums; with one chunk the first kernel writes the result.
+// carries no rounding of P.  A second kernel joins the parts of the sequences
+// that several CTAs worked on by their maxima and sums.
 #include <cmath>
 #include <type_traits>
 
@@ -33,18 +35,67 @@ constexpr int kStages = 3;           // boxes in flight per warp
 constexpr int kBox = 8192;           // 16 keys: K_1 2 KB, K_2 2 KB, V 4 KB
 constexpr int kStageBytes = kWarps * kStages * kBox;
 constexpr int kSplitSmem = kStageBytes + 512 + 1024;
-constexpr int kMinChunk = 256;       // keys: 4 boxes a warp
-constexpr int kTargetCtas = 148 * 8; // chunks at full lengths: enough that sequences of different lengths even out
+constexpr int kShareCtas = 148 * 2;  // CTAs that share the keys
+constexpr int kMinShare = 4;         // blocks of 64 keys: 4 boxes a warp
+constexpr int kMaxBatch = 1024;      // sequences whose lengths a CTA sums up
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
 __device__ int g_diff_split_error;
 
 struct SplitArgs {
-  int group, row_blocks, splits, chunk;
-  float* part;       // [unit][split][row][map][dv] unscaled outputs
-  float2* part_ml;   // [unit][split][row][map] maximum (log2 units) and sum
+  int group, row_blocks, shared;   // shared: the keys are shared out (else a unit a CTA)
+  float* part;       // [CTA][first or last unit][row][map][dv] unscaled outputs
+  float2* part_ml;   // [CTA][first or last unit][row][map] maximum (log2 units) and sum
 };
+
+// A unit is one sequence, key head and block of 16 rows.  Its blocks of 64
+// keys stand on one line after those of the units before it.
+struct Unit {
+  int b, u, blocks;      // u: key head and row block
+  int64_t first;         // its first block on the line
+};
+__device__ __forceinline__ int seq_blocks(const amc_diff_attention& p, int b) {
+  const DiffLens len = diff_lens(p, b);
+  return len.nq > 0 ? (len.nk + 63) / 64 : 0;
+}
+// All blocks of the line, by one warp.
+__device__ __forceinline__ int64_t line_blocks(const amc_diff_attention& p, int per_seq) {
+  int64_t n = 0;
+  for (int b = threadIdx.x & 31; b < p.batch; b += 32) n += seq_blocks(p, b);
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  return n * per_seq;
+}
+// The unit of block x, by one warp.
+__device__ __forceinline__ Unit find_unit(const amc_diff_attention& p, int per_seq, int64_t x) {
+  int64_t before = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    const int b = b0 + (threadIdx.x & 31);
+    const int64_t mine = b < p.batch ? (int64_t)seq_blocks(p, b) * per_seq : 0;
+    int64_t upto = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if ((threadIdx.x & 31) >= o) upto += v;
+    }
+    const unsigned here = __ballot_sync(0xffffffffu, before + upto > x);
+    if (here) {
+      const int l = __ffs(here) - 1;
+      Unit r;
+      r.b = b0 + l;
+      r.blocks = (int)(__shfl_sync(0xffffffffu, mine, l) / per_seq);
+      const int64_t start = before + __shfl_sync(0xffffffffu, upto, l) - (int64_t)r.blocks * per_seq;
+      r.u = (int)((x - start) / r.blocks);
+      r.first = start + (int64_t)r.u * r.blocks;
+      return r;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return Unit{0, 0, 0, x};
+}
+__device__ __forceinline__ int64_t share_of(int64_t total) {
+  const int64_t n = (total + kShareCtas - 1) / kShareCtas;
+  return n < kMinShare ? kMinShare : n;
+}
 
 template <typename T>
 __device__ __forceinline__ float lam_of(const amc_diff_attention& p, int h) {
@@ -107,26 +158,24 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane >> 2, pos = lane & 3;
   uint64_t* full = (uint64_t*)(sm + kStageBytes) + warp * kStages;
   volatile int* failed = (volatile int*)(sm + kStageBytes + 256);
-  const int unit = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
-  const int rb = unit % a.row_blocks, g = unit / a.row_blocks % p.kv_heads, b = unit / a.row_blocks / p.kv_heads;
-  const int rows = min(kRows, a.group * p.nq - rb * kRows);
-  const DiffLens len = diff_lens(p, b);
-  int kmax = 0;   // keys that any row of the block sees
-  int lim[2];     // of this lane's two rows
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int rr = quad + 8 * r;
-    int h, i;
-    unit_row(p, a, g, rb * kRows + min(rr, rows - 1), h, i);
-    lim[r] = rr < rows ? diff_limit(len, p.causal, i) : 0;
-    kmax = max(kmax, lim[r]);
+  const int per_seq = p.kv_heads * a.row_blocks;
+  int64_t at, end;   // this CTA's blocks on the line
+  Unit first_unit{0, 0, 0, 0};
+  if (a.shared) {
+    const int64_t total = line_blocks(p, per_seq), share = share_of(total);
+    at = share * blockIdx.x;
+    end = at + share < total ? at + share : total;
+    if (at >= end) {
+      if (blockIdx.x) return;
+      end = at;
+    }
+  } else {
+    first_unit.b = blockIdx.x / per_seq;
+    first_unit.u = blockIdx.x % per_seq;
+    first_unit.blocks = seq_blocks(p, first_unit.b);
+    at = 0;
+    end = first_unit.blocks;
   }
-#pragma unroll
-  for (int o = 16; o >= 4; o >>= 1) kmax = max(kmax, __shfl_xor_sync(0xffffffffu, kmax, o));
-  const int kbeg = split * a.chunk, kend = min(kmax, kbeg + a.chunk);
-  // box n of this warp starts at key kbeg + 16 (warp + 4 n)
-  const int boxes = kend > kbeg ? (kend - kbeg + 15) / 16 : 0;
-  const int mine = boxes > warp ? (boxes - warp + kWarps - 1) / kWarps : 0;
   unsigned char* ring = sm + warp * kStages * kBox;
   if (lane == 0) {
     for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
@@ -134,13 +183,34 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
     mbar_fence_init();
   }
   __syncthreads();
+  const int64_t begin = at;
+  int used = 0;   // boxes of this warp before this part
+  do {
+  const Unit unit = a.shared ? find_unit(p, per_seq, at) : first_unit;
+  const int rb = unit.u % a.row_blocks, g = unit.u / a.row_blocks, b = unit.b;
+  const int rows = min(kRows, a.group * p.nq - rb * kRows);
+  const DiffLens len = diff_lens(p, b);
+  const int64_t stop = min(end, unit.first + unit.blocks);
+  const int kbeg = (int)(at - unit.first) * 64, kend = min(len.nq > 0 ? len.nk : 0, (int)(stop - unit.first) * 64);
+  int lim[2];     // keys that this lane's two rows see
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int rr = quad + 8 * r;
+    int h, i;
+    unit_row(p, a, g, rb * kRows + min(rr, rows - 1), h, i);
+    lim[r] = rr < rows ? diff_limit(len, p.causal, i) : 0;
+  }
+  // box n of this warp starts at key kbeg + 16 (warp + 4 n)
+  const int boxes = kend > kbeg ? (kend - kbeg + 15) / 16 : 0;
+  const int mine = boxes > warp ? (boxes - warp + kWarps - 1) / kWarps : 0;
   auto load = [&](int n) {
-    unsigned char* st = ring + n % kStages * kBox;
+    const int s = (used + n) % kStages;
+    unsigned char* st = ring + s * kBox;
     const int key = kbeg + 16 * (warp + kWarps * n);
-    mbar_expect_tx(&full[n % kStages], 4096 + NV / 64 * 2048);
-    tma_load_4d(st, &mK, 0, key, 2 * g, b, &full[n % kStages]);
-    tma_load_4d(st + 2048, &mK, 0, key, 2 * g + 1, b, &full[n % kStages]);
-    for (int c = 0; c < NV / 64; ++c) tma_load_4d(st + 4096 + c * 2048, &mV, 64 * c, key, g, b, &full[n % kStages]);
+    mbar_expect_tx(&full[s], 4096 + NV / 64 * 2048);
+    tma_load_4d(st, &mK, 0, key, 2 * g, b, &full[s]);
+    tma_load_4d(st + 2048, &mK, 0, key, 2 * g + 1, b, &full[s]);
+    for (int c = 0; c < NV / 64; ++c) tma_load_4d(st + 4096 + c * 2048, &mV, 64 * c, key, g, b, &full[s]);
   };
   if (lane == 0)
     for (int n = 0; n < kStages && n < mine; ++n) load(n);
@@ -174,9 +244,10 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
   const int mrow = lane & 7, mid = lane >> 3;   // ldmatrix: row and matrix of this lane's address
   bool ok = true;
   for (int n = 0; n < mine; ++n) {
-    unsigned char* st = ring + n % kStages * kBox;
+    const int s = (used + n) % kStages;
+    unsigned char* st = ring + s * kBox;
     const int key = kbeg + 16 * (warp + kWarps * n);
-    ok = __all_sync(0xffffffffu, mbar_wait(&full[n % kStages], (uint32_t)(n / kStages) & 1u));
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (uint32_t)((used + n) / kStages) & 1u));
     if (!ok) break;
     if (key + 16 > len.nk && len.nk < p.nk) {
       // V behind the length may hold anything, and 0 times it is not 0
@@ -191,27 +262,27 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
     uint32_t ph[2][4], pl[2][4];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      float s[2][4] = {};
+      float sc[2][4] = {};
       const uint32_t kb = smem_addr(st + m * 2048) + (mrow + (mid >> 1) * 8) * 128;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         uint32_t f[4];
         ldsm4(f, kb + (((2 * k + (mid & 1)) ^ mrow) << 4));
-        mma16<T>(s[0], q[m][k], f[0], f[1]);
-        mma16<T>(s[1], q[m][k], f[2], f[3]);
+        mma16<T>(sc[0], q[m][k], f[0], f[1]);
+        mma16<T>(sc[1], q[m][k], f[2], f[3]);
       }
       if (key + 16 > min(lim[0], lim[1])) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (key + 8 * t + 2 * pos + (e & 1) >= lim[e >> 1]) s[t][e] = -INFINITY;
+            if (key + 8 * t + 2 * pos + (e & 1) >= lim[e >> 1]) sc[t][e] = -INFINITY;
       }
       bool up = false;
       float mt[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float x = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+        float x = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
         mt[r] = x * c2;
@@ -237,7 +308,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float base = top[m][r] == -INFINITY ? 0.f : top[m][r];
-          const float p0 = ex2_approx(fmaf(s[t][2 * r], c2, -base)), p1 = ex2_approx(fmaf(s[t][2 * r + 1], c2, -base));
+          const float p0 = ex2_approx(fmaf(sc[t][2 * r], c2, -base)), p1 = ex2_approx(fmaf(sc[t][2 * r + 1], c2, -base));
           sum[m][r] += p0 + p1;
           const uint32_t hi = pack2<T>(p0, p1);
           const float2 back = unpack2<T>(hi);
@@ -265,7 +336,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
     if (lane == 0) {
       *failed = 1;
       atomicExch(&g_diff_split_error, AMC_ERR_TIMEOUT);
-      for (int s = 0; s < kStages && s < mine; ++s) mbar_wait(&full[s], 0, 1 << 14);
+      for (int s = 0; s < kStages; ++s) mbar_wait(&full[s], 0, 1 << 14);
     }
   }
   // ---- join the four warps: rows' maxima, then sums and outputs over them
@@ -309,14 +380,16 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
           acc[m][c] = fmaf(xo[((w * 2 + m) * kRows + row) * NV + 32 * c + lane], f, acc[m][c]);
       }
     }
-    if (a.splits > 1) {
-      const int64_t at = ((int64_t)blockIdx.x * kRows + row) * 2;
+    if (a.shared && stop - at < unit.blocks) {
+      // part of a unit: the end of one that this CTA's share begins with, or
+      // (or also) the beginning of one
+      const int64_t slot = (((int64_t)blockIdx.x * 2 + (at > begin)) * kRows + row) * 2;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        if (lane == 0) a.part_ml[at + m] = make_float2(mx[m], l[m]);
+        if (lane == 0) a.part_ml[slot + m] = make_float2(mx[m], l[m]);
 #pragma unroll
         for (int c = 0; c < NV / 32; ++c)
-          if (32 * c + lane < p.dv) a.part[(at + m) * p.dv + 32 * c + lane] = acc[m][c];
+          if (32 * c + lane < p.dv) a.part[(slot + m) * p.dv + 32 * c + lane] = acc[m][c];
       }
     } else {
       const float lam = lam_of<T>(p, h);
@@ -332,40 +405,74 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
       }
     }
   }
+  used += mine;
+  at = stop;
+  __syncthreads();   // the exchange is read before the next part's boxes land there
+  fence_proxy_async();
+  } while (at < end);
 }
 
-// One CTA per (batch, head, row): its chunks' outputs over their joint maxima.
+// One CTA per (batch, head, row) of the sequences that several CTAs worked on,
+// and of those without a key: the parts' outputs over their joint maxima.
 template <typename T>
-__global__ void __launch_bounds__(128) k_diff_join(const __grid_constant__ amc_diff_attention p,
+__global__ void __launch_bounds__(256) k_diff_join(const __grid_constant__ amc_diff_attention p,
                                                    const __grid_constant__ SplitArgs a) {
+  __shared__ float2 ml[2][kShareCtas + 1];
+  __shared__ float other[256];
   const int i = blockIdx.x % p.nq, h = blockIdx.x / p.nq % p.heads, b = blockIdx.x / p.nq / p.heads;
-  const int g = h / a.group, rr = (h - g * a.group) * p.nq + i;
-  const int64_t unit = ((int64_t)b * p.kv_heads + g) * a.row_blocks + rr / kRows;
-  const DiffLens len = diff_lens(p, b);
-  const int n = min(a.splits, (diff_limit(len, p.causal, i) + a.chunk - 1) / a.chunk);   // chunks this row sees
-  const float lam = lam_of<T>(p, h);
-  const int64_t at0 = (unit * a.splits * kRows + rr % kRows) * 2;
-  const int64_t step = kRows * 2;
-  float res[2], lse[2];
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    float mx = -INFINITY;
-    for (int s = 0; s < n; ++s) mx = fmaxf(mx, a.part_ml[at0 + s * step + m].x);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float l = 0.f, acc = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-      const float2 e = a.part_ml[at0 + s * step + m];
-      const float f = exp2f(e.x - base);
-      l = fmaf(e.y, f, l);
-      if (threadIdx.x < p.dv) acc = fmaf(a.part[(at0 + s * step + m) * p.dv + threadIdx.x], f, acc);
+  const int g = h / a.group, rr = (h - g * a.group) * p.nq + i, per_seq = p.kv_heads * a.row_blocks;
+  const int tid = threadIdx.x, m = tid >> 7, c = tid & 127;
+  const int blocks = seq_blocks(p, b);
+  int n = 0, c0 = 0;
+  int64_t first = 0, share = 1;
+  if (blocks) {
+    // this unit's place on the line: the blocks of the sequences before, by every warp
+    int64_t before = 0, total = 0;
+    for (int q = tid & 31; q < p.batch; q += 32) {
+      const int64_t s = seq_blocks(p, q);
+      total += s;
+      if (q < b) before += s;
     }
-    res[m] = l > 0.f ? acc / l : 0.f;
-    lse[m] = l > 0.f ? fmaf(mx, kLn2, logf(l)) : -INFINITY;
+    for (int o = 16; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    share = share_of(total * per_seq);
+    first = before * per_seq + (int64_t)(g * a.row_blocks + rr / kRows) * blocks;
+    c0 = (int)(first / share);
+    n = (int)((first + blocks - 1) / share) - c0 + 1;
+    if (n == 1) return;   // one CTA saw all its keys and wrote the result
   }
-  if (threadIdx.x < p.dv) put_result<T>(p, b, h, i, threadIdx.x, fmaf(-lam, res[1], res[0]), res[1]);
-  if (p.lse && threadIdx.x < 2)
-    p.lse[((int64_t)b * 2 * p.heads + 2 * h + threadIdx.x) * p.nq + i] = threadIdx.x ? lse[1] : lse[0];
+  // CTA c0 + k holds this unit as its first, but for c0 itself if its share began before
+  auto slot = [&](int k) -> int64_t {
+    const int second = k == 0 && first > c0 * share;
+    return (((int64_t)(c0 + k) * 2 + second) * kRows + rr % kRows) * 2 + m;
+  };
+  for (int k = c; k < n; k += 128) ml[m][k] = a.part_ml[slot(k)];
+  __syncthreads();
+  float mx = -INFINITY, l = 0.f;
+  for (int k = tid & 31; k < n; k += 32) mx = fmaxf(mx, ml[m][k].x);
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const float base = mx == -INFINITY ? 0.f : mx;
+  for (int k = tid & 31; k < n; k += 32) l = fmaf(ml[m][k].y, exp2f(ml[m][k].x - base), l);
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float lam = lam_of<T>(p, h);
+  for (int c1 = 0; c1 < p.dv; c1 += 128) {
+    const int col = c1 + c;
+    float acc = 0.f;
+    if (col < p.dv) {
+#pragma unroll 8
+      for (int k = 0; k < n; ++k) acc = fmaf(a.part[slot(k) * p.dv + col], exp2f(ml[m][k].x - base), acc);
+    }
+    acc *= inv;
+    other[tid] = acc;
+    __syncthreads();
+    if (m == 0 && col < p.dv) put_result<T>(p, b, h, i, col, fmaf(-lam, other[tid + 128], acc), other[tid + 128]);
+    __syncthreads();
+  }
+  if (p.lse && c == 0)
+    p.lse[((int64_t)b * 2 * p.heads + 2 * h + m) * p.nq + i] = l > 0.f ? fmaf(mx, kLn2, logf(l)) : -INFINITY;
 }
 
 namespace {
@@ -374,29 +481,24 @@ SplitArgs plan(const amc_diff_attention& p) {
   SplitArgs a{};
   a.group = p.heads / p.kv_heads;
   a.row_blocks = (int)(((int64_t)a.group * p.nq + kRows - 1) / kRows);
+  // Units go to a CTA each where there are plenty of them, or where a cache
+  // is so short that a second kernel would cost more than it shares out.
   const int64_t units = (int64_t)p.batch * p.kv_heads * a.row_blocks;
-  int64_t want = (kTargetCtas + units - 1) / units;
-  const int64_t most = (p.nk + kMinChunk - 1) / kMinChunk;
-  if (want > most) want = most;
-  if (want < 1) want = 1;
-  a.chunk = (int)(((p.nk + want - 1) / want + 63) / 64 * 64);
-  a.splits = (p.nk + a.chunk - 1) / a.chunk;
+  a.shared = units < 2 * kShareCtas && p.batch <= kMaxBatch && p.nk > 64 * kMinShare;
   return a;
 }
 
-size_t part_elems(const amc_diff_attention& p, const SplitArgs& a) {
-  return (size_t)p.batch * p.kv_heads * a.row_blocks * a.splits * kRows * 2;
-}
+constexpr size_t kPartRows = (size_t)kShareCtas * 2 * kRows * 2;
 
 template <typename T, int NV>
 int split_launch(const amc_diff_attention& p, const SplitArgs& a, const CUtensorMap (&map)[2], cudaStream_t s) {
   static std::atomic<uint64_t> attr{0};
   if (int rc = smem_attr_once(k_diff_split<T, NV>, kSplitSmem, attr)) return rc;
-  const unsigned grid = (unsigned)((int64_t)p.batch * p.kv_heads * a.row_blocks * a.splits);
+  const unsigned grid = a.shared ? kShareCtas : (unsigned)((int64_t)p.batch * p.kv_heads * a.row_blocks);
   k_diff_split<T, NV><<<grid, kWarps * 32, kSplitSmem, s>>>(map[0], map[1], p, a);
   AMC_CUDA(cudaGetLastError());
-  if (a.splits > 1) {
-    k_diff_join<T><<<(unsigned)((int64_t)p.batch * p.heads * p.nq), 128, 0, s>>>(p, a);
+  if (a.shared) {
+    k_diff_join<T><<<(unsigned)((int64_t)p.batch * p.heads * p.nq), 256, 0, s>>>(p, a);
     AMC_CUDA(cudaGetLastError());
   }
   return AMC_OK;
@@ -411,9 +513,8 @@ static bool split_shape(const amc_diff_attention& p) {
 }
 
 size_t diff_split_bytes(const amc_diff_attention& p) {
-  if (!split_shape(p)) return 0;
-  const SplitArgs a = plan(p);
-  return a.splits > 1 ? part_elems(p, a) * (p.dv * sizeof(float) + sizeof(float2)) : 0;
+  if (!split_shape(p) || !plan(p).shared) return 0;
+  return kPartRows * (p.dv * sizeof(float) + sizeof(float2));
 }
 
 int diff_fwd_split(const amc_diff_attention& p, cudaStream_t s, bool* handled) {
@@ -430,7 +531,7 @@ int diff_fwd_split(const amc_diff_attention& p, cudaStream_t s, bool* handled) {
   *handled = true;
   SplitArgs a = plan(p);
   a.part_ml = (float2*)p.workspace;
-  a.part = (float*)(a.part_ml + part_elems(p, a));
+  a.part = (float*)(a.part_ml + kPartRows);
   if (bf16) return p.dv <= 64 ? split_launch<__nv_bfloat16, 64>(p, a, map, s) : split_launch<__nv_bfloat16, 128>(p, a, map, s);
   return p.dv <= 64 ? split_launch<__half, 64>(p, a, map, s) : split_launch<__half, 128>(p, a, map, s);
 }

@@ -246,6 +246,11 @@ FWD = [
     dict(B=3, H=4, K=1, nq=1, nk=1500, d=64, causal=True, q_lens=[1, 1, 0], kv_lens=[1500, 257, 9]),   # one token
     dict(B=2, H=4, K=2, nq=4, nk=1030, d=64, causal=True, kv_lens=[1029, 2]),    # a few; rows that see no key
     dict(B=1, H=16, K=1, nq=1, nk=700, d=32),
+    dict(B=7, H=4, K=2, nq=1, nk=3001, d=64, causal=True, q_lens=[1, 1, 0, 1, 1, 1, 1],      # shared out unevenly
+         kv_lens=[3001, 64, 500, 0, 65, 1, 2900]),
+    dict(B=40, H=2, K=1, nq=3, nk=5000, d=16),                                               # shares of several units
+    dict(B=300, H=2, K=2, nq=1, nk=300, d=32, causal=True, kv_lens=[(7 * i) % 301 for i in range(300)]),
+    dict(B=3, H=2, K=1, nq=1, nk=700, d=64, q_lens=[0, 0, 0]),
     dict(B=1, H=2, K=2, nq=16, nk=530, d=40, dv=72),
     dict(B=2, H=3, K=3, nq=2, nk=137, d=64, heads_inner=False),
     dict(B=1, H=2, K=1, nq=70, nk=70, d=100, dv=200, causal=True),    # wide head
