@@ -1,11 +1,14 @@
 // Rotary positions: pair i of a row at position p turns by p * freqs[i].
 //   a' = ms (a cos - b sin),  b' = ms (b cos + a sin);  the inverse turn is
 //   the gradient (the transpose of the same matrix).
-// The bound is HBM: each element is read and written once.  A thread keeps
-// the sines of V pairs of one row in registers and applies them to every head
-// of that row it owns, so the angles cost little: the turn count is formed
-// and reduced to half a turn in f64 (a position of 2^40 keeps its angle), its
-// sine and cosine in f32.  No table is read.
+// The bound is HBM: each element is read and written once.  A warp owns one row
+// (a position) of the batch: its lanes form the sines and cosines of the row's
+// pairs once, into shared memory, and then go over the 16-byte vectors of every
+// head of both tensors, four in flight a lane, so a position's heads, which a
+// projection leaves side by side, move in whole lines.  The first vectors are
+// loaded before the angles are formed.  The turn count is formed and reduced to
+// half a turn in f64 (a position of 2^40 keeps its angle), its sine and cosine
+// in f32.  No table is read.
 #include <cmath>
 
 #include "amc_half.cuh"
@@ -15,14 +18,15 @@ namespace amc {
 
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeWarps = 4;
+constexpr int kRopeFlight = 4;       // vectors (pairs of them) in flight a lane
+constexpr int kRopeMaxRot = 1024;
 
 struct RopeArgs {
   amc_rope_tensor t[2];
-  int chunks0;                 // head chunks of tensor 0; the rest are tensor 1's
-  int heads_per;               // heads per chunk
   int64_t rows, n;             // batch * n, n
-  int d, rot, pair_units, units;
+  int d, rot, pair_units, units;   // V pairs each, and with the V-element pieces behind rot
+  int items0, items;           // vectors of a row: of tensor 0, of both
   const int64_t* pos;
   int64_t pos_stride;
   const double* freqs;
@@ -60,69 +64,98 @@ struct Vec {
 
 }  // namespace
 
-// One thread: one row, V pairs (or V copied elements behind rot), heads_per heads.
 template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(kRopeThreads) k_rope(const __grid_constant__ RopeArgs a) {
-  const int64_t id = (int64_t)blockIdx.x * kRopeThreads + threadIdx.x;
-  const int64_t row = id / a.units;
-  const int u = (int)(id % a.units);
+__global__ void __launch_bounds__(kRopeWarps * 32) k_rope(const __grid_constant__ RopeArgs a) {
+  extern __shared__ float2 rope_sm[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * kRopeWarps + warp;
   if (row >= a.rows) return;
-  const int which = (int)blockIdx.y >= a.chunks0;
-  const amc_rope_tensor& t = a.t[which];
-  const int64_t h0 = (int64_t)(blockIdx.y - (which ? a.chunks0 : 0)) * a.heads_per;
-  const int64_t h1 = min(h0 + a.heads_per, t.heads);
+  float2* turn = rope_sm + warp * (a.rot / 2);   // (cos, sin) of each pair
   const int64_t b = row / a.n, i = row % a.n;
-  const T* x = (const T*)t.x + b * t.xs[0] + h0 * t.xs[1] + i * t.xs[2];
-  T* o = (T*)t.out + b * t.os[0] + h0 * t.os[1] + i * t.os[2];
-  const int64_t xh = t.xs[1], oh = t.os[1];
-  if (u >= a.pair_units) {
-    const int c = a.rot + (u - a.pair_units) * V;
-    for (int64_t h = h0; h < h1; ++h, x += xh, o += oh) {
-      Vec<T, V> v;
-      v.load(x + c);
-      v.store(o + c);
-    }
-    return;
+  const T* x[2];
+  T* o[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    x[k] = (const T*)a.t[k].x + b * a.t[k].xs[0] + i * a.t[k].xs[2];
+    o[k] = (T*)a.t[k].out + b * a.t[k].os[0] + i * a.t[k].os[2];
   }
-  float co[V], si[V];
+  Vec<T, V> va[kRopeFlight], vb[kRopeFlight];
+  // item -> its tensor, head and unit; the first of its elements (a pair's
+  // other half is `gap` further, nothing behind rot)
+  auto place = [&](int item, int& k, int64_t& h, int& u, int& c) {
+    k = item >= a.items0;
+    const int q = item - (k ? a.items0 : 0);
+    h = q / a.units;
+    u = q - (int)h * a.units;
+    c = u >= a.pair_units ? a.rot + (u - a.pair_units) * V : INTER ? u * 2 * V : u * V;
+  };
+  const int gap = INTER ? V : a.rot / 2;
+  auto load = [&](int base) {
+#pragma unroll
+    for (int f = 0; f < kRopeFlight; ++f) {
+      const int item = base + 32 * f;
+      if (item >= a.items) break;
+      int k, u, c;
+      int64_t h;
+      place(item, k, h, u, c);
+      const T* src = (k ? x[1] : x[0]) + h * a.t[k].xs[1] + c;
+      va[f].load(src);
+      if (u < a.pair_units) vb[f].load(src + gap);
+    }
+  };
+  load(lane);
   const double p = (double)a.pos[b * a.pos_stride + i];
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    double turns = p * (a.freqs[u * V + k] * 0.15915494309189533577);   // 1 / (2 pi)
+  for (int k = lane; k < a.rot / 2; k += 32) {
+    double turns = p * (a.freqs[k] * 0.15915494309189533577);   // 1 / (2 pi)
     turns -= rint(turns);
-    sincospif(2.f * (float)turns, &si[k], &co[k]);
-    co[k] *= a.mscale;
-    si[k] *= a.inverse ? -a.mscale : a.mscale;
+    float2 t;
+    sincospif(2.f * (float)turns, &t.y, &t.x);
+    turn[k] = make_float2(t.x * a.mscale, t.y * (a.inverse ? -a.mscale : a.mscale));
   }
-  const int ca = INTER ? u * 2 * V : u * V, cb = INTER ? ca + V : ca + a.rot / 2;
-#pragma unroll 4
-  for (int64_t h = h0; h < h1; ++h, x += xh, o += oh) {
-    Vec<T, V> va, vb;
-    va.load(x + ca);
-    vb.load(x + cb);
-    if constexpr (INTER) {
-      float e[2 * V];
+  __syncwarp();
+  for (int base = lane; base < a.items; base += 32 * kRopeFlight) {
+    if (base != lane) load(base);
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        e[k] = to_f32(va.e[k]);
-        e[V + k] = to_f32(vb.e[k]);
-      }
+    for (int f = 0; f < kRopeFlight; ++f) {
+      const int item = base + 32 * f;
+      if (item >= a.items) break;
+      int k, u, c;
+      int64_t h;
+      place(item, k, h, u, c);
+      T* dst = (k ? o[1] : o[0]) + h * a.t[k].os[1] + c;
+      if (u < a.pair_units) {
+        if constexpr (INTER) {
+          float e[2 * V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float r = e[2 * k] * co[k] - e[2 * k + 1] * si[k], q = e[2 * k + 1] * co[k] + e[2 * k] * si[k];
-        (2 * k < V ? va.e[2 * k < V ? 2 * k : 0] : vb.e[2 * k < V ? 0 : 2 * k - V]) = from_f32<T>(r);
-        (2 * k + 1 < V ? va.e[2 * k + 1 < V ? 2 * k + 1 : 0] : vb.e[2 * k + 1 < V ? 0 : 2 * k + 1 - V]) = from_f32<T>(q);
-      }
-    } else {
+          for (int q = 0; q < V; ++q) {
+            e[q] = to_f32(va[f].e[q]);
+            e[V + q] = to_f32(vb[f].e[q]);
+          }
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float xa = to_f32(va.e[k]), xb = to_f32(vb.e[k]);
-        va.e[k] = from_f32<T>(xa * co[k] - xb * si[k]);
-        vb.e[k] = from_f32<T>(xb * co[k] + xa * si[k]);
+          for (int q = 0; q < V; ++q) {
+            const float2 t = turn[u * V + q];
+            const float xa = e[2 * q], xb = e[2 * q + 1];
+            e[2 * q] = xa * t.x - xb * t.y;
+            e[2 * q + 1] = xb * t.x + xa * t.y;
+          }
+#pragma unroll
+          for (int q = 0; q < V; ++q) {
+            va[f].e[q] = from_f32<T>(e[q]);
+            vb[f].e[q] = from_f32<T>(e[V + q]);
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < V; ++q) {
+            const float2 t = turn[u * V + q];
+            const float xa = to_f32(va[f].e[q]), xb = to_f32(vb[f].e[q]);
+            va[f].e[q] = from_f32<T>(xa * t.x - xb * t.y);
+            vb[f].e[q] = from_f32<T>(xb * t.x + xa * t.y);
+          }
+        }
+        vb[f].store(dst + gap);
       }
+      va[f].store(dst);
     }
-    va.store(o + ca);
-    vb.store(o + cb);
   }
 }
 
@@ -132,19 +165,14 @@ template <typename T, int V>
 int rope_launch(RopeArgs& a, int count, bool inter, cudaStream_t s) {
   a.pair_units = a.rot / 2 / V;
   a.units = a.pair_units + (a.d - a.rot) / V;
-  const int64_t threads = a.rows * a.units;
-  const int64_t blocks = (threads + kRopeThreads - 1) / kRopeThreads;
-  if (blocks > 0x7fffffff) return fail(AMC_ERR_INVALID, "amc_rope: too many rows");
-  // Heads per thread: as many as leave four full waves of threads.
-  const int64_t hmax = count > 1 && a.t[1].heads > a.t[0].heads ? a.t[1].heads : a.t[0].heads;
-  int64_t per = 16;
-  while (per > 1 && blocks * ((hmax + per - 1) / per) < 4 * (int64_t)num_sms()) per /= 2;
-  a.heads_per = (int)per;
-  a.chunks0 = (int)((a.t[0].heads + per - 1) / per);
-  const int chunks = a.chunks0 + (count > 1 ? (int)((a.t[1].heads + per - 1) / per) : 0);
-  const dim3 grid((unsigned)blocks, (unsigned)chunks);
-  if (inter) k_rope<T, V, true><<<grid, kRopeThreads, 0, s>>>(a);
-  else k_rope<T, V, false><<<grid, kRopeThreads, 0, s>>>(a);
+  const int64_t blocks = (a.rows + kRopeWarps - 1) / kRopeWarps;
+  const int64_t items0 = a.t[0].heads * a.units, items1 = count > 1 ? a.t[1].heads * a.units : 0;
+  if (blocks > 0x7fffffff || items0 + items1 > 0x3fffffff) return fail(AMC_ERR_INVALID, "amc_rope: too many rows or elements a row");
+  a.items0 = (int)items0;
+  a.items = (int)(items0 + items1);
+  const size_t sm = (size_t)kRopeWarps * (a.rot / 2) * sizeof(float2);
+  if (inter) k_rope<T, V, true><<<(unsigned)blocks, kRopeWarps * 32, sm, s>>>(a);
+  else k_rope<T, V, false><<<(unsigned)blocks, kRopeWarps * 32, sm, s>>>(a);
   AMC_CUDA(cudaGetLastError());
   return AMC_OK;
 }
@@ -183,8 +211,8 @@ int amc_rope(const amc_rope_tensor* t, int32_t count, int32_t dtype, int64_t bat
   if (!t || count < 1 || count > 2) return fail(AMC_ERR_INVALID, "amc_rope: one or two tensors");
   if (dtype != AMC_F32 && dtype != AMC_BF16 && dtype != AMC_F16)
     return fail(AMC_ERR_INVALID, "amc_rope: dtype must be f32, bf16 or f16");
-  if (batch < 0 || n < 0 || d <= 0 || rot <= 0 || rot > d || rot % 2)
-    return fail(AMC_ERR_INVALID, "amc_rope: bad sizes (rot even, 2..d)");
+  if (batch < 0 || n < 0 || d <= 0 || rot <= 0 || rot > d || rot % 2 || rot > kRopeMaxRot)
+    return fail(AMC_ERR_INVALID, "amc_rope: bad sizes (rot even, 2..d, at most 1024)");
   RopeArgs a{};
   bool any = false;
   for (int k = 0; k < count; ++k) {

@@ -77,7 +77,7 @@ def c_rope(count=1, dtype=A.F32, batch=1, n=1, d=8, rot=8, pos=16, freqs=16, x=1
 
 
 @pytest.mark.parametrize("bad", [dict(count=0), dict(count=3), dict(dtype=A.F64), dict(d=0), dict(rot=10), dict(rot=3),
-                                 dict(rot=0), dict(batch=-1), dict(n=-1), dict(pos=None), dict(freqs=None),
+                                 dict(rot=0), dict(rot=1026, d=1100), dict(batch=-1), dict(n=-1), dict(pos=None), dict(freqs=None),
                                  dict(x=None), dict(heads=-1), dict(heads=40000), dict(batch=1 << 30, n=1 << 30)])
 def test_c_rope_refusals(bad):
     assert c_rope(**bad) == 1
