@@ -18,6 +18,7 @@
 
 #include "amc_diffattn.h"
 #include "amc_half.cuh"
+#include "amc_tc.cuh"
 
 namespace amc {
 
@@ -48,13 +49,32 @@ __device__ __forceinline__ float lam_of(const amc_diff_attention& p, int h) {
 }
 
 // rows r0 .. r0+TT of a (rows, dim) matrix into dst[TT][W], zero outside
-// rows < rows_end and columns < dim.
+// rows < rows_end and columns < dim.  f32 rows on 16-byte boundaries are
+// copied asynchronously (complete at tile_wait), others converted on the way.
 template <typename T, int TT, int W, int PITCH>
 __device__ __forceinline__ void load_tile(float* dst, const T* src, int64_t stride, int r0, int rows_end, int dim) {
+  if constexpr (sizeof(T) == 4) {
+    if (!((uintptr_t)src & 15) && stride % 4 == 0 && dim % 4 == 0) {
+      for (int i = threadIdx.x; i < TT * W / 4; i += 256) {
+        const int r = i / (W / 4), c = i % (W / 4) * 4;
+        const bool in = r0 + r < rows_end && c < dim;
+        const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst + r * PITCH + c);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                     ::"r"(to), "l"(in ? src + (int64_t)(r0 + r) * stride + c : src), "r"(in ? 16 : 0) : "memory");
+      }
+      return;
+    }
+  }
   for (int i = threadIdx.x; i < TT * W; i += 256) {
     const int r = i / W, c = i % W;
     dst[r * PITCH + c] = (r0 + r < rows_end && c < dim) ? to_f32(src[(int64_t)(r0 + r) * stride + c]) : 0.f;
   }
+}
+__device__ __forceinline__ void tile_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the latest `N` committed loads of this thread are complete.
+template <int N>
+__device__ __forceinline__ void tile_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // acc[i][j] += sum_c A[ty + 16 i][c] B[tx + 16 j][c]
@@ -74,15 +94,12 @@ __device__ __forceinline__ void dot_rows(float (&acc)[R][R], const float* A, con
   }
 }
 
-// out[i][4 g + e] += sum_k W(ty + 16 i, k) X[k][4 tx + 64 g + e]; W is
-// w[row * PW + k], or transposed w[k * PW + row].
+// out[i][4 g + e] += sum_k W(row i, k) X[k][4 tx + 64 g + e].  W is
+// w[row * PW + k] with rows ty + 16 i, or transposed w[k * PW + row] with rows
+// R ty + i: either way one access brings several of its values.
 template <int R, int NC, int TT, int PW, int PX, bool TRANS>
 __device__ __forceinline__ void mul_rows(float (&out)[R][NC], const float* w, const float* X, int ty, int tx) {
-#pragma unroll 4
-  for (int k = 0; k < TT; ++k) {
-    float a[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i) a[i] = TRANS ? w[k * PW + ty + 16 * i] : w[(ty + 16 * i) * PW + k];
+  auto step = [&](const float (&a)[R], int k) {
 #pragma unroll
     for (int g = 0; g < NC / 4; ++g) {
       const float4 x = *reinterpret_cast<const float4*>(X + k * PX + 4 * tx + 64 * g);
@@ -94,15 +111,50 @@ __device__ __forceinline__ void mul_rows(float (&out)[R][NC], const float* w, co
         out[i][4 * g + 3] = fmaf(a[i], x.w, out[i][4 * g + 3]);
       }
     }
+  };
+  if constexpr (TRANS) {
+#pragma unroll 4
+    for (int k = 0; k < TT; ++k) {
+      float a[R];
+      if constexpr (R == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(w + k * PW + 4 * ty);
+        a[0] = v.x; a[1] = v.y; a[2] = v.z; a[3] = v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(w + k * PW + 2 * ty);
+        a[0] = v.x; a[1] = v.y;
+      }
+      step(a, k);
+    }
+  } else {
+#pragma unroll 2
+    for (int k = 0; k < TT; k += 4) {
+      float4 v[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) v[i] = *reinterpret_cast<const float4*>(w + (ty + 16 * i) * PW + k);
+      float a[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) a[i] = v[i].x;
+      step(a, k);
+#pragma unroll
+      for (int i = 0; i < R; ++i) a[i] = v[i].y;
+      step(a, k + 1);
+#pragma unroll
+      for (int i = 0; i < R; ++i) a[i] = v[i].z;
+      step(a, k + 2);
+#pragma unroll
+      for (int i = 0; i < R; ++i) a[i] = v[i].w;
+      step(a, k + 3);
+    }
   }
 }
 
-template <typename T, int R, int NC>
+// Rows as mul_rows has them.
+template <typename T, int R, int NC, bool TRANS>
 __device__ __forceinline__ void store_rows(T* dst, int64_t stride, const float (&v)[R][NC], float f, int r0, int rows,
                                            int dim, int ty, int tx) {
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const int r = r0 + ty + 16 * i;
+    const int r = r0 + (TRANS ? R * ty + i : ty + 16 * i);
     if (r >= rows) continue;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -115,7 +167,8 @@ __device__ __forceinline__ void store_rows(T* dst, int64_t stride, const float (
 template <int TT, int DM, int DV>
 struct Tile {
   static constexpr int R = TT / 16, PD = DM + 4, PV = DV + 4, PP = TT + 4;
-  static constexpr int fwd = (4 * TT * PD + TT * PV + 2 * TT * PP) * 4;
+  static constexpr int stage = 2 * TT * PD + TT * PV;   // K_1, K_2 and V of the forward's streamed tile
+  static constexpr int fwd = (2 * TT * PD + 2 * stage + 2 * TT * PP) * 4;
   static constexpr int dkv = (4 * TT * PD + 2 * TT * PV + 3 * TT * PP) * 4;
   static constexpr int dq = (4 * TT * PD + 2 * TT * PV + 2 * TT * PP) * 4;
 };
@@ -127,7 +180,7 @@ __global__ void __launch_bounds__(256, 1) k_diff_fwd_simt(const __grid_constant_
   using L = Tile<TT, DM, DV>;
   constexpr int R = L::R;
   extern __shared__ float diff_sm[];
-  float *sQ = diff_sm, *sK = sQ + 2 * TT * L::PD, *sV = sK + 2 * TT * L::PD, *sP = sV + TT * L::PV;
+  float *sQ = diff_sm, *sP = sQ + 2 * TT * L::PD, *stages = sP + 2 * TT * L::PP;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int r0 = blockIdx.x * TT, h = blockIdx.y, b = blockIdx.z, g = h / (p.heads / p.kv_heads);
   const DiffLens len = diff_lens(p, b);
@@ -152,13 +205,22 @@ __global__ void __launch_bounds__(256, 1) k_diff_fwd_simt(const __grid_constant_
   }
   const int last = min(r0 + TT, len.nq) - 1;
   const int kend = last >= r0 ? diff_limit(len, p.causal, last) : 0;
-  for (int k0 = 0; k0 < kend; k0 += TT) {
-    __syncthreads();
+  auto load = [&](int k0, int buf) {
+    float* st = stages + buf * L::stage;
     for (int m = 0; m < 2; ++m)
-      load_tile<T, TT, DM, L::PD>(sK + m * TT * L::PD, (const T*)p.k + b * p.ks[0] + (2 * g + m) * p.ks[1], p.ks[2], k0,
+      load_tile<T, TT, DM, L::PD>(st + m * TT * L::PD, (const T*)p.k + b * p.ks[0] + (2 * g + m) * p.ks[1], p.ks[2], k0,
                                   len.nk, p.d);
-    load_tile<T, TT, DV, L::PV>(sV, (const T*)p.v + b * p.vs[0] + g * p.vs[1], p.vs[2], k0, len.nk, p.dv);
+    load_tile<T, TT, DV, L::PV>(st + 2 * TT * L::PD, (const T*)p.v + b * p.vs[0] + g * p.vs[1], p.vs[2], k0, len.nk, p.dv);
+  };
+  if (kend > 0) load(0, 0);
+  tile_commit();
+  for (int k0 = 0, buf = 0; k0 < kend; k0 += TT, buf ^= 1) {
+    __syncthreads();   // the tile before is used up
+    if (k0 + TT < kend) load(k0 + TT, buf ^ 1);
+    tile_commit();
+    tile_wait<1>();
     __syncthreads();
+    const float *sK = stages + buf * L::stage, *sV = sK + 2 * TT * L::PD;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       float s[R][R] = {};
@@ -195,6 +257,7 @@ __global__ void __launch_bounds__(256, 1) k_diff_fwd_simt(const __grid_constant_
     for (int m = 0; m < 2; ++m)
       mul_rows<R, DV / 16, TT, L::PP, L::PV, false>(o[m], sP + m * TT * L::PP, sV, ty, tx);
   }
+  tile_wait<0>();
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int r = r0 + ty + 16 * i;
@@ -212,8 +275,8 @@ __global__ void __launch_bounds__(256, 1) k_diff_fwd_simt(const __grid_constant_
       o[0][i][c] = fmaf(-lam, o[1][i][c], o[0][i][c] * inv[0]);
     }
   }
-  store_rows<T, R, DV / 16>((T*)p.o + b * p.os[0] + h * p.os[1], p.os[2], o[0], 1.f, r0, p.nq, p.dv, ty, tx);
-  if (p.o2) store_rows<T, R, DV / 16>((T*)p.o2 + b * p.o2s[0] + h * p.o2s[1], p.o2s[2], o[1], 1.f, r0, p.nq, p.dv, ty, tx);
+  store_rows<T, R, DV / 16, false>((T*)p.o + b * p.os[0] + h * p.os[1], p.os[2], o[0], 1.f, r0, p.nq, p.dv, ty, tx);
+  if (p.o2) store_rows<T, R, DV / 16, false>((T*)p.o2 + b * p.o2s[0] + h * p.o2s[1], p.o2s[2], o[1], 1.f, r0, p.nq, p.dv, ty, tx);
 }
 
 // nlse and nsum from lse, o, o2 and dO, and lam of every head.  A row is
@@ -270,17 +333,20 @@ __global__ void __launch_bounds__(256) k_diff_bwd_rows(const __grid_constant__ a
   }
 }
 
-// dK, dV of TT keys of one key head: streams the rows of its query heads.
+// dK, dV of TT keys of one key head: streams the rows of its query heads.  Its
+// heads are shared by the `share` CTAs of a cluster, which add their parts up
+// in order of rank (as in the tensor-core kernel).
 template <typename T, int TT, int DM, int DV>
 __global__ void __launch_bounds__(256, 1) k_diff_dkv_simt(const __grid_constant__ amc_diff_attention p,
-                                                          const __grid_constant__ DiffBwdWork wk) {
+                                                          const __grid_constant__ DiffBwdWork wk, int share) {
   using L = Tile<TT, DM, DV>;
   constexpr int R = L::R;
   extern __shared__ float diff_sm[];
   float *sK = diff_sm, *sQ = sK + 2 * TT * L::PD, *sV = sQ + 2 * TT * L::PD, *sG = sV + TT * L::PV;
   float *sB = sG + TT * L::PV, *sS = sB + TT * L::PP;   // P_1 - lam P_2, then dS_1 and dS_2, as [row][key]
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int k0 = blockIdx.x * TT, g = blockIdx.y, b = blockIdx.z, group = p.heads / p.kv_heads;
+  const int k0 = blockIdx.x / share * TT, rank = blockIdx.x % share, g = blockIdx.y, b = blockIdx.z;
+  const int heads = p.heads / p.kv_heads / share, head0 = (g * share + rank) * heads;
   const DiffLens len = diff_lens(p, b);
   const float c2 = p.scale * kLog2e;
   const int dim4 = (p.d + 3) & ~3, dimv4 = (p.dv + 3) & ~3;
@@ -290,7 +356,7 @@ __global__ void __launch_bounds__(256, 1) k_diff_dkv_simt(const __grid_constant_
   load_tile<T, TT, DV, L::PV>(sV, (const T*)p.v + b * p.vs[0] + g * p.vs[1], p.vs[2], k0, len.nk, p.dv);
   float dk[2][R][DM / 16] = {}, dv[R][DV / 16] = {};
   const int first = diff_first_row(len, p.causal, k0) / TT * TT;
-  for (int h = g * group; h < (g + 1) * group; ++h) {
+  for (int h = head0; h < head0 + heads; ++h) {
     const float lam = wk.lam[h];
     for (int r0 = first; r0 < len.nq; r0 += TT) {
       __syncthreads();
@@ -298,6 +364,8 @@ __global__ void __launch_bounds__(256, 1) k_diff_dkv_simt(const __grid_constant_
         load_tile<T, TT, DM, L::PD>(sQ + m * TT * L::PD, (const T*)p.q + b * p.qs[0] + (2 * h + m) * p.qs[1], p.qs[2],
                                     r0, len.nq, p.d);
       load_tile<T, TT, DV, L::PV>(sG, (const T*)p.d_o + b * p.dos[0] + h * p.dos[1], p.dos[2], r0, len.nq, p.dv);
+      tile_commit();
+      tile_wait<0>();
       __syncthreads();
       float gv[R][R] = {}, both[R][R];
       dot_rows<R, L::PV>(gv, sG, sV, dimv4, ty, tx);
@@ -332,10 +400,51 @@ __global__ void __launch_bounds__(256, 1) k_diff_dkv_simt(const __grid_constant_
         mul_rows<R, DM / 16, TT, L::PP, L::PD, true>(dk[m], sS + m * TT * L::PP, sQ + m * TT * L::PD, ty, tx);
     }
   }
+  tile_wait<0>();
+  if (share > 1) {
+    // [map 1 | map 2 | dV] of this CTA, then each CTA's rows of the sum
+    constexpr int W = 2 * DM + DV;
+    float* part = diff_sm;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      float* row = part + (R * ty + i) * W;
+#pragma unroll
+      for (int c = 0; c < DM / 16; c += 4)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+          *reinterpret_cast<float4*>(row + m * DM + 4 * tx + 16 * c) =
+              make_float4(dk[m][i][c], dk[m][i][c + 1], dk[m][i][c + 2], dk[m][i][c + 3]);
+#pragma unroll
+      for (int c = 0; c < DV / 16; c += 4)
+        *reinterpret_cast<float4*>(row + 2 * DM + 4 * tx + 16 * c) = make_float4(dv[i][c], dv[i][c + 1], dv[i][c + 2], dv[i][c + 3]);
+    }
+    tc::cluster_sync();
+    const int rows = (TT + share - 1) / share;
+    for (int q = threadIdx.x; q < rows * (W / 4); q += 256) {
+      const int row = rank * rows + q / (W / 4), c = q % (W / 4) * 4, key = k0 + row;
+      if (row >= TT || key >= p.nk) continue;
+      float4 sum = tc::ld_cluster(part + row * W + c, 0);
+      for (int r = 1; r < share; ++r) {
+        const float4 v = tc::ld_cluster(part + row * W + c, r);
+        sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+      }
+      const int m = c / DM, cc = m < 2 ? c % DM : c - 2 * DM, dim = m < 2 ? p.d : p.dv;
+      const float f = m < 2 ? p.scale : 1.f;
+      T* dst = m < 2 ? (T*)p.dk + b * p.dks[0] + (2 * g + m) * p.dks[1] + (int64_t)key * p.dks[2]
+                     : (T*)p.dv_ + b * p.dvs[0] + g * p.dvs[1] + (int64_t)key * p.dvs[2];
+      const float s4[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (cc + e < dim) dst[cc + e] = from_f32<T>(s4[e] * f);
+    }
+    tc::cluster_sync();   // the others have read this CTA's part
+    return;
+  }
   for (int m = 0; m < 2; ++m)
-    store_rows<T, R, DM / 16>((T*)p.dk + b * p.dks[0] + (2 * g + m) * p.dks[1], p.dks[2], dk[m], p.scale, k0, p.nk, p.d,
+    store_rows<T, R, DM / 16, true>((T*)p.dk + b * p.dks[0] + (2 * g + m) * p.dks[1], p.dks[2], dk[m], p.scale, k0, p.nk, p.d,
                               ty, tx);
-  store_rows<T, R, DV / 16>((T*)p.dv_ + b * p.dvs[0] + g * p.dvs[1], p.dvs[2], dv, 1.f, k0, p.nk, p.dv, ty, tx);
+  store_rows<T, R, DV / 16, true>((T*)p.dv_ + b * p.dvs[0] + g * p.dvs[1], p.dvs[2], dv, 1.f, k0, p.nk, p.dv, ty, tx);
 }
 
 // dQ of TT rows, and this tile's part of sum P_2 G.
@@ -381,6 +490,8 @@ __global__ void __launch_bounds__(256, 1) k_diff_dq_simt(const __grid_constant__
       load_tile<T, TT, DM, L::PD>(sK + m * TT * L::PD, (const T*)p.k + b * p.ks[0] + (2 * g + m) * p.ks[1], p.ks[2], k0,
                                   len.nk, p.d);
     load_tile<T, TT, DV, L::PV>(sV, (const T*)p.v + b * p.vs[0] + g * p.vs[1], p.vs[2], k0, len.nk, p.dv);
+    tile_commit();
+    tile_wait<0>();
     __syncthreads();
     float gv[R][R] = {}, part = 0.f;
     dot_rows<R, L::PV>(gv, sG, sV, dimv4, ty, tx);
@@ -404,8 +515,9 @@ __global__ void __launch_bounds__(256, 1) k_diff_dq_simt(const __grid_constant__
     for (int m = 0; m < 2; ++m)
       mul_rows<R, DM / 16, TT, L::PP, L::PD, false>(dq[m], sS + m * TT * L::PP, sK + m * TT * L::PD, ty, tx);
   }
+  tile_wait<0>();
   for (int m = 0; m < 2; ++m)
-    store_rows<T, R, DM / 16>((T*)p.dq + b * p.dqs[0] + (2 * h + m) * p.dqs[1], p.dqs[2], dq[m], p.scale, r0, p.nq, p.d,
+    store_rows<T, R, DM / 16, false>((T*)p.dq + b * p.dqs[0] + (2 * h + m) * p.dqs[1], p.dqs[2], dq[m], p.scale, r0, p.nq, p.d,
                               ty, tx);
   for (int w = 16; w > 0; w >>= 1) pg += __shfl_xor_sync(0xffffffffu, pg, w);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = pg;
@@ -447,6 +559,18 @@ __global__ void __launch_bounds__(256) k_diff_dlam(const __grid_constant__ amc_d
 
 namespace {
 
+}  // namespace
+
+int diff_share(const amc_diff_attention& p, int64_t ctas) {
+  const int group = p.heads / p.kv_heads;
+  int share = 1;
+  for (int c = 2; c <= 8 && c <= group && ctas * share < num_sms(); ++c)
+    if (group % c == 0) share = c;
+  return share;
+}
+
+namespace {
+
 template <typename F>
 int by_type(int32_t dtype, F f) {
   if (dtype == AMC_F32) return f(float());
@@ -470,8 +594,19 @@ int bwd_simt(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s) 
   if (int rc = smem_attr_once(k_diff_dkv_simt<T, TT, DM, DV>, L::dkv, attr_dkv)) return rc;
   if (int rc = smem_attr_once(k_diff_dq_simt<T, TT, DM, DV>, L::dq, attr_dq)) return rc;
   if (p.nk) {
-    k_diff_dkv_simt<T, TT, DM, DV><<<dim3((p.nk + TT - 1) / TT, p.kv_heads, p.batch), 256, L::dkv, s>>>(p, w);
-    AMC_CUDA(cudaGetLastError());
+    const int key_tiles = (p.nk + TT - 1) / TT;
+    const int share = diff_share(p, (int64_t)key_tiles * p.kv_heads * p.batch);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(key_tiles * share, p.kv_heads, p.batch);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = L::dkv;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)share, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = share > 1 ? 1 : 0;
+    AMC_CUDA(cudaLaunchKernelEx(&cfg, k_diff_dkv_simt<T, TT, DM, DV>, p, w, share));
   }
   const int tiles = (p.nq + TT - 1) / TT;
   if (p.nq) {

@@ -72,6 +72,10 @@ int diff_fwd_tc(const amc_diff_attention& p, cudaStream_t s, bool* handled);
 size_t diff_split_bytes(const amc_diff_attention& p);
 int diff_fwd_split(const amc_diff_attention& p, cudaStream_t s, bool* handled);
 int launch_diff_fwd_simt(const amc_diff_attention& p, cudaStream_t s);
+// CTAs of a cluster that share the query heads of a key head in dK/dV: more
+// than one while `ctas`, one for each key tile of a key head, leave SMs idle
+// (6 heads over 2 at 5 x 1000 rows take 80).
+int diff_share(const amc_diff_attention& p, int64_t ctas);
 int launch_diff_bwd_rows(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s);
 int launch_diff_bwd_simt(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s);
 // Tensor-core gradients (after the rows), likewise.

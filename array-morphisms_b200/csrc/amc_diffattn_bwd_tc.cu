@@ -639,12 +639,7 @@ int bwd_tc(const amc_diff_attention& p, const DiffBwdWork& w, const CUtensorMap 
   if (int rc = smem_attr_once(k_diff_dq_tc<T, NV>, QSmem<NV>::bytes, attr_q)) return rc;
   const unsigned gk = (unsigned)((int64_t)((p.nk + 127) / 128) * p.kv_heads * p.batch);
   const int tiles = (p.nq + 127) / 128;
-  // Heads that share a key head go to a cluster of CTAs while one CTA for all
-  // of them leaves SMs idle: 6 heads over 2 at 5 x 1000 rows take 80 CTAs.
-  const int group = p.heads / p.kv_heads;
-  int share = 1;
-  for (int c = 2; c <= 8 && c <= group && (int64_t)gk * share < num_sms(); ++c)
-    if (group % c == 0) share = c;
+  const int share = diff_share(p, gk);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(gk * share);
   cfg.blockDim = dim3(kThreadsB);
