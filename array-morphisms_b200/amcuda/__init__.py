@@ -32,6 +32,6 @@ from .ssa import (morphism_to_ssa, ssa_constant_id, ssa_element_wise_fusion_pass
 from .realize import DeviceBuffer, Plan, force_morphism, init, morph_to_list, realize, to_numpy  # noqa: E402
 from .context import (MorphismContext, context_stats, finalize_context, make_morphism_context, plan_ctx,  # noqa: E402
                       realize_ctx, reset_context)
-from . import fn  # noqa: E402
+from . import fn, nn  # noqa: E402
 
 __all__ = [n for n in dir() if not n.startswith("_")]

@@ -97,7 +97,7 @@ def _rows(t, who: str, shape=None):
 def _written(t, strides, who: str) -> None:
     """An output must not map two elements to one place."""
     for n, s in zip(t.shape, strides):
-        if n > 1 and s == 0:
+        if n > 1 and s == 0 and t.numel():
             raise ValueError(f"{who}: an output cannot be broadcast (stride 0)")
 
 

@@ -661,7 +661,7 @@ int bwd_tc(const amc_diff_attention& p, const DiffBwdWork& w, const CUtensorMap 
 
 int diff_bwd_tc(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s, bool* handled) {
   *handled = false;
-  if (!diff_tc_shape(p) || p.nq <= 0) return AMC_OK;
+  if (!diff_tc_shape(p) || p.nq <= 0 || !(p.scale > 0.f)) return AMC_OK;   // masked scores are -inf before the scale
   if (!aligned_out(p.dq, p.dqs, 2 * p.heads, p.nq, p.batch) || !aligned_out(p.dk, p.dks, 2 * p.kv_heads, p.nk, p.batch) ||
       !aligned_out(p.dv_, p.dvs, p.kv_heads, p.nk, p.batch))
     return AMC_OK;

@@ -20,8 +20,9 @@
 //
 // Bound: per 128 x 128 tile of both maps the products take 1536 clocks of the
 // tensor pipe, their operands 1800 of the shared-memory port, and the 32768
-// exponentials 2048 of the special-function unit; a part of them goes to the
-// FMA pipe (exp2_poly2).
+// exponentials 2048 of the special-function unit.  Taking a part of those on
+// the FMA pipe by a polynomial gained nothing: the softmax threads' other
+// instructions then fill the time.
 // Every wait is bounded; on expiry the kernel records AMC_ERR_TIMEOUT and
 // leaves after its copies and products have drained.
 #include <cmath>

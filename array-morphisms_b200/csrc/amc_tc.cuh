@@ -265,25 +265,6 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
   asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^x on the FMA pipe for finite x in [-126, 127], to relieve the
-// special-function unit (16 a clock and SM): x = n + f with n the nearest
-// integer (added 1.5 * 2^23 leaves it in the low bits), the minimax polynomial
-// of degree 4 of 2^f on [-1/2, 1/2] (relative error 2.6e-6, by exchange), and
-// n added to the exponent.
-__device__ __forceinline__ float2 exp2_poly2(float2 x) {
-  const float2 big = make_float2(12582912.f, 12582912.f);
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
-  const float2 t = add2(x, big);
-  const float2 f = fma2(add2(t, make_float2(-12582912.f, -12582912.f)), make_float2(-1.f, -1.f), x);
-  float2 p = fma2(f, make_float2(0.009570102207362652f, 0.009570102207362652f),
-                  make_float2(0.05591785907745361f, 0.05591785907745361f));
-  p = fma2(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
-  p = fma2(p, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
-  p = fma2(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
-}
 // Nearest tf32 by integer rounding of the bit pattern (ties away from zero),
 // the same result as cvt.rna.tf32.f32 for finite values, on the integer pipe.
 __device__ __forceinline__ float round_tf32_int(float x) {

@@ -423,7 +423,9 @@ int amc_rope_freqs(double* host_out, int32_t rot, double base, int32_t kind, dou
  * with causal to j <= i + kv_lens[b] - q_lens[b] only: the last row sees the
  * last key.  Rows from q_lens[b] on, and rows that see no key, give 0 (lse
  * -inf) and no gradient.  Elements of q, k, v and d_o behind q_lens and
- * kv_lens are not used, whatever they hold.
+ * kv_lens are not used, whatever they hold; within the lengths a NaN or an
+ * infinity spreads as products spread it, masked or not.  Results must not
+ * overlap one another or what is read.
  * lse (batch, 2 heads, nq, contiguous) receives the natural-log row
  * log-sum-exp of each map, o2 (optional; the backward needs it) the second
  * map's P_2 V.  lam is (lam_rows, 4, d) contiguous of `dtype`, lam_rows 1

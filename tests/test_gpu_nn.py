@@ -253,6 +253,11 @@ FWD = [
     dict(B=3, H=2, K=1, nq=1, nk=700, d=64, q_lens=[0, 0, 0]),
     dict(B=1, H=2, K=2, nq=16, nk=530, d=40, dv=72),
     dict(B=2, H=3, K=3, nq=2, nk=137, d=64, heads_inner=False),
+    # many tiles: pairs of CTAs, several tiles each
+    dict(B=10, H=16, K=4, nq=130, nk=257, d=64, causal=True, q_lens=[130, 0, 1, 129, 128, 127, 77, 130, 130, 2],
+         kv_lens=[257, 257, 0, 5, 256, 255, 129, 64, 65, 200]),
+    dict(B=5, H=16, K=16, nq=300, nk=300, d=32, kv_lens=[300, 0, 299, 128, 1]),
+    dict(B=3, H=25, K=5, nq=513, nk=700, d=48, causal=True),
     dict(B=1, H=2, K=1, nq=70, nk=70, d=100, dv=200, causal=True),    # wide head
     dict(B=1, H=1, K=1, nq=33, nk=65, d=13, dv=7),                    # odd dims
     dict(B=1, H=2, K=1, nq=33, nk=65, d=64, heads_inner=False, lam_rows=1),
@@ -448,3 +453,182 @@ def test_adamw_more_tensors_than_one_launch_holds(nn):
     empty = torch.tensor([4, 0], device="cuda")
     nn.AdamW([], [], [], [], empty).step()
     assert empty.tolist() == [5, 0]
+
+
+# ---------------------------------------------------------------------------- how calls are made
+def test_diff_attention_alignments_and_strides_other_than_the_kernels_like(nn):
+    """Rows off 16 bytes, keys broadcast over the batch, a negative scale."""
+    c = Case(B=2, H=2, K=1, nq=70, nk=90, d=64, dtype="bf16", causal=True)
+    wide = randn((2, 90, 2 * 64 + 3), 7, torch.bfloat16)
+    c.k = wide[..., 3:].unflatten(-1, (2, 64)).transpose(1, 2)
+    o, lse, o2 = c.fwd(nn)
+    c.check({"o": o, "lse": lse, "o2": o2}, c.reference(), 90)
+    c.k = randn((1, 2, 90, 64), 8, torch.bfloat16).expand(2, 2, 90, 64)
+    got = c.fwd(nn)
+    c.check(dict(zip(("o", "lse", "o2"), got)), c.reference(), 90)
+    c.k = c.k.contiguous()
+    c.scale = -0.125
+    got = c.fwd(nn)
+    c.check({**dict(zip(("o", "lse", "o2"), got)), **c.bwd(nn, *got)}, c.reference(backward=True), 140)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,nq,nk", [(2, 5, 0), (2, 0, 5), (0, 5, 5), (2, 1, 0)])
+def test_diff_attention_of_nothing(nn, dtype, B, nq, nk):
+    """No keys, no rows, no sequences: zeros where there is something to write."""
+    c = Case(B=B, H=2, K=1, nq=nq, nk=nk, d=64, dtype=dtype, causal=True)
+    o, lse, o2 = c.fwd(nn)
+    g = c.bwd(nn, o, lse, o2)
+    assert all((x == 0).all() for x in (o, o2, *g.values())) and (lse == -math.inf).all()
+    empty = randn((2, 0, 5, 8), 1, TYPES[dtype])
+    nn.rope(empty, torch.arange(5, device="cuda"), nn.rope_freqs(8)[0].cuda(), empty)
+
+
+def test_diff_attention_offsets_past_32_bits(nn):
+    """The last head of a cache whose rows stand 8192 elements apart, 2.4e9 elements in all."""
+    n = 300_000
+    cache = torch.zeros((1, n, 128, 64), dtype=torch.bfloat16, device="cuda")
+    cache[:, :, -4:] = randn((1, n, 4, 64), 3, torch.bfloat16)
+    c = Case(B=1, H=2, K=1, nq=1, nk=n, d=64, dtype="bf16", causal=True)
+    c.k = cache[:, :, -4:-2].transpose(1, 2)
+    c.v = cache[:, :, -2:].reshape(1, n, 1, 128).transpose(1, 2)
+    assert c.k.stride(2) * n > 2 ** 31
+    got = dict(zip(("o", "lse", "o2"), c.fwd(nn)))
+    c.check(got, c.reference(), n)
+
+
+def _everything(nn, dtype, nq, nk):
+    """A layer's operators on fixed tensors: (call, its outputs)."""
+    c = Case(B=3, H=4, K=2, nq=nq, nk=nk, d=64, dtype=dtype, causal=True)
+    freqs = nn.rope_freqs(64)[0].cuda()
+    pos = torch.arange(nq, device="cuda")
+    q = torch.empty_like(c.q)
+    o = torch.empty((3, 4, nq, 128), dtype=c.t, device="cuda")
+    o2, lse = torch.empty_like(o), torch.empty((3, 8, nq), device="cuda")
+    grads = [torch.empty_like(x) for x in (c.q, c.k, c.v, c.lam)]
+    ws = torch.empty(nn.diff_attention_workspace(q, c.k, c.v, backward=True), dtype=torch.uint8, device="cuda")
+
+    def call(stream=None):
+        nn.rope(c.q, pos, freqs, q, stream=stream)
+        nn.diff_attention_fwd(q, c.k, c.v, c.lam, o, lse, LAM_INIT, c.scale, causal=True, o2=o2, workspace=ws, stream=stream)
+        nn.diff_attention_bwd(q, c.k, c.v, c.lam, o, o2, lse, c.do, *grads, LAM_INIT, c.scale, causal=True, workspace=ws,
+                              stream=stream)
+        nn.rope(grads[0], pos, freqs, grads[0], inverse=True, stream=stream)
+    return call, [q, o, o2, lse, *grads]
+
+
+# pairs of CTAs, single ones, the single-token form, f32
+@pytest.mark.parametrize("dtype,nq,nk", [("bf16", 5000, 5000), ("f16", 300, 300), ("bf16", 1, 2000), ("f32", 70, 70)])
+def test_captured_and_on_other_streams(nn, dtype, nq, nk):
+    """An eager run, a captured one replayed twice over cleared outputs, and two
+    runs at once on two streams give the same bits."""
+    call, outs = _everything(nn, dtype, nq, nk)
+    call()
+    torch.cuda.synchronize()
+    want = [x.clone() for x in outs]
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        call()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            call()
+    for _ in range(2):
+        for x in outs:
+            x.fill_(3)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    other, outs2 = _everything(nn, dtype, nq, nk)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        call(s1)
+        other(s2)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) and torch.equal(c, b) for a, b, c in zip(outs, want, outs2))
+    from amcuda import _abi
+    _abi.call("amc_synchronize")      # no wait of the kernels gave up
+
+
+def test_adamw_captured_with_a_rate_on_the_device(nn):
+    """Each replay counts a step and reads the rate anew."""
+    p, g = [randn((1000,), 1, torch.float32)], [randn((1000,), 2, torch.float32)]
+    m, v = [torch.zeros(1000, device="cuda")], [torch.zeros(1000, device="cuda")]
+    state, lr = torch.tensor([0, 0], device="cuda"), torch.tensor([0.5], device="cuda")
+    opt = nn.AdamW(p, g, m, v, state, lr=lr, beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.0)
+    start = p[0].clone()
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        opt.step()
+    assert state.tolist() == [0, 0] and torch.equal(p[0], start)
+    x, mm, vv = start.double(), torch.zeros(1000, device="cuda").double(), torch.zeros(1000, device="cuda").double()
+    for t, rate in ((1, 0.5), (2, 0.25), (3, 0.125)):
+        lr.fill_(rate)
+        graph.replay()
+        torch.cuda.synchronize()
+        x, mm, vv, tol = adamw_ref(x, g[0].double(), mm, vv, t, rate, 0.9, 0.99, 1e-8, 0.0)
+        assert state.tolist() == [t, 0]
+        assert ((p[0] - x).abs() <= t * tol).all()
+
+
+def test_a_layer_trains(nn):
+    """Projections, rotated queries and keys, differential attention and the
+    optimizer as one training step: gradients of every parameter against
+    autograd in 64 bits, then an AdamW step on them."""
+    B, n, H, K, d, width = 2, 75, 4, 2, 16, 48
+    t = torch.float32
+    x, target = randn((B, n, width), 1, t), randn((B, n, H * 2 * d), 2, t)
+    wq, wk, wv = (randn((width, k), 3 + i, t, 0.2) for i, k in enumerate((2 * H * d, 2 * K * d, 2 * K * d)))
+    lam = randn((H, 4, d), 6, t, 0.2)
+    params = [wq, wk, wv, lam]
+    pos = torch.arange(n, device="cuda")
+    freqs, _ = nn.rope_freqs(d)
+    freqs, scale = freqs.cuda(), 1 / math.sqrt(d)
+
+    def heads(y, h):
+        return y.view(B, n, h, -1).transpose(1, 2)
+    q, k, v = (x.view(B * n, width) @ w for w in params[:3])
+    q, k, v = heads(q, 2 * H), heads(k, 2 * K), heads(v, K)
+    nn.rope(q, pos, freqs, q, k, k)
+    o = torch.empty((B, n, H, 2 * d), device="cuda").transpose(1, 2)
+    o2, lse = torch.empty_like(o), torch.empty((B, 2 * H, n), device="cuda")
+    nn.diff_attention_fwd(q, k, v, lam, o, lse, LAM_INIT, scale, causal=True, o2=o2)
+    do = o - heads(target, H)
+    dq, dk, dv, dlam = (torch.empty_like(y) for y in (q, k, v, lam))
+    ws = torch.empty(nn.diff_attention_workspace(q, k, v, backward=True), dtype=torch.uint8, device="cuda")
+    nn.diff_attention_bwd(q, k, v, lam, o, o2, lse, do, dq, dk, dv, dlam, LAM_INIT, scale, causal=True, workspace=ws)
+    nn.rope(dq, pos, freqs, dq, dk, dk, inverse=True)
+    flat = [y.transpose(1, 2).reshape(B * n, -1) for y in (dq, dk, dv)]
+    grads = [x.view(B * n, width).t() @ y for y in flat] + [dlam]
+
+    leaves = [y.double().requires_grad_() for y in params]
+    q, k, v = (x.view(B * n, width).double() @ w for w in leaves[:3])
+    q, k, v = heads(q, 2 * H), heads(k, 2 * K), heads(v, K)
+    ang = pos.double()[:, None] * freqs
+    co, si = ang.cos(), ang.sin()
+
+    def turn(y):
+        a, b = y[..., :d // 2], y[..., d // 2:]
+        return torch.cat([a * co - b * si, b * co + a * si], -1)
+    q, k = turn(q).unflatten(1, (H, 2)), turn(k).unflatten(1, (K, 2)).repeat_interleave(H // K, 1)
+    s = (q @ k.transpose(-1, -2)) * scale
+    p = torch.softmax(s.masked_fill(torch.ones(n, n, device="cuda").triu(1).bool(), -math.inf), -1)
+    l4 = leaves[3]
+    lm = torch.exp((l4[:, 0] * l4[:, 1]).sum(-1)) - torch.exp((l4[:, 2] * l4[:, 3]).sum(-1)) + LAM_INIT
+    out = (p[:, :, 0] - lm[:, None, None] * p[:, :, 1]) @ v.repeat_interleave(H // K, 1)
+    loss = 0.5 * (out - heads(target, H)).square().sum()
+    want = torch.autograd.grad(loss, leaves)
+    for a, b in zip(grads, want):
+        # f32 throughout: sums of at most 150 products of products, each a few
+        # half steps off, and scores below 40 whose exponentials move 2^-16
+        assert (a - b).abs().max() < 2.0 ** -13 * b.abs().max()
+    m, v2 = [torch.zeros_like(y) for y in params], [torch.zeros_like(y) for y in params]
+    state = torch.tensor([0, 0], device="cuda")
+    before = [y.clone() for y in params]
+    nn.AdamW(params, grads, m, v2, state, lr=1e-2, weight_decay=0.0).step()
+    for y, z, g in zip(params, before, grads):
+        # the first step is lr against the gradient's sign, but where |g| is near eps
+        sure = g.abs() > 1e-4
+        assert ((z - y - 1e-2 * g.sign()).abs()[sure] < 1e-5).all()
