@@ -27,27 +27,6 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
-// lam of head h, on every lane; each warp calls it converged.
-template <typename T>
-__device__ __forceinline__ float2 lam_exps(const amc_diff_attention& p, int row) {
-  const T* l = (const T*)p.lam + (size_t)row * 4 * p.d;
-  float a = 0.f, c = 0.f;
-  for (int i = threadIdx.x & 31; i < p.d; i += 32) {
-    a = fmaf(to_f32(l[i]), to_f32(l[p.d + i]), a);
-    c = fmaf(to_f32(l[2 * p.d + i]), to_f32(l[3 * p.d + i]), c);
-  }
-  for (int o = 16; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    c += __shfl_xor_sync(0xffffffffu, c, o);
-  }
-  return make_float2(expf(a), expf(c));
-}
-template <typename T>
-__device__ __forceinline__ float lam_of(const amc_diff_attention& p, int h) {
-  const float2 e = lam_exps<T>(p, p.lam_rows == 1 ? 0 : h);
-  return e.x - e.y + p.lam_init;
-}
-
 // rows r0 .. r0+TT of a (rows, dim) matrix into dst[TT][W], zero outside
 // rows < rows_end and columns < dim.  f32 rows on 16-byte boundaries are
 // copied asynchronously (complete at tile_wait), others converted on the way.
@@ -290,7 +269,10 @@ __global__ void __launch_bounds__(256) k_diff_bwd_rows(const __grid_constant__ a
   const int sub = threadIdx.x % LANES, h = blockIdx.y, b = blockIdx.z;
   const int i = blockIdx.x * kRowsPerCta + threadIdx.x / LANES;
   const float lam = lam_of<T>(p, h);
-  if (blockIdx.x == 0 && b == 0 && threadIdx.x == 0) w.lam[h] = lam;
+  if (blockIdx.x == 0 && b == 0 && threadIdx.x == 0) {
+    w.lam[h] = lam;
+    w.done[h] = 0;
+  }
   const DiffLens len = diff_lens(p, b);
   const bool live = i < p.nq && diff_limit(len, p.causal, i) > 0;
   float d = 0.f, d2 = 0.f;
@@ -527,39 +509,14 @@ __global__ void __launch_bounds__(256, 1) k_diff_dq_simt(const __grid_constant__
     for (int w = 0; w < 8; ++w) t += red[w];
     wk.partials[((int64_t)h * p.batch + b) * gridDim.x + blockIdx.x] = t;
   }
+  diff_dlam_last<T>(p, wk, h, gridDim.x, reinterpret_cast<double*>(diff_sm));
 }
 
-// dlam rows from the partials of sum P_2 G: one CTA per row of lam, a fixed
-// order of summation, in double.
+// dlam where there are no rows: zeros.
 template <typename T>
-__global__ void __launch_bounds__(256) k_diff_dlam(const __grid_constant__ amc_diff_attention p,
-                                                   const float* __restrict__ partials, int64_t per_head) {
-  __shared__ double red[256];
-  const int64_t n = p.lam_rows == 1 ? per_head * p.heads : per_head;
-  const float* x = partials + (int64_t)blockIdx.x * per_head;
-  double t = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 256) t += x[i];
-  red[threadIdx.x] = t;
-  __syncthreads();
-  for (int w = 128; w > 0; w >>= 1) {
-    if (threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
-    __syncthreads();
-  }
-  const float dl = (float)-red[0];
-  const float2 e = lam_exps<T>(p, blockIdx.x);
-  const T* l = (const T*)p.lam + (size_t)blockIdx.x * 4 * p.d;
-  T* o = (T*)p.dlam + (size_t)blockIdx.x * 4 * p.d;
-  for (int i = threadIdx.x; i < p.d; i += 256) {
-    o[i] = from_f32<T>(dl * e.x * to_f32(l[p.d + i]));
-    o[p.d + i] = from_f32<T>(dl * e.x * to_f32(l[i]));
-    o[2 * p.d + i] = from_f32<T>(-dl * e.y * to_f32(l[3 * p.d + i]));
-    o[3 * p.d + i] = from_f32<T>(-dl * e.y * to_f32(l[2 * p.d + i]));
-  }
+__global__ void __launch_bounds__(256) k_diff_no_dlam(const __grid_constant__ amc_diff_attention p) {
+  for (int64_t i = threadIdx.x; i < (int64_t)p.lam_rows * 4 * p.d; i += 256) ((T*)p.dlam)[i] = from_f32<T>(0.f);
 }
-
-namespace {
-
-}  // namespace
 
 int diff_share(const amc_diff_attention& p, int64_t ctas) {
   const int group = p.heads / p.kv_heads;
@@ -608,12 +565,12 @@ int bwd_simt(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s) 
     cfg.numAttrs = share > 1 ? 1 : 0;
     AMC_CUDA(cudaLaunchKernelEx(&cfg, k_diff_dkv_simt<T, TT, DM, DV>, p, w, share));
   }
-  const int tiles = (p.nq + TT - 1) / TT;
   if (p.nq) {
+    const int tiles = (p.nq + TT - 1) / TT;
     k_diff_dq_simt<T, TT, DM, DV><<<dim3(tiles, p.heads, p.batch), 256, L::dq, s>>>(p, w);
     AMC_CUDA(cudaGetLastError());
   }
-  return launch_diff_dlam(p, w, tiles, s);
+  return AMC_OK;
 }
 
 }  // namespace
@@ -647,9 +604,9 @@ int launch_diff_bwd_simt(const amc_diff_attention& p, const DiffBwdWork& w, cuda
   });
 }
 
-int launch_diff_dlam(const amc_diff_attention& p, const DiffBwdWork& w, int tiles, cudaStream_t s) {
+static int launch_no_dlam(const amc_diff_attention& p, cudaStream_t s) {
   return by_type(p.dtype, [&](auto t) {
-    k_diff_dlam<decltype(t)><<<p.lam_rows, 256, 0, s>>>(p, w.partials, (int64_t)p.batch * tiles);
+    k_diff_no_dlam<decltype(t)><<<1, 256, 0, s>>>(p);
     AMC_CUDA(cudaGetLastError());
     return AMC_OK;
   });
@@ -726,7 +683,9 @@ int amc_diff_attention_bwd(const amc_diff_attention* p, void* stream) {
   if (fault_injected("launch")) return fail(AMC_ERR_INJECTED, "diff_attention: injected launch failure (AMC_FAULT=launch)");
   cudaStream_t s = pick_stream(stream);
   const DiffBwdWork w = diff_bwd_work(*p);
-  if (!p->batch) return launch_diff_dlam(*p, w, 0, s);
+  if (!p->batch || !p->nq)
+    if (int rc = launch_no_dlam(*p, s)) return rc;
+  if (!p->batch) return AMC_OK;
   if (int rc = launch_diff_bwd_rows(*p, w, s)) return rc;
   bool handled = false;
   if (int rc = diff_bwd_tc(*p, w, s, &handled)) return rc;

@@ -1,6 +1,7 @@
 // Shared by the differential-attention translation units.
 #pragma once
 
+#include "amc_half.cuh"
 #include "amc_internal.h"
 
 namespace amc {
@@ -33,13 +34,14 @@ __device__ __forceinline__ int diff_first_row(const DiffLens& l, int causal, int
 //          exp2(s + nlse) is 0
 //   nsum = -D_m, D_m = rowsum(dO * O_m)
 // (rows padded to a multiple of 4, so that a tile of them is a bulk copy),
-// then lam of every head, then one partial of sum P_2 G for every (head,
-// batch, row tile).
+// then lam and a counter for every head, then one partial of sum P_2 G for
+// every (head, batch, row tile).
 constexpr int kDiffTile = 32;
 struct DiffBwdWork {
   float4* nlse;
   float4* nsum;
   float* lam;
+  unsigned* done;      // CTAs of this row of lam that have written their partials
   float* partials;
   int pitch;   // rows of a (batch, head)
 };
@@ -51,7 +53,7 @@ inline int diff_row_pitch(const amc_diff_attention& p) { return (p.nq + 3) & ~3;
 inline size_t diff_bwd_bytes(const amc_diff_attention& p) {
   const size_t rows = (size_t)p.batch * p.heads * diff_row_pitch(p);
   const size_t partials = (size_t)p.batch * p.heads * ((p.nq + kDiffTile - 1) / kDiffTile);
-  return rows * sizeof(float4) + (size_t)p.heads * sizeof(float) + partials * sizeof(float);
+  return rows * sizeof(float4) + 2 * (size_t)p.heads * sizeof(float) + partials * sizeof(float);
 }
 inline DiffBwdWork diff_bwd_work(const amc_diff_attention& p) {
   const size_t rows = (size_t)p.batch * p.heads * diff_row_pitch(p);
@@ -59,7 +61,8 @@ inline DiffBwdWork diff_bwd_work(const amc_diff_attention& p) {
   w.nlse = (float4*)p.workspace;
   w.nsum = w.nlse + rows / 2;
   w.lam = (float*)(w.nsum + rows / 2);
-  w.partials = w.lam + p.heads;
+  w.done = (unsigned*)(w.lam + p.heads);
+  w.partials = (float*)(w.done + p.heads);
   w.pitch = diff_row_pitch(p);
   return w;
 }
@@ -80,7 +83,74 @@ int launch_diff_bwd_rows(const amc_diff_attention& p, const DiffBwdWork& w, cuda
 int launch_diff_bwd_simt(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s);
 // Tensor-core gradients (after the rows), likewise.
 int diff_bwd_tc(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s, bool* handled);
-// tiles: partials per (head, batch)
-int launch_diff_dlam(const amc_diff_attention& p, const DiffBwdWork& w, int tiles, cudaStream_t s);
+
+// exp(l0 . l1) and exp(l2 . l3) of row `row` of lam, on every lane of a converged warp.
+template <typename T>
+__device__ __forceinline__ float2 lam_exps(const amc_diff_attention& p, int row) {
+  const T* l = (const T*)p.lam + (size_t)row * 4 * p.d;
+  float a = 0.f, c = 0.f;
+  for (int i = threadIdx.x & 31; i < p.d; i += 32) {
+    a = fmaf(to_f32(l[i]), to_f32(l[p.d + i]), a);
+    c = fmaf(to_f32(l[2 * p.d + i]), to_f32(l[3 * p.d + i]), c);
+  }
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    c += __shfl_xor_sync(0xffffffffu, c, o);
+  }
+  return make_float2(expf(a), expf(c));
+}
+// lam of head h, likewise.
+template <typename T>
+__device__ __forceinline__ float lam_of(const amc_diff_attention& p, int h) {
+  const float2 e = lam_exps<T>(p, p.lam_rows == 1 ? 0 : h);
+  return e.x - e.y + p.lam_init;
+}
+
+// A row of dlam from its partials of sum P_2 G, by the first 256 threads of a
+// CTA that all call it: a fixed order of summation, in double.
+template <typename T>
+__device__ __forceinline__ void diff_dlam_row(const amc_diff_attention& p, const DiffBwdWork& w, int row, int tiles,
+                                              double* red) {
+  const int64_t per_head = (int64_t)p.batch * tiles, n = p.lam_rows == 1 ? per_head * p.heads : per_head;
+  const float* x = w.partials + row * per_head;
+  double t = 0.0;
+  if (threadIdx.x < 256) {
+    for (int64_t i = threadIdx.x; i < n; i += 256) t += __ldcg(x + i);
+    red[threadIdx.x] = t;
+  }
+  __syncthreads();
+  for (int k = 128; k > 0; k >>= 1) {
+    if (threadIdx.x < k) red[threadIdx.x] += red[threadIdx.x + k];
+    __syncthreads();
+  }
+  const float dl = (float)-red[0];
+  const float2 e = lam_exps<T>(p, row);
+  const T* l = (const T*)p.lam + (size_t)row * 4 * p.d;
+  T* o = (T*)p.dlam + (size_t)row * 4 * p.d;
+  for (int i = threadIdx.x; i < p.d; i += blockDim.x) {
+    o[i] = from_f32<T>(dl * e.x * to_f32(l[p.d + i]));
+    o[p.d + i] = from_f32<T>(dl * e.x * to_f32(l[i]));
+    o[2 * p.d + i] = from_f32<T>(-dl * e.y * to_f32(l[3 * p.d + i]));
+    o[3 * p.d + i] = from_f32<T>(-dl * e.y * to_f32(l[2 * p.d + i]));
+  }
+}
+// Called by every dQ CTA of head h after it has written its partial: the last
+// of its row of lam (the rows' kernel zeroed the counter) makes that row of
+// dlam.  `red`: 256 doubles of shared memory.
+template <typename T>
+__device__ __forceinline__ void diff_dlam_last(const amc_diff_attention& p, const DiffBwdWork& w, int h, int tiles,
+                                               double* red) {
+  __shared__ int last;
+  const int row = p.lam_rows == 1 ? 0 : h;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    const unsigned all = (unsigned)((int64_t)p.batch * tiles * (p.lam_rows == 1 ? p.heads : 1));
+    last = atomicAdd(w.done + row, 1u) == all - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  if (last) diff_dlam_row<T>(p, w, row, tiles, red);
+}
 
 }  // namespace amc

@@ -6,14 +6,16 @@
 // Both maps share G, and the difference of the maps is taken before dV's
 // product, so a (row, key) pair costs 16 d + 12 d operations in two kernels
 // against 20 d were dQ added up across CTAs; without atomics the results are
-// the same at every call.
-//   k_diff_dkv_tc  one CTA per 128 keys of a key head; streams 64-row tiles of
+// the same at every call.  One launch holds both kinds of CTA, those of dK/dV
+// first, so that neither waits for the other's last ones:
+//   dkv_cta        one CTA per 128 keys of a key head; streams 64-row tiles of
 //                  every query head that shares it, or, where such CTAs would
 //                  not fill the GPU, one cluster of CTAs that take a share of
 //                  those heads each and add up through distributed shared
 //                  memory, in order of rank;
-//   k_diff_dq_tc   one CTA per 128 rows of a query head; streams 64-key tiles,
-//                  and sums P_2 G (dlam) in f32 on the way.
+//   dq_cta         one CTA per 128 rows of a query head; streams 64-key tiles,
+//                  and sums P_2 G (dlam) in f32 on the way; the last CTA of a
+//                  row of lam adds its partial sums up, in their order.
 // The operands that the threads make (the difference of the maps, dS_1, dS_2)
 // are rounded to the tensors' type and stay in tensor memory, written over
 // the scores they came from; a thread writes only columns it has read.  A
@@ -99,10 +101,9 @@ __device__ __forceinline__ void zero_row(unsigned char* row) {
 // exponentials of tile i+1.  One thread issues everything, so a buffer that
 // an earlier product reads may be the target of a later one.
 template <typename T, int NV>
-__global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
-    const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mK,
-    const __grid_constant__ CUtensorMap mV, const __grid_constant__ CUtensorMap mG,
-    const __grid_constant__ amc_diff_attention p, const __grid_constant__ DiffBwdWork wk, int share) {
+__device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap& mK, const CUtensorMap& mV,
+                                        const CUtensorMap& mG, const amc_diff_attention& p, const DiffBwdWork& wk,
+                                        int share) {
   using L = KvSmem<NV>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ unsigned char diff_sm_raw[];
@@ -158,8 +159,10 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
   if (warp == 16) {
     if (lane == 0 && nt > 0) {
       mbar_expect_tx(kv_full, 32768 + NV / 64 * 16384);
-      for (int m = 0; m < 2; ++m) tma_load_4d(sm + L::k + m * 16384, &mK, 0, k0, 2 * g + m, b, kv_full);
-      for (int c = 0; c < NV / 64; ++c) tma_load_4d(sm + L::v + c * 16384, &mV, 64 * c, k0, g, b, kv_full);
+      for (int r = 0; r < 128; r += 64) {
+        for (int m = 0; m < 2; ++m) tma_load_4d(sm + L::k + m * 16384 + r * 128, &mK, 0, k0 + r, 2 * g + m, b, kv_full);
+        for (int c = 0; c < NV / 64; ++c) tma_load_4d(sm + L::v + c * 16384 + r * 128, &mV, 64 * c, k0 + r, g, b, kv_full);
+      }
       int h = head0, r0 = first;
       for (int i = 0; i < nt; ++i) {
         const int s = i % kStages;
@@ -421,10 +424,9 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dkv_tc(
 // right after the products that read dS(j) from it, while the threads work on
 // tile j+1.
 template <typename T, int NV>
-__global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
-    const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mK,
-    const __grid_constant__ CUtensorMap mV, const __grid_constant__ CUtensorMap mG,
-    const __grid_constant__ amc_diff_attention p, const __grid_constant__ DiffBwdWork wk) {
+__device__ __forceinline__ void dq_cta(const CUtensorMap& mQ, const CUtensorMap& mK, const CUtensorMap& mV,
+                                       const CUtensorMap& mG, const amc_diff_attention& p, const DiffBwdWork& wk,
+                                       int index) {
   using L = QSmem<NV>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ unsigned char diff_sm_raw[];
@@ -440,7 +442,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
   float* red = (float*)(sm + L::bar + 256);  // [16]
   const int tid = threadIdx.x, warp = (int)warp_uniform(tid >> 5), lane = tid & 31;
   const int per = p.heads * p.batch, tiles = (p.nq + 127) / 128;
-  const int tile = tiles - 1 - (int)(blockIdx.x / per), h = blockIdx.x % per % p.heads, b = blockIdx.x % per / p.heads;
+  const int tile = tiles - 1 - index / per, h = index % per % p.heads, b = index % per / p.heads;
   const int g = h / (p.heads / p.kv_heads), r0 = tile * 128;
   const DiffLens len = diff_lens(p, b);
   const int last = min(r0 + 128, len.nq) - 1;
@@ -471,8 +473,10 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
   if (warp == 16) {
     if (lane == 0 && nt > 0) {
       mbar_expect_tx(q_full, 32768 + NV / 64 * 16384);
-      for (int m = 0; m < 2; ++m) tma_load_4d(sm + L::q + m * 16384, &mQ, 0, r0, 2 * h + m, b, q_full);
-      for (int c = 0; c < NV / 64; ++c) tma_load_4d(sm + L::g + c * 16384, &mG, 64 * c, r0, h, b, q_full);
+      for (int r = 0; r < 128; r += 64) {
+        for (int m = 0; m < 2; ++m) tma_load_4d(sm + L::q + m * 16384 + r * 128, &mQ, 0, r0 + r, 2 * h + m, b, q_full);
+        for (int c = 0; c < NV / 64; ++c) tma_load_4d(sm + L::g + c * 16384 + r * 128, &mG, 64 * c, r0 + r, h, b, q_full);
+      }
       for (int j = 0; j < nt; ++j) {
         const int s = j % kStages;
         if (j >= kStages && !mbar_wait(&f_empty[s], (uint32_t)(j / kStages - 1) & 1u)) { *abort_flag = 1; break; }
@@ -622,6 +626,17 @@ __global__ void __launch_bounds__(kThreadsB, 1) k_diff_dq_tc(
     mbar_wait(acc_full, 0, 1 << 14);
   }
   if (warp == 0) tmem_dealloc(tmem, 512);
+  diff_dlam_last<T>(p, wk, h, tiles, reinterpret_cast<double*>(sm));   // all products are done
+}
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(kThreadsB, 1) k_diff_bwd_tc(
+    const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mK,
+    const __grid_constant__ CUtensorMap mV, const __grid_constant__ CUtensorMap mG,
+    const __grid_constant__ amc_diff_attention p, const __grid_constant__ DiffBwdWork wk, int dkv_ctas, int dq_ctas,
+    int share) {
+  if ((int)blockIdx.x < dkv_ctas) dkv_cta<T, NV>(mQ, mK, mV, mG, p, wk, share);
+  else if ((int)blockIdx.x - dkv_ctas < dq_ctas) dq_cta<T, NV>(mQ, mK, mV, mG, p, wk, (int)blockIdx.x - dkv_ctas);
 }
 
 namespace {
@@ -632,29 +647,26 @@ bool aligned_out(const void* x, const int64_t s[3], int64_t heads, int64_t rows,
 }
 
 template <typename T, int NV>
-int bwd_tc(const amc_diff_attention& p, const DiffBwdWork& w, const CUtensorMap (&kv)[4], const CUtensorMap (&q)[4],
-           cudaStream_t s) {
-  static std::atomic<uint64_t> attr_kv{0}, attr_q{0};
-  if (int rc = smem_attr_once(k_diff_dkv_tc<T, NV>, KvSmem<NV>::bytes, attr_kv)) return rc;
-  if (int rc = smem_attr_once(k_diff_dq_tc<T, NV>, QSmem<NV>::bytes, attr_q)) return rc;
-  const unsigned gk = (unsigned)((int64_t)((p.nk + 127) / 128) * p.kv_heads * p.batch);
-  const int tiles = (p.nq + 127) / 128;
-  const int share = diff_share(p, gk);
+int bwd_tc(const amc_diff_attention& p, const DiffBwdWork& w, const CUtensorMap (&map)[4], cudaStream_t s) {
+  static std::atomic<uint64_t> once{0};
+  constexpr int bytes = KvSmem<NV>::bytes > QSmem<NV>::bytes ? KvSmem<NV>::bytes : QSmem<NV>::bytes;
+  if (int rc = smem_attr_once(k_diff_bwd_tc<T, NV>, bytes, once)) return rc;
+  const int64_t units = (int64_t)((p.nk + 127) / 128) * p.kv_heads * p.batch;
+  const int share = diff_share(p, units);
+  const int64_t dq = (int64_t)((p.nq + 127) / 128) * p.heads * p.batch;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(gk * share);
+  cfg.gridDim = dim3((unsigned)(units * share + (dq + share - 1) / share * share));
   cfg.blockDim = dim3(kThreadsB);
-  cfg.dynamicSmemBytes = KvSmem<NV>::bytes;
+  cfg.dynamicSmemBytes = bytes;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {(unsigned)share, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = share > 1 ? 1 : 0;
-  AMC_CUDA(cudaLaunchKernelEx(&cfg, k_diff_dkv_tc<T, NV>, kv[0], kv[1], kv[2], kv[3], p, w, share));
-  const unsigned gq = (unsigned)((int64_t)tiles * p.heads * p.batch);
-  k_diff_dq_tc<T, NV><<<gq, kThreadsB, QSmem<NV>::bytes, s>>>(q[0], q[1], q[2], q[3], p, w);
-  AMC_CUDA(cudaGetLastError());
-  return launch_diff_dlam(p, w, tiles, s);
+  AMC_CUDA(cudaLaunchKernelEx(&cfg, k_diff_bwd_tc<T, NV>, map[0], map[1], map[2], map[3], p, w, (int)(units * share),
+                              (int)dq, share));
+  return AMC_OK;
 }
 
 }  // namespace
@@ -665,25 +677,19 @@ int diff_bwd_tc(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t 
   if (!aligned_out(p.dq, p.dqs, 2 * p.heads, p.nq, p.batch) || !aligned_out(p.dk, p.dks, 2 * p.kv_heads, p.nk, p.batch) ||
       !aligned_out(p.dv_, p.dvs, p.kv_heads, p.nk, p.batch))
     return AMC_OK;
-  if ((int64_t)((p.nq + 127) / 128) * p.heads * p.batch > 0x7fffffff ||
-      (int64_t)((p.nk + 127) / 128) * p.kv_heads * p.batch > 0x7fffffff)
+  if ((int64_t)((p.nq + 127) / 128) * p.heads * p.batch + (int64_t)((p.nk + 127) / 128) * p.kv_heads * p.batch > 0x7ffffff0)
     return AMC_OK;
   const bool bf16 = p.dtype == AMC_BF16;
-  CUtensorMap kv[4], q[4];   // Q, K, V, dO: boxes of 128 rows for the resident side, 64 for the streamed one
-  int rc = AMC_OK;
-  for (int side = 0; side < 2 && !rc; ++side) {
-    CUtensorMap* m = side ? q : kv;
-    const uint32_t rq = side ? 128 : 64, rk = side ? 64 : 128;
-    rc = make_tmap_4d_16(&m[0], p.q, bf16, p.batch, 2 * p.heads, p.nq, p.d, p.qs, rq);
-    if (!rc) rc = make_tmap_4d_16(&m[1], p.k, bf16, p.batch, 2 * p.kv_heads, p.nk, p.d, p.ks, rk);
-    if (!rc) rc = make_tmap_4d_16(&m[2], p.v, bf16, p.batch, p.kv_heads, p.nk, p.dv, p.vs, rk);
-    if (!rc) rc = make_tmap_4d_16(&m[3], p.d_o, bf16, p.batch, p.heads, p.nq, p.dv, p.dos, rq);
-  }
+  CUtensorMap map[4];   // boxes of 64 rows
+  int rc = make_tmap_4d_16(&map[0], p.q, bf16, p.batch, 2 * p.heads, p.nq, p.d, p.qs, 64);
+  if (!rc) rc = make_tmap_4d_16(&map[1], p.k, bf16, p.batch, 2 * p.kv_heads, p.nk, p.d, p.ks, 64);
+  if (!rc) rc = make_tmap_4d_16(&map[2], p.v, bf16, p.batch, p.kv_heads, p.nk, p.dv, p.vs, 64);
+  if (!rc) rc = make_tmap_4d_16(&map[3], p.d_o, bf16, p.batch, p.heads, p.nq, p.dv, p.dos, 64);
   if (rc == AMC_ERR_UNSUPPORTED) return AMC_OK;
   if (rc) return rc;
   *handled = true;
-  if (bf16) return p.dv <= 64 ? bwd_tc<__nv_bfloat16, 64>(p, w, kv, q, s) : bwd_tc<__nv_bfloat16, 128>(p, w, kv, q, s);
-  return p.dv <= 64 ? bwd_tc<__half, 64>(p, w, kv, q, s) : bwd_tc<__half, 128>(p, w, kv, q, s);
+  if (bf16) return p.dv <= 64 ? bwd_tc<__nv_bfloat16, 64>(p, w, map, s) : bwd_tc<__nv_bfloat16, 128>(p, w, map, s);
+  return p.dv <= 64 ? bwd_tc<__half, 64>(p, w, map, s) : bwd_tc<__half, 128>(p, w, map, s);
 }
 
 int diff_bwd_check_error() {

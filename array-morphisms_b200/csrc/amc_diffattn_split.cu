@@ -97,21 +97,6 @@ __device__ __forceinline__ int64_t share_of(int64_t total) {
   return n < kMinShare ? kMinShare : n;
 }
 
-template <typename T>
-__device__ __forceinline__ float lam_of(const amc_diff_attention& p, int h) {
-  const T* l = (const T*)p.lam + (size_t)(p.lam_rows == 1 ? 0 : h) * 4 * p.d;
-  float a = 0.f, c = 0.f;
-  for (int i = threadIdx.x & 31; i < p.d; i += 32) {
-    a = fmaf(to_f32(l[i]), to_f32(l[p.d + i]), a);
-    c = fmaf(to_f32(l[2 * p.d + i]), to_f32(l[3 * p.d + i]), c);
-  }
-  for (int o = 16; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    c += __shfl_xor_sync(0xffffffffu, c, o);
-  }
-  return expf(a) - expf(c) + p.lam_init;
-}
-
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");

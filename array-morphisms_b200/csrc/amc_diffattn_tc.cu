@@ -56,22 +56,6 @@ struct FwdSmem {
 
 __device__ int g_diff_error;
 
-// lam of head h on every lane (the warp is converged).
-template <typename T>
-__device__ __forceinline__ float lam_of(const amc_diff_attention& p, int h) {
-  const T* l = (const T*)p.lam + (size_t)(p.lam_rows == 1 ? 0 : h) * 4 * p.d;
-  float a = 0.f, c = 0.f;
-  for (int i = threadIdx.x & 31; i < p.d; i += 32) {
-    a = fmaf(to_f32(l[i]), to_f32(l[p.d + i]), a);
-    c = fmaf(to_f32(l[2 * p.d + i]), to_f32(l[3 * p.d + i]), c);
-  }
-  for (int o = 16; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    c += __shfl_xor_sync(0xffffffffu, c, o);
-  }
-  return expf(a) - expf(c) + p.lam_init;
-}
-
 }  // namespace
 
 template <typename T, int NV>
