@@ -265,53 +265,63 @@ __global__ void __launch_bounds__(256, 1) k_diff_fwd_simt(const __grid_constant_
 template <typename T, int V, int LANES>
 __global__ void __launch_bounds__(256) k_diff_bwd_rows(const __grid_constant__ amc_diff_attention p,
                                                        const __grid_constant__ DiffBwdWork w) {
-  constexpr int kRowsPerCta = 256 / LANES;
+  constexpr int kAtOnce = 2, kRows = 256 / LANES;   // rows in flight a thread, rows of a CTA at a time
   const int sub = threadIdx.x % LANES, h = blockIdx.y, b = blockIdx.z;
-  const int i = blockIdx.x * kRowsPerCta + threadIdx.x / LANES;
-  const float lam = lam_of<T>(p, h);
+  const int i0 = blockIdx.x * kAtOnce * kRows + threadIdx.x / LANES;
+  const DiffLens len = diff_lens(p, b);
+  float d[kAtOnce] = {}, d2[kAtOnce] = {}, nl1[kAtOnce], nl2[kAtOnce];
+#pragma unroll
+  for (int r = 0; r < kAtOnce; ++r) {
+    const int i = i0 + r * kRows;
+    nl1[r] = nl2[r] = -INFINITY;
+    if (i < p.nq && diff_limit(len, p.causal, i) > 0) {
+      const float* lse = p.lse + ((int64_t)b * 2 * p.heads + 2 * h) * p.nq + i;
+      nl1[r] = -lse[0] * kLog2e;
+      nl2[r] = -lse[p.nq] * kLog2e;
+      const T* o = (const T*)p.o + b * p.os[0] + h * p.os[1] + (int64_t)i * p.os[2];
+      const T* o2 = (const T*)p.o2 + b * p.o2s[0] + h * p.o2s[1] + (int64_t)i * p.o2s[2];
+      const T* go = (const T*)p.d_o + b * p.dos[0] + h * p.dos[1] + (int64_t)i * p.dos[2];
+      for (int c = sub * V; c < p.dv; c += LANES * V) {
+        if constexpr (V == 8) {
+          const uint4 x = *reinterpret_cast<const uint4*>(go + c), y = *reinterpret_cast<const uint4*>(o + c),
+                      z = *reinterpret_cast<const uint4*>(o2 + c);
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 a = unpack2<T>(xs[k]), e = unpack2<T>(ys[k]), f = unpack2<T>(zs[k]);
+            d[r] = fmaf(a.x, e.x, fmaf(a.y, e.y, d[r]));
+            d2[r] = fmaf(a.x, f.x, fmaf(a.y, f.y, d2[r]));
+          }
+        } else {
+          const float x = to_f32(go[c]);
+          d[r] = fmaf(x, to_f32(o[c]), d[r]);
+          d2[r] = fmaf(x, to_f32(o2[c]), d2[r]);
+        }
+      }
+    }
+  }
+  const float lam = lam_of<T>(p, h);   // after the loads, not before them
   if (blockIdx.x == 0 && b == 0 && threadIdx.x == 0) {
     w.lam[h] = lam;
     w.done[h] = 0;
   }
-  const DiffLens len = diff_lens(p, b);
-  const bool live = i < p.nq && diff_limit(len, p.causal, i) > 0;
-  float d = 0.f, d2 = 0.f;
-  if (live) {
-    const T* o = (const T*)p.o + b * p.os[0] + h * p.os[1] + (int64_t)i * p.os[2];
-    const T* o2 = (const T*)p.o2 + b * p.o2s[0] + h * p.o2s[1] + (int64_t)i * p.o2s[2];
-    const T* go = (const T*)p.d_o + b * p.dos[0] + h * p.dos[1] + (int64_t)i * p.dos[2];
-    for (int c = sub * V; c < p.dv; c += LANES * V) {
-      if constexpr (V == 8) {
-        const uint4 x = *reinterpret_cast<const uint4*>(go + c), y = *reinterpret_cast<const uint4*>(o + c),
-                    z = *reinterpret_cast<const uint4*>(o2 + c);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 a = unpack2<T>(xs[k]), e = unpack2<T>(ys[k]), f = unpack2<T>(zs[k]);
-          d = fmaf(a.x, e.x, fmaf(a.y, e.y, d));
-          d2 = fmaf(a.x, f.x, fmaf(a.y, f.y, d2));
-        }
-      } else {
-        const float x = to_f32(go[c]);
-        d = fmaf(x, to_f32(o[c]), d);
-        d2 = fmaf(x, to_f32(o2[c]), d2);
-      }
+  for (int r = 0; r < kAtOnce; ++r) {
+#pragma unroll
+    for (int s = LANES / 2; s > 0; s >>= 1) {
+      d[r] += __shfl_xor_sync(0xffffffffu, d[r], s);
+      d2[r] += __shfl_xor_sync(0xffffffffu, d2[r], s);
     }
-  }
-#pragma unroll
-  for (int s = LANES / 2; s > 0; s >>= 1) {
-    d += __shfl_xor_sync(0xffffffffu, d, s);
-    d2 += __shfl_xor_sync(0xffffffffu, d2, s);
-  }
-  if (sub == 0 && i < w.pitch) {   // the padding too: the gradients multiply it by 0
-    const float* lse = p.lse + ((int64_t)b * 2 * p.heads + 2 * h) * p.nq + i;
-    const int64_t at = ((int64_t)b * p.heads + h) * w.pitch + i;
-    float* e = reinterpret_cast<float*>(w.nlse + at / 2) + (at & 1);
-    float* r = reinterpret_cast<float*>(w.nsum + at / 2) + (at & 1);
-    e[0] = live ? -lse[0] * kLog2e : -INFINITY;
-    e[2] = live ? -lse[p.nq] * kLog2e : -INFINITY;
-    r[0] = -fmaf(lam, d2, d);   // dO . O_1 = dO . (O + lam O_2)
-    r[2] = -d2;
+    const int i = i0 + r * kRows;
+    if (sub == 0 && i < w.pitch) {   // the padding too: the gradients multiply it by 0
+      const int64_t at = ((int64_t)b * p.heads + h) * w.pitch + i;
+      float* e = reinterpret_cast<float*>(w.nlse + at / 2) + (at & 1);
+      float* n = reinterpret_cast<float*>(w.nsum + at / 2) + (at & 1);
+      e[0] = nl1[r];
+      e[2] = nl2[r];
+      n[0] = -fmaf(lam, d2[r], d[r]);   // dO . O_1 = dO . (O + lam O_2)
+      n[2] = -d2[r];
+    }
   }
 }
 
@@ -587,7 +597,7 @@ int launch_diff_bwd_rows(const amc_diff_attention& p, const DiffBwdWork& w, cuda
   bool wide = p.dtype != AMC_F32 && p.dv % 8 == 0 && !(((uintptr_t)p.o | (uintptr_t)p.o2 | (uintptr_t)p.d_o) & 15);
   const int64_t extent[3] = {p.batch, p.heads, p.nq};
   for (int j = 0; j < 3; ++j) wide = wide && (extent[j] == 1 || (p.os[j] % 8 == 0 && p.o2s[j] % 8 == 0 && p.dos[j] % 8 == 0));
-  const dim3 grid16((w.pitch + 15) / 16, p.heads, p.batch), grid8((w.pitch + 7) / 8, p.heads, p.batch);
+  const dim3 grid16((w.pitch + 31) / 32, p.heads, p.batch), grid8((w.pitch + 15) / 16, p.heads, p.batch);
   if (wide && p.dtype == AMC_BF16) k_diff_bwd_rows<__nv_bfloat16, 8, 16><<<grid16, 256, 0, s>>>(p, w);
   else if (wide) k_diff_bwd_rows<__half, 8, 16><<<grid16, 256, 0, s>>>(p, w);
   else if (p.dtype == AMC_F32) k_diff_bwd_rows<float, 1, 32><<<grid8, 256, 0, s>>>(p, w);
