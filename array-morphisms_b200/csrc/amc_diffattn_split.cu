@@ -13,9 +13,13 @@
 // mma.sync m16n8k16: 16 rows fill a legacy tile, where a tcgen05 tile of 128
 // would be an eighth full, and at 16 rows they take less than half the time
 // of the loads.  P is taken into P V as the sum of two 16-bit values (the
-// rounded one and the rounding's remainder), which the loads hide: the result
-// carries no rounding of P.  A second kernel joins the parts of the sequences
-// that several CTAs worked on by their maxima and sums.
+// rounded one and the rounding's remainder): the result carries no rounding of
+// P.  With 8 rows or fewer the two maps share a tile of P, map 1 in its lower
+// half, which takes 48 products a box instead of 80.  A second kernel joins the
+// parts of the sequences that several CTAs worked on by their maxima and sums.
+// Measured, 16 query heads (d 64, dv 128) over 4 key heads, 8 caches of up to
+// 32768 keys (302 MB): 61 us without the join, 4.9 TB/s, with
+// the shared tile, 66 us without; full caches (537 MB): 94 us, 5.7 TB/s.
 #include <cmath>
 #include <type_traits>
 
@@ -132,12 +136,12 @@ __device__ __forceinline__ void put_result(const amc_diff_attention& p, int b, i
 
 }  // namespace
 
-template <typename T, int NV>
+template <typename T, int NV, bool PACK>
 __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constant__ CUtensorMap mK,
                                                            const __grid_constant__ CUtensorMap mV,
                                                            const __grid_constant__ amc_diff_attention p,
                                                            const __grid_constant__ SplitArgs a) {
-  constexpr int NT = NV / 8;
+  constexpr int NT = NV / 8, RR = PACK ? 1 : 2;   // rows of a lane and map
   extern __shared__ unsigned char diff_sm_raw[];
   unsigned char* sm = (unsigned char*)(((uintptr_t)diff_sm_raw + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane >> 2, pos = lane & 3;
@@ -177,9 +181,9 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
   const DiffLens len = diff_lens(p, b);
   const int64_t stop = min(end, unit.first + unit.blocks);
   const int kbeg = (int)(at - unit.first) * 64, kend = min(len.nq > 0 ? len.nk : 0, (int)(stop - unit.first) * 64);
-  int lim[2];     // keys that this lane's two rows see
+  int lim[RR];    // keys that this lane's rows see
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
+  for (int r = 0; r < RR; ++r) {
     const int rr = quad + 8 * r;
     int h, i;
     unit_row(p, a, g, rb * kRows + min(rr, rows - 1), h, i);
@@ -205,6 +209,11 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
+      if (r >= RR) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[m][k][r] = q[m][k][r + 2] = 0u;
+        continue;
+      }
       int h, i;
       unit_row(p, a, g, rb * kRows + min(quad + 8 * r, rows - 1), h, i);
       const T* src = (const T*)p.q + b * p.qs[0] + (2 * h + m) * p.qs[1] + (int64_t)i * p.qs[2];
@@ -218,14 +227,18 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
         }
     }
   const float c2 = p.scale * kLog2e;
-  float top[2][2], sum[2][2], o[2][NT][4];
+  float top[2][RR], sum[2][RR], o[RR][NT][4];   // PACK: one output, map m in registers 2 m, 2 m + 1
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    top[m][0] = top[m][1] = -INFINITY;
-    sum[m][0] = sum[m][1] = 0.f;
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int r = 0; r < RR; ++r) {
+      top[m][r] = -INFINITY;
+      sum[m][r] = 0.f;
+    }
+#pragma unroll
+  for (int m = 0; m < RR; ++m)
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
-  }
   const int mrow = lane & 7, mid = lane >> 3;   // ldmatrix: row and matrix of this lane's address
   bool ok = true;
   for (int n = 0; n < mine; ++n) {
@@ -244,7 +257,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
       fence_proxy_async();
       __syncwarp();
     }
-    uint32_t ph[2][4], pl[2][4];
+    uint32_t ph[RR][4], pl[RR][4];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       float sc[2][4] = {};
@@ -256,17 +269,17 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
         mma16<T>(sc[0], q[m][k], f[0], f[1]);
         mma16<T>(sc[1], q[m][k], f[2], f[3]);
       }
-      if (key + 16 > min(lim[0], lim[1])) {
+      if (key + 16 > min(lim[0], lim[RR - 1])) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < 2 * RR; ++e)
             if (key + 8 * t + 2 * pos + (e & 1) >= lim[e >> 1]) sc[t][e] = -INFINITY;
       }
       bool up = false;
-      float mt[2];
+      float mt[RR];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
+      for (int r = 0; r < RR; ++r) {
         float x = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
@@ -276,29 +289,29 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
       if (__any_sync(0xffffffffu, up)) {
         // raise the maxima that lag by more than 2^8
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < RR; ++r) {
           const bool raise = mt[r] > top[m][r] + 8.f;
           const float corr = raise ? ex2_approx(top[m][r] - mt[r]) : 1.f;
           if (raise) top[m][r] = mt[r];
           sum[m][r] *= corr;
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            o[m][t][2 * r] *= corr;
-            o[m][t][2 * r + 1] *= corr;
+            o[PACK ? 0 : m][t][2 * (PACK ? m : r)] *= corr;
+            o[PACK ? 0 : m][t][2 * (PACK ? m : r) + 1] *= corr;
           }
         }
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < RR; ++r) {
           const float base = top[m][r] == -INFINITY ? 0.f : top[m][r];
           const float p0 = ex2_approx(fmaf(sc[t][2 * r], c2, -base)), p1 = ex2_approx(fmaf(sc[t][2 * r + 1], c2, -base));
           sum[m][r] += p0 + p1;
           const uint32_t hi = pack2<T>(p0, p1);
           const float2 back = unpack2<T>(hi);
-          ph[m][2 * t + r] = hi;
-          pl[m][2 * t + r] = pack2<T>(p0 - back.x, p1 - back.y);
+          ph[PACK ? 0 : m][2 * t + (PACK ? m : r)] = hi;
+          pl[PACK ? 0 : m][2 * t + (PACK ? m : r)] = pack2<T>(p0 - back.x, p1 - back.y);
         }
     }
 #pragma unroll
@@ -307,7 +320,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
       const int chunk = 2 * (t & 3) + (mid >> 1);
       ldsm4_t(f, smem_addr(st + 4096 + (t >> 2) * 2048) + (mrow + (mid & 1) * 8) * 128 + ((chunk ^ mrow) << 4));
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
+      for (int m = 0; m < RR; ++m) {
         mma16<T>(o[m][2 * t], ph[m], f[0], f[1]);
         mma16<T>(o[m][2 * t + 1], ph[m], f[2], f[3]);
         mma16<T>(o[m][2 * t], pl[m], f[0], f[1]);
@@ -332,7 +345,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+    for (int r = 0; r < RR; ++r) {
       float l = sum[m][r];
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -341,7 +354,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
 #pragma unroll
       for (int t = 0; t < NT; ++t)
         *reinterpret_cast<float2*>(xo + ((warp * 2 + m) * kRows + row) * NV + 8 * t + 2 * pos) =
-            make_float2(o[m][t][2 * r], o[m][t][2 * r + 1]);
+            make_float2(o[PACK ? 0 : m][t][2 * (PACK ? m : r)], o[PACK ? 0 : m][t][2 * (PACK ? m : r) + 1]);
     }
   __syncthreads();
   for (int row = warp; row < rows; row += kWarps) {
@@ -475,13 +488,20 @@ SplitArgs plan(const amc_diff_attention& p) {
 
 constexpr size_t kPartRows = (size_t)kShareCtas * 2 * kRows * 2;
 
+template <typename T, int NV, bool PACK>
+int split_main(const amc_diff_attention& p, const SplitArgs& a, const CUtensorMap (&map)[2], cudaStream_t s) {
+  static std::atomic<uint64_t> attr{0};
+  if (int rc = smem_attr_once(k_diff_split<T, NV, PACK>, kSplitSmem, attr)) return rc;
+  const unsigned grid = a.shared ? kShareCtas : (unsigned)((int64_t)p.batch * p.kv_heads * a.row_blocks);
+  k_diff_split<T, NV, PACK><<<grid, kWarps * 32, kSplitSmem, s>>>(map[0], map[1], p, a);
+  AMC_CUDA(cudaGetLastError());
+  return AMC_OK;
+}
+
 template <typename T, int NV>
 int split_launch(const amc_diff_attention& p, const SplitArgs& a, const CUtensorMap (&map)[2], cudaStream_t s) {
-  static std::atomic<uint64_t> attr{0};
-  if (int rc = smem_attr_once(k_diff_split<T, NV>, kSplitSmem, attr)) return rc;
-  const unsigned grid = a.shared ? kShareCtas : (unsigned)((int64_t)p.batch * p.kv_heads * a.row_blocks);
-  k_diff_split<T, NV><<<grid, kWarps * 32, kSplitSmem, s>>>(map[0], map[1], p, a);
-  AMC_CUDA(cudaGetLastError());
+  const bool pack = a.group * p.nq <= 8;
+  if (int rc = pack ? split_main<T, NV, true>(p, a, map, s) : split_main<T, NV, false>(p, a, map, s)) return rc;
   if (a.shared) {
     k_diff_join<T><<<(unsigned)((int64_t)p.batch * p.heads * p.nq), 256, 0, s>>>(p, a);
     AMC_CUDA(cudaGetLastError());
