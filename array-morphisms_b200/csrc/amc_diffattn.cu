@@ -14,6 +14,13 @@
 // tile and TT/16 rows x DV/16 columns of an output.  They run f32 tensors,
 // where a tensor core would round the operands, and the shapes the
 // tensor-core kernels do not take.
+//
+// Bound: the FMA pipe, 128 a clock and SM, and beside it the reads of shared
+// memory: products go by twos (fma.rn.f32x2), which leaves the issue slots to
+// them, and the forward's two maps share each read of V (216 -> 187 us for 4 x 8
+// heads, 512 x 512, d 64; the FMAs alone take 89 us, 103 with 256 CTAs on 148
+// SMs).  16 warps instead of 8, a map each half, gained nothing.  2048 x 2048:
+// 2.46 ms, 58 % of the FMA rate.
 #include <cmath>
 
 #include "amc_diffattn.h"
@@ -59,6 +66,11 @@ __device__ __forceinline__ void tile_wait() {
 // acc[i][j] += sum_c A[ty + 16 i][c] B[tx + 16 j][c]
 template <int R, int PITCH>
 __device__ __forceinline__ void dot_rows(float (&acc)[R][R], const float* A, const float* B, int dim, int ty, int tx) {
+  float2 acc2[R][R];   // sums of even and of odd columns
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < R; ++j) acc2[i][j] = make_float2(acc[i][j], 0.f);
   for (int c = 0; c < dim; c += 4) {
     float4 a[R], b[R];
 #pragma unroll
@@ -69,14 +81,20 @@ __device__ __forceinline__ void dot_rows(float (&acc)[R][R], const float* A, con
     for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int j = 0; j < R; ++j)
-        acc[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, acc[i][j]))));
+        acc2[i][j] = tc::fma2(make_float2(a[i].x, a[i].y), make_float2(b[j].x, b[j].y),
+                              tc::fma2(make_float2(a[i].z, a[i].w), make_float2(b[j].z, b[j].w), acc2[i][j]));
   }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < R; ++j) acc[i][j] = acc2[i][j].x + acc2[i][j].y;
 }
 
 // out[i][4 g + e] += sum_k W(row i, k) X[k][4 tx + 64 g + e].  W is
 // w[row * PW + k] with rows ty + 16 i, or transposed w[k * PW + row] with rows
-// R ty + i: either way one access brings several of its values.
-template <int R, int NC, int TT, int PW, int PX, bool TRANS>
+// R ty + i: either way one access brings several of its values.  The R rows are
+// those of M matrices W, PM values apart, on the same X.
+template <int R, int NC, int TT, int PW, int PX, bool TRANS, int M = 1, int PM = 0>
 __device__ __forceinline__ void mul_rows(float (&out)[R][NC], const float* w, const float* X, int ty, int tx) {
   auto step = [&](const float (&a)[R], int k) {
 #pragma unroll
@@ -84,10 +102,13 @@ __device__ __forceinline__ void mul_rows(float (&out)[R][NC], const float* w, co
       const float4 x = *reinterpret_cast<const float4*>(X + k * PX + 4 * tx + 64 * g);
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        out[i][4 * g] = fmaf(a[i], x.x, out[i][4 * g]);
-        out[i][4 * g + 1] = fmaf(a[i], x.y, out[i][4 * g + 1]);
-        out[i][4 * g + 2] = fmaf(a[i], x.z, out[i][4 * g + 2]);
-        out[i][4 * g + 3] = fmaf(a[i], x.w, out[i][4 * g + 3]);
+        const float2 aa = make_float2(a[i], a[i]);
+        const float2 lo = tc::fma2(aa, make_float2(x.x, x.y), make_float2(out[i][4 * g], out[i][4 * g + 1]));
+        const float2 hi = tc::fma2(aa, make_float2(x.z, x.w), make_float2(out[i][4 * g + 2], out[i][4 * g + 3]));
+        out[i][4 * g] = lo.x;
+        out[i][4 * g + 1] = lo.y;
+        out[i][4 * g + 2] = hi.x;
+        out[i][4 * g + 3] = hi.y;
       }
     }
   };
@@ -109,7 +130,8 @@ __device__ __forceinline__ void mul_rows(float (&out)[R][NC], const float* w, co
     for (int k = 0; k < TT; k += 4) {
       float4 v[R];
 #pragma unroll
-      for (int i = 0; i < R; ++i) v[i] = *reinterpret_cast<const float4*>(w + (ty + 16 * i) * PW + k);
+      for (int i = 0; i < R; ++i)
+        v[i] = *reinterpret_cast<const float4*>(w + i / (R / M) * PM + (ty + 16 * (i % (R / M))) * PW + k);
       float a[R];
 #pragma unroll
       for (int i = 0; i < R; ++i) a[i] = v[i].x;
@@ -129,7 +151,7 @@ __device__ __forceinline__ void mul_rows(float (&out)[R][NC], const float* w, co
 
 // Rows as mul_rows has them.
 template <typename T, int R, int NC, bool TRANS>
-__device__ __forceinline__ void store_rows(T* dst, int64_t stride, const float (&v)[R][NC], float f, int r0, int rows,
+__device__ __forceinline__ void store_rows(T* dst, int64_t stride, const float (*v)[NC], float f, int r0, int rows,
                                            int dim, int ty, int tx) {
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -170,7 +192,7 @@ __global__ void __launch_bounds__(256, 1) k_diff_fwd_simt(const __grid_constant_
     load_tile<T, TT, DM, L::PD>(sQ + m * TT * L::PD, (const T*)p.q + b * p.qs[0] + (2 * h + m) * p.qs[1], p.qs[2], r0,
                                 len.nq, p.d);
   int lim[R];
-  float top[2][R], sum[2][R], o[2][R][DV / 16];
+  float top[2][R], sum[2][R], o[2 * R][DV / 16];   // rows of map m from m R on
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     lim[i] = diff_limit(len, p.causal, r0 + ty + 16 * i);
@@ -179,7 +201,7 @@ __global__ void __launch_bounds__(256, 1) k_diff_fwd_simt(const __grid_constant_
       top[m][i] = -INFINITY;
       sum[m][i] = 0.f;
 #pragma unroll
-      for (int c = 0; c < DV / 16; ++c) o[m][i][c] = 0.f;
+      for (int c = 0; c < DV / 16; ++c) o[m * R + i][c] = 0.f;
     }
   }
   const int last = min(r0 + TT, len.nq) - 1;
@@ -228,13 +250,11 @@ __global__ void __launch_bounds__(256, 1) k_diff_fwd_simt(const __grid_constant_
         sum[m][i] = sum[m][i] * corr + add;
         top[m][i] = mx;
 #pragma unroll
-        for (int c = 0; c < DV / 16; ++c) o[m][i][c] *= corr;
+        for (int c = 0; c < DV / 16; ++c) o[m * R + i][c] *= corr;
       }
     }
     __syncthreads();
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-      mul_rows<R, DV / 16, TT, L::PP, L::PV, false>(o[m], sP + m * TT * L::PP, sV, ty, tx);
+    mul_rows<2 * R, DV / 16, TT, L::PP, L::PV, false, 2, TT * L::PP>(o, sP, sV, ty, tx);
   }
   tile_wait<0>();
 #pragma unroll
@@ -250,12 +270,12 @@ __global__ void __launch_bounds__(256, 1) k_diff_fwd_simt(const __grid_constant_
     }
 #pragma unroll
     for (int c = 0; c < DV / 16; ++c) {
-      o[1][i][c] *= inv[1];
-      o[0][i][c] = fmaf(-lam, o[1][i][c], o[0][i][c] * inv[0]);
+      o[R + i][c] *= inv[1];
+      o[i][c] = fmaf(-lam, o[R + i][c], o[i][c] * inv[0]);
     }
   }
-  store_rows<T, R, DV / 16, false>((T*)p.o + b * p.os[0] + h * p.os[1], p.os[2], o[0], 1.f, r0, p.nq, p.dv, ty, tx);
-  if (p.o2) store_rows<T, R, DV / 16, false>((T*)p.o2 + b * p.o2s[0] + h * p.o2s[1], p.o2s[2], o[1], 1.f, r0, p.nq, p.dv, ty, tx);
+  store_rows<T, R, DV / 16, false>((T*)p.o + b * p.os[0] + h * p.os[1], p.os[2], o, 1.f, r0, p.nq, p.dv, ty, tx);
+  if (p.o2) store_rows<T, R, DV / 16, false>((T*)p.o2 + b * p.o2s[0] + h * p.o2s[1], p.o2s[2], o + R, 1.f, r0, p.nq, p.dv, ty, tx);
 }
 
 // nlse and nsum from lse, o, o2 and dO, and lam of every head.  A row is
