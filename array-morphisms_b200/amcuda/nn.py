@@ -306,7 +306,9 @@ class AdamW:
     done, 0); each step counts it, so a step captured into a CUDA graph goes
     on counting at its replays.  lr is a number, or a float32 tensor of one
     element on the device that is read at every step.  Two steps of the same
-    tensors must not overlap."""
+    tensors must not overlap.  Tensors that are given other memory later
+    (`p.data = ...`) need an AdamW of their own: this one keeps the memory it
+    was made with."""
 
     def __init__(self, params, grads, m, v, state, lr=1e-3, beta1: float = 0.9, beta2: float = 0.999,
                  eps: float = 1e-8, weight_decay: float = 0.01, masters=None, m_scales=None, v_scales=None):
@@ -343,10 +345,14 @@ class AdamW:
                     raise ValueError(f"AdamW: {name}[{i}] does not match its parameter in type, device, layout or size")
             e = table[i]
             e.p, e.n, e.g, e.m, e.v = p.data_ptr(), p.numel(), grads[i].data_ptr(), m[i].data_ptr(), v[i].data_ptr()
-            if p.numel():
-                if p.data_ptr() in seen:
-                    raise ValueError("AdamW: the same parameter twice")
-                seen.add(p.data_ptr())
+            for name, x in (("params", params), *lists.items()):
+                # a master may be its parameter (both f32); nothing else is written twice
+                at = x[i].data_ptr()
+                if name == "grads" or not x[i].numel() or (name == "masters" and at == p.data_ptr()):
+                    continue
+                if at in seen:
+                    raise ValueError(f"AdamW: {name}[{i}] is another tensor of the step as well")
+                seen.add(at)
             if masters is not None:
                 e.master = lists["masters"][i].data_ptr()
             if bits8:
@@ -360,7 +366,8 @@ class AdamW:
         self.state, self._table, self._n = state, table, n
         self._kinds = (_dtype(params[0], "AdamW"), _dtype(grads[0], "AdamW")) if n else (A.F32, A.F32)
         self._kinds += (A.E4M3 if bits8 else A.F32,)
-        self._keep = (params, lists)     # the addresses in the table stay valid
+        # the table's addresses stay valid, even if a tensor is given other memory
+        self._keep = [t.untyped_storage() for x in (params, *lists.values()) for t in x]
 
     def step(self, stream=None) -> None:
         """One update of every tensor; `lr` may be assigned between steps."""

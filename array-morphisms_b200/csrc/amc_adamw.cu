@@ -37,6 +37,7 @@ namespace {
 
 constexpr int kAdamTensors = 256;    // descriptors per launch
 constexpr int kAdamChunk = 2048;     // elements of a CTA's pass: a block a warp
+constexpr int64_t kAdamMost = (int64_t)0x7fffffff * kAdamChunk;
 constexpr int kAdamCtas = 4;         // a SM, at 64 registers a thread
 constexpr int kAdamBlock = 256;      // elements per scale
 constexpr float kE4m3Max = 448.f;
@@ -367,10 +368,14 @@ int amc_adamw(const amc_adamw_tensor* t, int32_t count, int32_t p_dtype, int32_t
     return fail(AMC_ERR_INVALID, "amc_adamw: betas in [0, 1), lr, eps and weight_decay not negative");
   const bool bits8 = state_dtype == AMC_E4M3;
   bool master = false;
+  int64_t all = 0;
   for (int i = 0; i < count && !master; ++i) master = t[i].n > 0 && t[i].master;
   for (int i = 0; i < count; ++i) {
     const amc_adamw_tensor& x = t[i];
     if (x.n < 0) return fail(AMC_ERR_INVALID, "amc_adamw: negative size");
+    // chunks are counted in 32 bits, and no launch is made of a step that fails
+    if (x.n > kAdamMost || (all += x.n / kAdamChunk + 1) > 0x7fffffff)
+      return fail(AMC_ERR_INVALID, "amc_adamw: too many elements");
     if (x.n && (!x.p || !x.g || !x.m || !x.v)) return fail(AMC_ERR_INVALID, "amc_adamw: null tensor");
     if (x.n && (x.master != nullptr) != master) return fail(AMC_ERR_INVALID, "amc_adamw: masters for all tensors or for none");
     if (x.n && bits8 && (!x.m_scale || !x.v_scale)) return fail(AMC_ERR_INVALID, "amc_adamw: 8-bit states need their scales");
@@ -400,7 +405,6 @@ int amc_adamw(const amc_adamw_tensor* t, int32_t count, int32_t p_dtype, int32_t
       a.t[0] = AdamTensor{};
       a.count = 1;
     }
-    if (chunks > 0x7fffffff) return fail(AMC_ERR_INVALID, "amc_adamw: too many elements");
     if (!chunks && !a.last) continue;
     a.chunks = chunks;
     const int64_t most = (int64_t)num_sms() * kAdamCtas;

@@ -22,6 +22,7 @@
 // SMs).  16 warps instead of 8, a map each half, gained nothing.  2048 x 2048:
 // 2.46 ms, 58 % of the FMA rate.
 #include <cmath>
+#include <initializer_list>
 
 #include "amc_diffattn.h"
 #include "amc_half.cuh"
@@ -661,6 +662,16 @@ int check_sizes(const amc_diff_attention* p, const char* who) {
   return AMC_OK;
 }
 
+// No result may be another result or something that is read.
+int check_results(std::initializer_list<const void*> written, std::initializer_list<const void*> read, const char* who) {
+  for (auto w = written.begin(); w != written.end(); ++w) {
+    bool twice = false;
+    for (auto o = written.begin(); o != w; ++o) twice = twice || (*w && *w == *o);
+    for (const void* r : read) twice = twice || (*w && *w == r);
+    if (twice) return fail(AMC_ERR_INVALID, std::string(who) + ": a result lies on another tensor of the call");
+  }
+  return AMC_OK;
+}
 
 int check_workspace(const amc_diff_attention* p, size_t need, const char* who) {
   if (!need) return AMC_OK;
@@ -694,6 +705,9 @@ int amc_diff_attention_fwd(const amc_diff_attention* p, void* stream) {
     return fail(AMC_ERR_INVALID, "amc_diff_attention_fwd: null tensor");
   if (int rc = check_workspace(p, diff_split_bytes(*p), "amc_diff_attention_fwd")) return rc;
   if (fault_injected("launch")) return fail(AMC_ERR_INJECTED, "diff_attention: injected launch failure (AMC_FAULT=launch)");
+  if (int rc = check_results({p->o, p->o2, p->lse}, {p->q, p->nk ? p->k : nullptr, p->nk ? p->v : nullptr, p->lam},
+                             "amc_diff_attention_fwd"))
+    return rc;
   cudaStream_t s = pick_stream(stream);
   bool handled = false;
   if (int rc = diff_fwd_split(*p, s, &handled)) return rc;
@@ -711,6 +725,10 @@ int amc_diff_attention_bwd(const amc_diff_attention* p, void* stream) {
     return fail(AMC_ERR_INVALID, "amc_diff_attention_bwd: null tensor");
   if (int rc = check_workspace(p, diff_bwd_bytes(*p), "amc_diff_attention_bwd")) return rc;
   if (fault_injected("launch")) return fail(AMC_ERR_INJECTED, "diff_attention: injected launch failure (AMC_FAULT=launch)");
+  if (p->batch && p->nq && p->nk)
+    if (int rc = check_results({p->dq, p->dk, p->dv_, p->dlam},
+                               {p->q, p->k, p->v, p->lam, p->o, p->o2, p->lse, p->d_o}, "amc_diff_attention_bwd"))
+      return rc;
   cudaStream_t s = pick_stream(stream);
   const DiffBwdWork w = diff_bwd_work(*p);
   if (!p->batch || !p->nq)

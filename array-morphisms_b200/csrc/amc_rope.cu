@@ -227,6 +227,9 @@ int amc_rope(const amc_rope_tensor* t, int32_t count, int32_t dtype, int64_t bat
       for (int j = 0; j < 3; ++j)
         if (t[k].xs[j] != t[k].os[j]) return fail(AMC_ERR_INVALID, "amc_rope: in place needs the same strides");
   }
+  if (count == 2 && t[0].heads && t[1].heads &&
+      (t[0].out == t[1].out || t[0].out == t[1].x || t[1].out == t[0].x))
+    return fail(AMC_ERR_INVALID, "amc_rope: the tensors' results must not lie on one another's");
   if (!pos || !freqs) return fail(AMC_ERR_INVALID, "amc_rope: null positions or frequencies");
   if (n > ((int64_t)1 << 40) / batch) return fail(AMC_ERR_INVALID, "amc_rope: too many rows");
   if (fault_injected("launch")) return fail(AMC_ERR_INJECTED, "rope: injected launch failure (AMC_FAULT=launch)");

@@ -386,7 +386,7 @@ int amc_conv2d_wgrad_f32(const float* X, const float* dY, float* dW, int32_t N, 
  * elements (i, i + rot/2), or (2i, 2i + 1) when interleaved; elements from
  * rot on are copied.  inverse != 0 turns back, which is the gradient.  One or
  * two tensors (queries and keys) of one batch, n, d and dtype in one launch;
- * out may be x itself, with the same strides.  pos is s64, element (b, i) at
+ * out may be x itself, with the same strides, but not the other's.  pos is s64, element (b, i) at
  * pos[b * pos_stride + i]; freqs rot/2 doubles on the device; rot up to 1024. */
 typedef struct amc_rope_tensor {
   const void* x;

@@ -456,6 +456,53 @@ def test_adamw_more_tensors_than_one_launch_holds(nn):
 
 
 # ---------------------------------------------------------------------------- how calls are made
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("B,H,K,nq,nk", [(3, 4, 2, 1, 3000), (3, 12, 1, 1, 700), (300, 2, 2, 1, 300), (2, 2, 1, 7, 137),
+                                         (10, 16, 4, 130, 257), (6, 4, 2, 300, 333)])
+def test_diff_attention_over_caches_that_are_not_filled(nn, dtype, B, H, K, nq, nk):
+    """Keys and rows behind the lengths hold NaN and infinities, in every form
+    of the forward (the single-token one with 8 rows or fewer and with more, CTA
+    pairs, single CTAs, f32): the result is that of zeros there."""
+    kv = [nk - (37 * i + 16) % nk for i in range(B)]
+    ql = [max(nq - 5 * i, 0) if nq > 1 else 1 for i in range(B)]
+    make = lambda: Case(B=B, H=H, K=K, nq=nq, nk=nk, d=64, dtype=dtype, causal=True, q_lens=ql, kv_lens=kv)
+    c, e = make(), make()
+    for i in range(B):
+        c.k[i, :, kv[i]:], c.v[i, :, kv[i]:], c.q[i, :, ql[i]:] = 0, 0, 0
+        e.k[i, :, kv[i]:], e.v[i, :, kv[i]:], e.q[i, :, ql[i]:] = math.nan, math.inf if i % 2 else math.nan, math.nan
+    assert all(torch.equal(x, y) for x, y in zip(c.fwd(nn), e.fwd(nn)))
+
+
+def test_single_tokens_one_after_another_in_one_workspace(nn):
+    """The joining kernel of a step, launched early, and the first kernel of the
+    next share a workspace: each step's result is its own, also in a graph."""
+    cases = [Case(B=8, H=16, K=4, nq=1, nk=9000, d=64, dtype="bf16", seed=10 * s, kv_lens=[9000 - 1000 * i for i in range(8)])
+             for s in range(3)]
+    want = [c.fwd(nn)[0] for c in cases]
+    outs = [[torch.empty_like(want[0]) for _ in cases] for _ in range(20)]
+    c = cases[0]
+    ws = torch.empty(nn.diff_attention_workspace(c.q, c.k, c.v), dtype=torch.uint8, device="cuda")
+    assert ws.numel()
+
+    def steps(outs, stream=None):
+        for row in outs:
+            for c, o in zip(cases, row):
+                nn.diff_attention_fwd(c.q, c.k, c.v, c.lam, o, None, LAM_INIT, c.scale, kv_lens=c.kv_lens, workspace=ws,
+                                      stream=stream)
+    steps(outs)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for row in outs for o, w in zip(row, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        steps(outs)
+    for row in outs:
+        for o in row:
+            o.fill_(3)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for row in outs for o, w in zip(row, want))
+
+
 def test_diff_attention_alignments_and_strides_other_than_the_kernels_like(nn):
     """Rows off 16 bytes, keys broadcast over the batch, a negative scale."""
     c = Case(B=2, H=2, K=1, nq=70, nk=90, d=64, dtype="bf16", causal=True)

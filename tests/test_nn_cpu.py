@@ -231,3 +231,68 @@ for f in (T.c_rope, T.c_diff, T.c_adamw):
     out = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, AMC_FAULT="launch"), capture_output=True,
                          text=True, timeout=120)
     assert out.returncode == 0, out.stderr
+
+
+def test_c_rope_refuses_results_on_the_other_tensor():
+    def call(x0, o0, x1, o1, heads1=1):
+        t = (A.RopeTensor * 2)()
+        (t[0].x, t[0].out, t[0].heads), (t[1].x, t[1].out, t[1].heads) = (x0, o0, 1), (x1, o1, heads1)
+        return A.load().amc_rope(C.cast(t, C.c_void_p), 2, A.F32, 1, 1, 8, 8, None, 0, 16, 1.0, 0, 0, None)
+    for bad in ((16, 32, 48, 32), (16, 48, 48, 64), (16, 32, 48, 16)):
+        assert call(*bad) == 1 and "on one another" in A.last_error()
+    # separate ones, two turns of one tensor, and an empty second pass this check and meet the next
+    for fine in ((16, 16, 48, 48), (16, 32, 16, 48), (16, 32, 48, 32, 0)):
+        assert call(*fine) == 1 and "null positions" in A.last_error()
+
+
+def c_diff_apart(entry, **change):
+    """A call with every tensor in a place of its own (addresses only) but for the changes; it never reaches a launch."""
+    p = A.DiffAttention(dtype=A.F32, batch=1, heads=2, kv_heads=1, nq=3, nk=5, d=8, dv=8, lam_rows=1, scale=1.0)
+    p.workspace, p.workspace_bytes = 4096 * 30, 1 << 30
+    for i, name in enumerate(("q", "k", "v", "lam", "o", "o2", "d_o", "dq", "dk", "dv_", "dlam")):
+        setattr(p, name, 4096 * (i + 1))
+    p.lse = 4096 * 20
+    for k, v in change.items():
+        setattr(p, k, v)
+    rc = getattr(A.load(), entry)(C.byref(p), None)
+    return rc, A.last_error()
+
+
+@pytest.mark.parametrize("entry,change", [
+    ("amc_diff_attention_fwd", {"o": 4096}), ("amc_diff_attention_fwd", {"o2": 4096 * 5}),
+    ("amc_diff_attention_fwd", {"o2": 4096 * 3}), ("amc_diff_attention_fwd", {"lse": 4096 * 5}),
+    ("amc_diff_attention_bwd", {"dq": 4096}), ("amc_diff_attention_bwd", {"dk": 4096 * 8}),
+    ("amc_diff_attention_bwd", {"dv_": 4096 * 7}), ("amc_diff_attention_bwd", {"dlam": 4096 * 4}),
+    ("amc_diff_attention_bwd", {"dq": 4096 * 20}),
+])
+def test_c_diff_attention_refuses_results_on_other_tensors(entry, change):
+    rc, text = c_diff_apart(entry, **change)
+    assert rc == 1 and "lies on another tensor" in text
+
+
+def test_adamw_refuses_a_tensor_in_two_places():
+    z = torch.zeros(300)
+    for change in ({"m": [z, torch.zeros(300)], "v": [z, torch.zeros(300)]}, {"v": [z, z]},
+                   {"masters": [z, z]}, {"params": [z, torch.zeros(300)], "m": [torch.zeros(300), z]}):
+        with pytest.raises(ValueError, match="as well"):
+            nn.AdamW(**adamw_args(**change))
+    p = [torch.zeros(300), torch.zeros(300)]
+    nn.AdamW(**adamw_args(params=p, masters=p))
+    nn.AdamW(**adamw_args(grads=[z, z]))
+    e = torch.zeros(0)
+    nn.AdamW(params=[e, e], grads=[e, e], m=[e, e], v=[e, e], state=torch.zeros(2, dtype=torch.int64))
+
+
+def test_adamw_keeps_the_memory_it_was_made_with():
+    a = adamw_args()
+    opt = nn.AdamW(**a)
+    at = a["params"][0].data_ptr()
+    a["params"][0].data = torch.zeros(300)
+    assert opt._table[0].p == at and any(s.data_ptr() == at for s in opt._keep)
+
+
+def test_c_adamw_refuses_more_than_it_can_count():
+    assert c_adamw(n=1 << 45) == 1
+    assert "too many" in A.last_error()
+    assert c_adamw(count=2, n=(1 << 42) - (1 << 12)) == 1
+    assert "too many" in A.last_error()
