@@ -9,6 +9,8 @@
 // loaded before the angles are formed.  The turn count is formed and reduced to
 // half a turn in f64 (a position of 2^40 keeps its angle), its sine and cosine
 // in f32.  No table is read.
+// Measured: queries and keys of 16 x 2048 tokens, 16 heads each, d 64, bf16
+// (268 MB): 48 us, 5.6 TB/s; 16 tokens: 5 us, of which the launch is most.
 #include <cmath>
 
 #include "amc_half.cuh"
