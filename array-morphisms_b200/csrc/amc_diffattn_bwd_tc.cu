@@ -98,15 +98,17 @@ __device__ __forceinline__ void zero_row(unsigned char* row) {
 }  // namespace
 
 // ------------------------------------------------------------------ dK, dV
-// Tensor memory: four 64-column buffers in two pairs, dV at 256, dK_1, dK_2 at
-// 384 and 448.  Tile i has S_1, S_2 in pair X = i & 1 and G in the first
-// buffer of the other pair Y.  The threads take the exponentials of S(i) as
-// soon as S(i) is there, then read G(i); that frees Y's first buffer (Y's
-// second held dS_2(i-1), whose product was issued before), so S(i+1) goes to
-// Y while the threads write the operands of tile i over X; their products and
-// then G(i+1), into X's first buffer, run while the threads take the
-// exponentials of tile i+1.  One thread issues everything, so a buffer that
-// an earlier product reads may be the target of a later one.
+// Tensor memory: four 64-column buffers, dV at 256, dK_1, dK_2 at 384 and 448.
+// Even tiles have S_1, S_2 and G in buffers 0, 1 and 2, odd ones in 3, 2 and 1.
+// The threads write W = P_1 - lam P_2 and dS_1 over S_1, dS_2 over S_2, so
+//   S_1(i+2) follows the products of W and dS_1(i), which leave its buffer,
+//   S_2(i+1) takes the place of G(i) once the threads have read that, and
+//   G(i+1) that of dS_2(i), whose product is the first of its tile:
+// the scores of the next tile are there when a warp is done with this one, and
+// G after the exponentials.  (With both scores issued when G had been read, the
+// warps waited 450 to 900 clocks a tile for them: 2800 a tile.)  One thread
+// issues everything, so a buffer that an earlier product reads may be the target
+// of a later one.
 template <typename T, int NV>
 __device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap& mK, const CUtensorMap& mV,
                                         const CUtensorMap& mG, const amc_diff_attention& p, const DiffBwdWork& wk,
@@ -118,11 +120,12 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap
   uint64_t* kv_full = (uint64_t*)(sm + L::bar);
   uint64_t* f_full = kv_full + 1;            // [kStages] Q, dO and row pairs landed
   uint64_t* f_empty = f_full + kStages;      // [kStages] their products are done and the pairs read
-  uint64_t* s_full = f_empty + kStages;      // S(i) complete
-  uint64_t* g_full = s_full + 1;             // G(i) complete
-  uint64_t* g_read = s_full + 2;             // the threads have read G(i) (16 warps)
-  uint64_t* p_full = s_full + 3;             // operands of tile i written (16 warps)
-  uint64_t* acc_full = s_full + 4;
+  uint64_t* s1_full = f_empty + kStages;     // [2] S_1(i) complete, even and odd i
+  uint64_t* s2_full = s1_full + 2;           // S_2(i) complete
+  uint64_t* g_full = s1_full + 3;            // G(i) complete
+  uint64_t* g_read = s1_full + 4;            // the threads have read G(i) (16 warps)
+  uint64_t* p_full = s1_full + 5;            // operands of tile i written (16 warps)
+  uint64_t* acc_full = s1_full + 6;
   uint32_t* tslot = (uint32_t*)(sm + L::bar + 192);
   volatile int* abort_flag = (volatile int*)(sm + L::bar + 196);
   const int tid = threadIdx.x, warp = (int)warp_uniform(tid >> 5), lane = tid & 31;
@@ -146,7 +149,7 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap
       mbar_init(&f_full[i], 1);
       mbar_init(&f_empty[i], 1 + kRowWarps);
     }
-    mbar_init(s_full, 1);
+    for (int i = 0; i < 3; ++i) mbar_init(&s1_full[i], 1);
     mbar_init(g_full, 1);
     mbar_init(g_read, kRowWarps);
     mbar_init(p_full, kRowWarps);
@@ -197,63 +200,65 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap
       const uint32_t id_dv = idesc_f16(128, NV, kBf16, false, true);
       const uint64_t kd = sdesc(smem_addr(sm + L::k), 16, 1024), vd = sdesc(smem_addr(sm + L::v), 16, 1024);
       const uint64_t fd = sdesc(smem_addr(sm + L::f), 16, 1024), fmn = sdesc_mn16(smem_addr(sm + L::f), 8192);
-      auto issue_s = [&](int i) {
-        const uint64_t st = desc_add(fd, (i % kStages) * L::stage);
+      auto issue_s = [&](int i, int m) {
+        const uint64_t st = desc_add(fd, (i % kStages) * L::stage + m * 8192);
+        const uint32_t to = tmem + 64 * (m ? 1 + (i & 1) : 3 * (i & 1));
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_f16(tmem + (i & 1) * 128 + m * 64, desc_add(kd, m * 16384 + k * 32), desc_add(st, m * 8192 + k * 32), id,
-                    k > 0);
-        mma_commit_warp(s_full);
+        for (int k = 0; k < 4; ++k)
+          mma_f16(to, desc_add(kd, m * 16384 + k * 32), desc_add(st, k * 32), id, k > 0);
+        mma_commit_warp(m ? s2_full : &s1_full[i & 1]);
       };
       auto issue_g = [&](int i) {
         const uint64_t st = desc_add(fd, (i % kStages) * L::stage + 16384);
 #pragma unroll
         for (int k = 0; k < NV / 16; ++k)
-          mma_f16(tmem + (~i & 1) * 128, desc_add(vd, (k >> 2) * 16384 + (k & 3) * 32),
+          mma_f16(tmem + 64 * (2 - (i & 1)), desc_add(vd, (k >> 2) * 16384 + (k & 3) * 32),
                   desc_add(st, (k >> 2) * 8192 + (k & 3) * 32), id, k > 0);
         mma_commit_warp(g_full);
       };
       // A operands: warpgroup k wrote rows 16 k .. 16 k + 15 of the tile (K
       // step k) at columns 16 k (+8 for dS_1) of the buffers
+      auto issue_dk2 = [&](int i) {
+        const uint64_t st = desc_add(fmn, (i % kStages) * L::stage + 8192);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_f16_ts(t_dk + 64, tmem + 64 * (1 + (i & 1)) + k * 16, desc_add(st, k * 2048), id_dk, i > 0 || k > 0);
+      };
       auto issue_acc = [&](int i) {
         const uint64_t st = desc_add(fmn, (i % kStages) * L::stage);
-        const uint32_t x = tmem + (i & 1) * 128;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t a = x + k * 16;
+          const uint32_t a = tmem + 192 * (i & 1) + k * 16;
           mma_f16_ts(t_dv, a, desc_add(st, 16384 + k * 2048), id_dv, i > 0 || k > 0);
           mma_f16_ts(t_dk, a + 8, desc_add(st, k * 2048), id_dk, i > 0 || k > 0);
         }
-      };
-      auto issue_acc2 = [&](int i) {
-        const uint64_t st = desc_add(fmn, (i % kStages) * L::stage);
-        const uint32_t x = tmem + (i & 1) * 128;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          mma_f16_ts(t_dk + 64, x + 64 + k * 16, desc_add(st, 8192 + k * 2048), id_dk, i > 0 || k > 0);
         mma_commit_warp(&f_empty[i % kStages]);
       };
-      bool ok = warp_wait(kv_full, 0) && warp_wait(&f_full[0], 0);
+      auto landed = [&](int i) { return warp_wait(&f_full[i % kStages], (uint32_t)(i / kStages) & 1u); };
+      bool ok = warp_wait(kv_full, 0) && landed(0);
       if (ok) {
         tc_fence_after();
-        issue_s(0);
+        issue_s(0, 0);
+        issue_s(0, 1);
         issue_g(0);
+        if (nt > 1 && (ok = landed(1))) issue_s(1, 0);
       }
       for (int i = 0; i < nt && ok; ++i) {
         const bool more = i + 1 < nt;
         if (more) {
-          if (!warp_wait(&f_full[(i + 1) % kStages], (uint32_t)((i + 1) / kStages) & 1u) ||
-              !warp_wait(g_read, (uint32_t)i & 1u)) { ok = false; break; }
+          if (!warp_wait(g_read, (uint32_t)i & 1u)) { ok = false; break; }
           tc_fence_after();
-          issue_s(i + 1);
+          issue_s(i + 1, 1);
         }
         if (!warp_wait(p_full, (uint32_t)i & 1u) || warp_uniform(*abort_flag)) { ok = false; break; }
         tc_fence_after();
+        issue_dk2(i);
+        if (more) issue_g(i + 1);
         issue_acc(i);
-        if (more) issue_g(i + 1);   // into the buffer that dV and dK_1 have read; dK_2 reads the other
-        issue_acc2(i);
+        if (i + 2 < nt) {
+          if (!landed(i + 2)) { ok = false; break; }
+          issue_s(i + 2, 0);
+        }
       }
       if (ok) mma_commit_warp(acc_full);
       else *abort_flag = 1;
@@ -272,28 +277,35 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap
     if (nt > 0) ok = __all_sync(0xffffffffu, mbar_wait(&f_full[0], 0));
     for (int i = 0; i < nt && ok; ++i) {
       const int s = i % kStages;
-      const uint32_t x = tmem + (i & 1) * 128 + lane_base + 16 * w;
+      const uint32_t x = tmem + lane_base + 16 * w;
+      const uint32_t x1 = x + 192 * (i & 1), x2 = x + 64 * (1 + (i & 1)), xg = x + 64 * (2 - (i & 1));
       // The row pairs come from shared memory, whose port the products'
       // operands keep busy: they are read before each wait, not after it.
       const float4* le = reinterpret_cast<const float4*>(sm + L::r + s * 1024 + 128 * w);
       float4 rp[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) rp[j] = le[j];
-      ok = __all_sync(0xffffffffu, mbar_wait(s_full, (uint32_t)i & 1u));
+      ok = __all_sync(0xffffffffu, mbar_wait(&s1_full[i & 1], (uint32_t)(i >> 1) & 1u));
       if (!ok) break;
       tc_fence_after();
-      uint32_t s1[16], s2[16];
-      tmem_ld16_nowait(x, s1);
-      tmem_ld16_nowait(x + 64, s2);
-      tmem_ld_wait();
       // P_1 and -lam P_2, two rows at a time
+      uint32_t sc[16];
       float2 p1[8], p2[8];
+      tmem_ld16_nowait(x1, sc);
+      tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float4 e = rp[j];
-        const float2 a = fma2(make_float2(__uint_as_float(s1[2 * j]), __uint_as_float(s1[2 * j + 1])), cc, make_float2(e.x, e.y));
-        const float2 c = fma2(make_float2(__uint_as_float(s2[2 * j]), __uint_as_float(s2[2 * j + 1])), cc, make_float2(e.z, e.w));
+        const float2 a = fma2(make_float2(__uint_as_float(sc[2 * j]), __uint_as_float(sc[2 * j + 1])), cc, make_float2(rp[j].x, rp[j].y));
         p1[j] = make_float2(ex2_approx(a.x), ex2_approx(a.y));
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(s2_full, (uint32_t)i & 1u));
+      if (!ok) break;
+      tc_fence_after();
+      tmem_ld16_nowait(x2, sc);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 c = fma2(make_float2(__uint_as_float(sc[2 * j]), __uint_as_float(sc[2 * j + 1])), cc, make_float2(rp[j].z, rp[j].w));
         p2[j] = mul2(make_float2(ex2_approx(c.x), ex2_approx(c.y)), make_float2(nlam, nlam));
       }
       const bool masked = r0 < fr_all || r0 + 64 > len.nq;
@@ -314,7 +326,7 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap
       if (!ok) break;
       tc_fence_after();
       uint32_t gv[16];
-      tmem_ld16_nowait(tmem + (~i & 1) * 128 + lane_base + 16 * w, gv);
+      tmem_ld16_nowait(xg, gv);
       tmem_ld_wait();
       tc_fence_before();
       warp_arrive(g_read);
@@ -342,9 +354,9 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap
         v1[j] = __uint_as_float(pack2<T>(a.x, a.y));
         v2[j] = __uint_as_float(pack2<T>(c.x, c.y));
       }
-      tmem_st8(x, v);
-      tmem_st8(x + 8, v1);
-      tmem_st8(x + 64, v2);
+      tmem_st8(x1, v);
+      tmem_st8(x1 + 8, v1);
+      tmem_st8(x2, v2);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(p_full);
@@ -395,7 +407,7 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap
     // bounded drain of copies and products still in flight
     mbar_wait(kv_full, 0, 1 << 14);
     for (int i = 0; i < kStages; ++i) mbar_wait(&f_full[i], 0, 1 << 14);
-    mbar_wait(s_full, 0, 1 << 14);
+    for (int i = 0; i < 3; ++i) mbar_wait(&s1_full[i], 0, 1 << 14);
     mbar_wait(g_full, 0, 1 << 14);
     mbar_wait(acc_full, 0, 1 << 14);
     __syncthreads();
