@@ -24,13 +24,15 @@
 // products.  Four warpgroups share a tile, 16 of its 64 columns each: with two
 // of them, 32 columns a thread, the two warps of a scheduler could not cover
 // each other's latencies.
-// Measured, 8 heads x 16 sequences, 2048 x 2048, d 64, no mask: 1280 us after a
-// row pass of 50 us (687 GFLOP counted as 20 d a pair: 537 TFLOP/s).  dkv_cta
-// takes 2800 clocks for a 128 x 64 tile, dq_cta 1750; at the rates of
-// either alone its products need 1370 and 1110 of them, its exponentials 1024.
-// The rest is the chain from scores through exponentials and G to the operands:
-// tensor memory, full with one tile in work and the sums, has no room for a
-// second.
+// Measured, 8 heads x 16 sequences, 2048 x 2048, d 64, no mask: 1150 us after a
+// row pass of 50 us (687 GFLOP counted as 20 d a pair: 600 TFLOP/s).  dkv_cta
+// takes 2300 clocks for a 128 x 64 tile, dq_cta 1600; at the rates of either
+// alone its products need 1370 and 1110 of them, its exponentials 1024.  The
+// rest are the chain from scores through exponentials and G to the operands and
+// the round trips at its barriers (200 to 300 clocks each beside the operands of
+// the products).  Testing two barriers in one trip, reading the row pairs a tile
+// ahead, one wait for both scores, and G of dq_cta behind a barrier of its own
+// gained nothing.
 // Every wait is bounded; on expiry the kernel records AMC_ERR_TIMEOUT, drains
 // and returns.
 #include <cmath>
@@ -106,7 +108,7 @@ __device__ __forceinline__ void zero_row(unsigned char* row) {
 //   G(i+1) that of dS_2(i), whose product is the first of its tile:
 // the scores of the next tile are there when a warp is done with this one, and
 // G after the exponentials.  (With both scores issued when G had been read, the
-// warps waited 450 to 900 clocks a tile for them: 2800 a tile.)  One thread
+// warps waited 450 to 900 clocks a tile for them: 2800 a tile, now 2300.)  One thread
 // issues everything, so a buffer that an earlier product reads may be the target
 // of a later one.
 template <typename T, int NV>
