@@ -354,6 +354,9 @@ __global__ void __launch_bounds__(kThreadsF, 1) k_diff_fwd_tc(const __grid_const
 // (scores ready, P written), a tile one for all its loads, and P V of the step
 // before needs none of its own: the scores after next follow it on the pipe,
 // and their barrier is committed even where there is no such step.
+// What the odd CTA's shared memory holds (loaded tiles, cleared rows of V) is
+// released and acquired at cluster scope; that costs nothing measurable (507 us
+// with and without it, 16 heads x 4 sequences, 4096 x 4096, causal).
 // Measured, causal, 16 heads x 4 sequences, 4096 x 4096, d 64: 470 to 515 us with
 // the GPU's power limit (412 GFLOP: 800 to 876 TFLOP/s); 8 x 16, 2048 x 2048
 // without a mask: 440 to 490 us.  A step takes 1577 clocks, of which the tensor
@@ -393,6 +396,11 @@ __device__ __forceinline__ PairItem pair_item(const amc_diff_attention& p, int w
   t.nt = (t.kend + 127) / 128;
   t.ns = (t.kend + 63) / 64;
   return t;
+}
+// Whether step j of an item reaches behind its sequence's keys, so that the
+// softmax warps clear rows of V: only the last step of a padded sequence.
+__device__ __forceinline__ bool clears_v(const PairItem& t, const amc_diff_attention& p, int j) {
+  return j * 64 + 64 > t.len.nk && t.len.nk < p.nk;
 }
 
 }  // namespace
@@ -487,11 +495,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsF, 1)
         const PairItem t = pair_item(p, w);
         if (!t.ns) continue;
         ok = mbar_wait(q_full, (uint32_t)it & 1u);
-        if (ok) mbar_arrive_at(q_ready, 0);
+        if (ok) mbar_arrive_release_at(q_ready, 0);
         for (int j = 0; j < t.nt && ok; ++j, ++kt) {
           const int s = kt % kPStages;
           ok = mbar_wait(&kv_full[s], (uint32_t)(kt / kPStages) & 1u) && !*abort_flag;
-          if (ok) mbar_arrive_at(&kv_ready[s], 0);
+          if (ok) mbar_arrive_release_at(&kv_ready[s], 0);
         }
         ++it;
       }
@@ -531,16 +539,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsF, 1)
           mma_commit_pair(&s_full[buf]);
           if (j + 1 == ns) mma_commit_pair(q_empty);
         };
-        ok = warp_wait(q_ready, it & 1) && warp_wait(&kv_ready[ks], kl);
+        ok = warp_wait_cluster(q_ready, it & 1) && warp_wait_cluster(&kv_ready[ks], kl);
         if (!ok) break;
         tc_fence_after();
         issue_s(0);
         issue_s(1);
         for (int j = 0; j < ns; ++j) {
           const uint32_t buf = warp_uniform((step + j) & 1);
-          if (!(j & 1) && j + 2 < ns) ok = warp_wait(&kv_ready[ks], kl);
+          if (!(j & 1) && j + 2 < ns) ok = warp_wait_cluster(&kv_ready[ks], kl);
           if (ok && j == 0 && it > 0) ok = warp_wait(o_free, (it - 1) & 1);
-          ok = ok && warp_wait(&p_full[buf], ((step + j) >> 1) & 1);
+          // where a step cleared rows of V, those stores have to reach the products of both CTAs
+          ok = ok && (clears_v(t, p, j) ? warp_wait_cluster(&p_full[buf], ((step + j) >> 1) & 1)
+                                        : warp_wait(&p_full[buf], ((step + j) >> 1) & 1));
           if (!ok) break;
           tc_fence_after();
           const uint64_t vb = desc_add(vd, warp_uniform(vs * L::stage + (j & 1) * 8192));
@@ -594,7 +604,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsF, 1)
         tmem_ld32_nowait(t_b, sr[0]);
         tmem_ld32_nowait(t_b + 32, sr[1]);
         tmem_ld_wait();
-        const bool masked = j * 64 + 64 > all_see;
+        const bool masked = j * 64 + 64 > all_see, clears = clears_v(a, p, j);
         if (masked) {
           const int n = lim - j * 64;
 #pragma unroll
@@ -602,7 +612,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsF, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (32 * c + i >= n) sr[c][i] = 0xff800000u;
-          if (j * 64 + 64 > a.len.nk && a.len.nk < p.nk) {
+          if (clears) {
             // V behind the length may hold anything, and 0 times it is not 0:
             // clear those rows of this CTA's half before any product reads them
             const int i = kt + (j >> 1), r = (j & 1) * 64 + (t & 63);
@@ -662,7 +672,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsF, 1)
         l2 = add2(l2, add2(add2(s4[0], s4[1]), add2(s4[2], s4[3])));
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_at(&p_full[buf], 0);
+        if (lane == 0) {
+          if (clears) mbar_arrive_release_at(&p_full[buf], 0);
+          else mbar_arrive_at(&p_full[buf], 0);
+        }
       }
       if (a.ns > 0 && ok) {
         ok = __all_sync(0xffffffffu, mbar_wait(acc_full, (uint32_t)it & 1u));

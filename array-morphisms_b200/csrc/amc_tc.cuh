@@ -332,14 +332,40 @@ __device__ __forceinline__ float4 ld_cluster(const float* p, uint32_t rank) {
       : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem_addr(p)), "r"(rank) : "memory");
   return v;
 }
-// Arrive at `bar` (this CTA's address) in the CTA of rank `rank`.  Without a
-// cluster-wide release: what such an arrival announces is in tensor memory or
-// shared memory read by the products (tcgen05 and proxy fences order those),
-// and a release at cluster scope delayed each arrival by about 1500 clocks.
+// Arrive at `bar` (this CTA's address) in the CTA of rank `rank`.
+// mbar_arrive_at releases at CTA scope, the default, and is for arrivals that
+// announce tensor memory alone: the tcgen05 fences around it order those
+// accesses, and that they do so across the pair rests on what is observed and
+// common in such kernels, not on a statement of the PTX document.
+// mbar_arrive_release_at releases at cluster scope, for arrivals that announce
+// this CTA's shared memory; the waiting side then acquires at cluster scope
+// (mbar_wait_cluster).  Such a release delayed each of the softmax warps'
+// arrivals by about 1500 clocks, so they make it only where they wrote there.
 __device__ __forceinline__ void mbar_arrive_at(uint64_t* bar, uint32_t rank) {
   asm volatile(
       "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\t"
       "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_addr(bar)), "r"(rank) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_release_at(uint64_t* bar, uint32_t rank) {
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\t"
+      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_addr(bar)), "r"(rank) : "memory");
+}
+// mbar_wait that acquires what the other CTA of the pair released.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int limit = 1 << 22) {
+  const uint32_t a = smem_addr(bar);
+  for (int i = 0; i < limit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(a), "r"(parity) : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ bool warp_wait_cluster(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity));
 }
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)), "r"(ncols)

@@ -679,3 +679,20 @@ def test_a_layer_trains(nn):
         # the first step is lr against the gradient's sign, but where |g| is near eps
         sure = g.abs() > 1e-4
         assert ((z - y - 1e-2 * g.sign()).abs()[sure] < 1e-5).all()
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 64), ("f16", 64), ("bf16", 32)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_pairs_of_ctas_see_the_values_that_either_cleared(nn, dtype, d, causal):
+    """Both CTAs of a pair clear their columns of V behind the length, and one of
+    them issues the products that read both: over lengths on every side of a
+    step of 64 keys, and many launches, NaN there never reaches a result."""
+    lens = [521, 520, 513, 512, 449, 447, 385, 383, 65, 1]
+    make = lambda: Case(B=10, H=16, K=4, nq=300, nk=521, d=d, dtype=dtype, causal=causal, kv_lens=lens)
+    c, e = make(), make()
+    for i, n in enumerate(lens):
+        c.k[i, :, n:], c.v[i, :, n:] = 0, 0
+        e.k[i, :, n:], e.v[i, :, n:] = math.nan, math.nan
+    want = c.fwd(nn)
+    for _ in range(30):
+        assert all(torch.equal(x, y) for x, y in zip(want, e.fwd(nn)))
