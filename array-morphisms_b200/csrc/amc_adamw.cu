@@ -161,18 +161,6 @@ __device__ __forceinline__ void store_codes(uint8_t* p, uint32_t w, int64_t e, i
 __device__ __forceinline__ float2 sum2(float2 a, float2 b) {
   return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y));
 }
-// The square root of x >= 0, rounded to nearest: one Newton step (Heron's
-// method) from the approximate reciprocal root, with the residual x - s^2
-// formed exactly by one fused operation; the library's root where that
-// residual could underflow, and for infinities and NaN.
-__device__ __forceinline__ float root_nearest(float x) {
-  float y;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  const float s = x * y;
-  float r = __fmaf_rn(__fmaf_rn(-s, s, x), 0.5f * y, s);
-  if (!(x >= 7.888609052210118e-31f && x <= 3e38f)) r = sqrtf(x);   // 2^-100
-  return r;
-}
 __device__ __forceinline__ float reciprocal(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -258,7 +246,7 @@ __global__ void __launch_bounds__(256, kAdamCtas) k_adamw(const __grid_constant_
         const float2 gg = get2(g[j], k);
         const float2 mm = sum2(mul2(get2(m[j], k), twice(b1)), mul2(gg, twice(r1)));
         const float2 vv = sum2(mul2(get2(v[j], k), twice(b2)), mul2(mul2(gg, gg), twice(r2)));
-        const float2 u = make_float2(root_nearest(vv.x), root_nearest(vv.y));
+        const float2 u = make_float2(__fsqrt_rn(vv.x), __fsqrt_rn(vv.y));
         const float2 den = add2(mul2(u, twice(root)), twice(a.eps));
         const float2 step = mul2(mm, make_float2(reciprocal(den.x), reciprocal(den.y)));
         put2(p[j], k, add2(mul2(get2(p[j], k), twice(keep)), mul2(twice(-rate), step)));

@@ -696,3 +696,25 @@ def test_pairs_of_ctas_see_the_values_that_either_cleared(nn, dtype, d, causal):
     want = c.fwd(nn)
     for _ in range(30):
         assert all(torch.equal(x, y) for x, y in zip(want, e.fwd(nn)))
+
+
+@pytest.mark.parametrize("b2", [0.0, 0.5])
+def test_adamw_8bit_roots_are_rounded_to_nearest(nn, b2):
+    """One element a block: its scale is sqrt(v) / 448, the root and the product
+    each rounded to nearest.  From zero states v = (1 - b2) g^2, at b2 = 0 and 1/2
+    one rounding of g^2 and both parities of its exponent; over the range of f32
+    with its edges, in which the smallest root, 2^-74.5, is above the least scale."""
+    n = 1 << 15
+    g1 = torch.rand(n, generator=torch.Generator().manual_seed(3)) + 1
+    g1 = g1 * 2.0 ** torch.randint(-72, 62, (n,), generator=torch.Generator().manual_seed(4)).float()
+    g1[:6] = torch.tensor([2.0 ** -74, 2.0 ** -63, 1.5 * 2.0 ** -50, 2.0 ** -50 * (1 - 2.0 ** -24), 1.8e19, 1.0])
+    g = torch.zeros(n, 256)
+    g[:, 0] = g1
+    g = g.view(-1).cuda()
+    p, m, v = torch.zeros_like(g), *(torch.zeros(g.shape, dtype=torch.float8_e4m3fn, device="cuda") for _ in range(2))
+    ms, vs = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    state = torch.tensor([0, 0], device="cuda")
+    nn.AdamW([p], [g], [m], [v], state, beta2=b2, m_scales=[ms], v_scales=[vs]).step()
+    x = (g1 * g1) * (1 - b2)                         # f32, IEEE on the host
+    root = x.double().sqrt().float()                 # 53 bits, then 24: no double rounding for a root of 24 bits
+    assert torch.equal(vs.cpu(), root * torch.tensor(1 / 448, dtype=torch.float32))
