@@ -33,7 +33,6 @@ namespace amc {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.69314718055994530942f;
 
 // rows r0 .. r0+TT of a (rows, dim) matrix into dst[TT][W], zero outside
 // rows < rows_end and columns < dim.  f32 rows on 16-byte boundaries are
@@ -264,10 +263,10 @@ __global__ void __launch_bounds__(256, 1) k_diff_fwd_simt(const __grid_constant_
     float inv[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      inv[m] = sum[m][i] > 0.f ? 1.f / sum[m][i] : 0.f;
+      inv[m] = sum[m][i] != 0.f ? 1.f / sum[m][i] : 0.f;
       if (p.lse && tx == 0 && r < p.nq)
         p.lse[((int64_t)b * 2 * p.heads + 2 * h + m) * p.nq + r] =
-            sum[m][i] > 0.f ? fmaf(top[m][i], kLn2, logf(sum[m][i])) : -INFINITY;
+            row_lse(top[m][i], sum[m][i]);
     }
 #pragma unroll
     for (int c = 0; c < DV / 16; ++c) {

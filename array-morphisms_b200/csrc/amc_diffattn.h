@@ -1,6 +1,8 @@
 // Shared by the differential-attention translation units.
 #pragma once
 
+#include <cmath>
+
 #include "amc_half.cuh"
 #include "amc_internal.h"
 
@@ -25,6 +27,12 @@ __device__ __forceinline__ int diff_limit(const DiffLens& l, int causal, int i) 
 __device__ __forceinline__ int diff_first_row(const DiffLens& l, int causal, int j) {
   if (j >= l.nk) return l.nq;
   return causal ? min(l.nq, max(0, j - (l.nk - l.nq))) : 0;
+}
+
+// The natural-log row log-sum-exp from a row's maximum (log2 units) and sum: -inf
+// only where nothing was summed, so that a NaN among the scores stays one.
+__device__ __forceinline__ float row_lse(float top, float sum) {
+  return sum == 0.f ? -INFINITY : fmaf(top, 0.69314718055994530942f, logf(sum));
 }
 
 // Workspace of the backward.  For every two rows (2 r, 2 r + 1) of a (batch,

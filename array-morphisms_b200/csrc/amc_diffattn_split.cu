@@ -43,7 +43,6 @@ constexpr int kShareCtas = 148 * 2;  // CTAs that share the keys
 constexpr int kMinShare = 4;         // blocks of 64 keys: 4 boxes a warp
 constexpr int kMaxBatch = 1024;      // sequences whose lengths a CTA sums up
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.69314718055994530942f;
 
 __device__ int g_diff_split_error;
 
@@ -392,7 +391,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
       }
     } else {
       const float lam = lam_of<T>(p, h);
-      const float f0 = l[0] > 0.f ? 1.f / l[0] : 0.f, f1 = l[1] > 0.f ? 1.f / l[1] : 0.f;
+      const float f0 = l[0] != 0.f ? 1.f / l[0] : 0.f, f1 = l[1] != 0.f ? 1.f / l[1] : 0.f;
 #pragma unroll
       for (int c = 0; c < NV / 32; ++c) {
         const float o1 = acc[1][c] * f1;
@@ -400,7 +399,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
       }
       if (p.lse && lane < 2) {
         const float ll = lane ? l[1] : l[0], mm = lane ? mx[1] : mx[0];
-        p.lse[((int64_t)b * 2 * p.heads + 2 * h + lane) * p.nq + i] = ll > 0.f ? fmaf(mm, kLn2, logf(ll)) : -INFINITY;
+        p.lse[((int64_t)b * 2 * p.heads + 2 * h + lane) * p.nq + i] = row_lse(mm, ll);
       }
     }
   }
@@ -458,7 +457,7 @@ __global__ void __launch_bounds__(256) k_diff_join(const __grid_constant__ amc_d
   const float base = mx == -INFINITY ? 0.f : mx;
   for (int k = tid & 31; k < n; k += 32) l = fmaf(ml[m][k].y, exp2f(ml[m][k].x - base), l);
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = l != 0.f ? 1.f / l : 0.f;
   const float lam = lam_of<T>(p, h);
   for (int c1 = 0; c1 < p.dv; c1 += 128) {
     const int col = c1 + c;
@@ -474,7 +473,7 @@ __global__ void __launch_bounds__(256) k_diff_join(const __grid_constant__ amc_d
     __syncthreads();
   }
   if (p.lse && c == 0)
-    p.lse[((int64_t)b * 2 * p.heads + 2 * h + m) * p.nq + i] = l > 0.f ? fmaf(mx, kLn2, logf(l)) : -INFINITY;
+    p.lse[((int64_t)b * 2 * p.heads + 2 * h + m) * p.nq + i] = row_lse(mx, l);
 }
 
 namespace {

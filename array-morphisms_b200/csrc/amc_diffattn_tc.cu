@@ -45,7 +45,6 @@ namespace {
 constexpr int kThreadsF = 352;      // warps 0-7 softmax, 8 loads, 9 and 10 issue
 constexpr int kKStages = 3, kVStages = 2;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.69314718055994530942f;
 
 template <int NV>
 struct FwdSmem {
@@ -278,14 +277,14 @@ __global__ void __launch_bounds__(kThreadsF, 1) k_diff_fwd_tc(const __grid_const
     if (ns > 0) ok = ok && mbar_wait(all_done, 0);
     const float lam = lam_of<T>(p, h);
     float* xch = (float*)(sm + L::x);
-    xch[m * 128 + t] = l > 0.f ? 1.f / l : 0.f;
+    xch[m * 128 + t] = l != 0.f ? 1.f / l : 0.f;
     ok = named_bar_and(1, 256, ok && !*abort_flag);
     if (ok) {
       // warpgroup m writes columns 64 m .. of both results (NV = 64: group 0 alone)
       tc_fence_after();
       if (row < p.nq) {
         if (p.lse) p.lse[((int64_t)b * 2 * p.heads + 2 * h + m) * p.nq + row] =
-            l > 0.f ? fmaf(top, kLn2, logf(l)) : -INFINITY;
+            row_lse(top, l);
       }
       const float f0 = xch[t], f1 = xch[128 + t], f = -lam;
       if (64 * m < NV) {
@@ -684,7 +683,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsF, 1)
       const float l = l2.x + l2.y;
       float f0 = 0.f, f1 = 0.f;
       if (a.ns > 0) {
-        xch[m * 128 + t] = l > 0.f ? 1.f / l : 0.f;
+        xch[m * 128 + t] = l != 0.f ? 1.f / l : 0.f;
         ok = named_bar_and(1, 256, ok && !*abort_flag);
         f0 = xch[t];
         f1 = xch[128 + t];
@@ -692,7 +691,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsF, 1)
       if (!ok) break;
       const float lam = lam_of<T>(p, a.h);
       if (p.lse && row < p.nq)
-        p.lse[((int64_t)a.b * 2 * p.heads + 2 * a.h + m) * p.nq + row] = l > 0.f ? fmaf(top, kLn2, logf(l)) : -INFINITY;
+        p.lse[((int64_t)a.b * 2 * p.heads + 2 * a.h + m) * p.nq + row] = row_lse(top, l);
       // warpgroup m writes columns 64 m .. of both results (NV = 64: group 0 alone)
       if (64 * m < NV) {
         T* o = (T*)p.o + a.b * p.os[0] + a.h * p.os[1] + (int64_t)row * p.os[2] + 64 * m;

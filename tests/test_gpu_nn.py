@@ -718,3 +718,28 @@ def test_adamw_8bit_roots_are_rounded_to_nearest(nn, b2):
     x = (g1 * g1) * (1 - b2)                         # f32, IEEE on the host
     root = x.double().sqrt().float()                 # 53 bits, then 24: no double rounding for a root of 24 bits
     assert torch.equal(vs.cpu(), root * torch.tensor(1 / 448, dtype=torch.float32))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B,H,K,nq,nk,d", [(2, 2, 1, 5, 40, 64),       # single tokens, 16 rows a key head
+                                           (1, 2, 2, 1, 2000, 64),     # their parts joined
+                                           (2, 4, 1, 1, 2000, 32),
+                                           (1, 2, 1, 130, 140, 64),    # single CTAs
+                                           (6, 16, 8, 260, 270, 64),   # pairs of CTAs
+                                           (1, 1, 1, 20, 40, 100)])    # wide heads
+def test_diff_attention_rows_that_hold_nan(nn, dtype, B, H, K, nq, nk, d):
+    """A row of Q that holds NaN has NaN for its log-sum-exp, not the -inf of a row
+    that sees no key, and NaN for its outputs and gradients; the other rows'
+    results are those of a call without it."""
+    make = lambda: Case(B=B, H=H, K=K, nq=nq, nk=nk, d=d, dtype=dtype)
+    c, e = make(), make()
+    at = nq // 2
+    e.q[0, 1, at, 3] = math.nan               # map 2 of head 0
+    (o, lse, o2), (on, lsen, o2n) = c.fwd(nn), e.fwd(nn)
+    assert lsen[0, 1, at].isnan() and on[0, 0, at].isnan().all() and o2n[0, 0, at].isnan().all()
+    assert lsen.isnan().sum() == 1 and on.isnan().sum() == o2n.isnan().sum() == on.shape[3]
+    for x, y in ((o, on), (o2, o2n), (lse, lsen)):
+        fine = ~y.isnan()
+        assert torch.equal(x[fine], y[fine])
+    g = e.bwd(nn, on, lsen, o2n)
+    assert g["dq"][0, :2, at].isnan().all() and g["dv"][0, 0].isnan().all() and g["dlam"][0].isnan().all()
