@@ -296,8 +296,9 @@ __global__ void __launch_bounds__(256) k_diff_bwd_rows(const __grid_constant__ a
     nl1[r] = nl2[r] = -INFINITY;
     if (i < p.nq && diff_limit(len, p.causal, i) > 0) {
       const float* lse = p.lse + ((int64_t)b * 2 * p.heads + 2 * h) * p.nq + i;
-      nl1[r] = -lse[0] * kLog2e;
-      nl2[r] = -lse[p.nq] * kLog2e;
+      // a row whose scores are all -inf has -inf here too: like a row that sees no key
+      nl1[r] = lse[0] == -INFINITY ? -INFINITY : -lse[0] * kLog2e;
+      nl2[r] = lse[p.nq] == -INFINITY ? -INFINITY : -lse[p.nq] * kLog2e;
       const T* o = (const T*)p.o + b * p.os[0] + h * p.os[1] + (int64_t)i * p.os[2];
       const T* o2 = (const T*)p.o2 + b * p.o2s[0] + h * p.o2s[1] + (int64_t)i * p.o2s[2];
       const T* go = (const T*)p.d_o + b * p.dos[0] + h * p.dos[1] + (int64_t)i * p.dos[2];

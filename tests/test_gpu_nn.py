@@ -743,3 +743,20 @@ def test_diff_attention_rows_that_hold_nan(nn, dtype, B, H, K, nq, nk, d):
         assert torch.equal(x[fine], y[fine])
     g = e.bwd(nn, on, lsen, o2n)
     assert g["dq"][0, :2, at].isnan().all() and g["dv"][0, 0].isnan().all() and g["dlam"][0].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("nq,nk,d", [(1, 700, 64), (140, 150, 64), (20, 30, 100)])
+def test_diff_attention_rows_whose_scores_are_all_minus_infinity(nn, dtype, nq, nk, d):
+    """Finite queries and keys whose products pass the range of f32: such a row
+    weighs no key, so its results and its gradients are 0, like those of a row
+    that sees none, and the other rows' are finite."""
+    c = Case(B=1, H=1, K=1, nq=nq, nk=nk, d=d, dtype=dtype, heads_inner=False)
+    c.q[..., 0], c.k[..., 0] = 0, -1e20
+    at = nq // 2
+    c.q[0, :, at, 0] = 1e25
+    o, lse, o2 = c.fwd(nn)
+    assert (lse[0, :, at] == -math.inf).all() and (o[0, 0, at] == 0).all() and (o2[0, 0, at] == 0).all()
+    g = c.bwd(nn, o, lse, o2)
+    assert (g["dq"][0, :, at] == 0).all()
+    assert all(torch.isfinite(x).all() for x in g.values())
