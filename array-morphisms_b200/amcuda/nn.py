@@ -302,7 +302,9 @@ class AdamW:
     (float32) the update is made on those and params receive them rounded.  m
     and v are float32, or torch.float8_e4m3fn codes of m and sqrt(v) with a
     float32 scale for every STATE_BLOCK elements in m_scales and v_scales
-    (zeros are a fresh state).  `state` is an int64 pair on the device, (steps
+    (zeros are a fresh state).  A NaN gradient makes its own element's
+    parameter and states NaN; an infinite one, with 8-bit states, its whole
+    block's at the next step.  `state` is an int64 pair on the device, (steps
     done, 0); each step counts it, so a step captured into a CUDA graph goes
     on counting at its replays.  lr is a number, or a float32 tensor of one
     element on the device that is read at every step.  Two steps of the same

@@ -17,7 +17,9 @@
 // hold m and sqrt(v) as e4m3 (4 significant bits, 2^-9 .. 448) of the value
 // over its block's largest.  Their rounding is random, up with the
 // probability of the remainder: with b2 = 0.999 a step changes v by about
-// 0.1 %, nearest rounding to a code 6 % away would never move it.  The bits
+// 0.1 %, nearest rounding to a code 6 % away would never move it.  A NaN keeps its
+// element's codes NaN and is left out of the block's largest value; an infinite
+// one makes its scale infinite, and the block NaN at the next step.  The bits
 // come from the lowbias32 mixer (C. Wellons, "Prospecting for Hash
 // Functions") of element, tensor and step.
 //
@@ -35,7 +37,7 @@ namespace amc {
 
 using tc::add2;
 using tc::max3;
-using tc::min3;
+using tc::min3_nan;
 using tc::mul2;
 
 namespace {
@@ -46,6 +48,7 @@ constexpr int64_t kAdamMost = (int64_t)0x7fffffff * kAdamChunk;
 constexpr int kAdamCtas = 4;         // a SM, at 64 registers a thread
 constexpr int kAdamBlock = 256;      // elements per scale
 constexpr float kE4m3Max = 448.f;
+constexpr uint32_t kE4m3Nan = 127;
 
 struct AdamTensor {
   amc_adamw_tensor t;
@@ -275,11 +278,12 @@ __global__ void __launch_bounds__(256, kAdamCtas) k_adamw(const __grid_constant_
           const float2 x = mul2(get2(m[j], k), twice(im)), u = mul2(get2(v[j], k), twice(iu));
           put2(m[j], k, x);
           put2(v[j], k, u);
-          least = min3(least, fabsf(x.x), fabsf(x.y));
-          least = min3(least, u.x, u.y);
+          least = min3_nan(least, fabsf(x.x), fabsf(x.y));
+          least = min3_nan(least, u.x, u.y);
         }
       // below 2^-6 of 448 the codes are even steps: about one block in forty
-      // of normally distributed values has any, and takes the longer way
+      // of normally distributed values has any, and takes the longer way, as
+      // one that holds NaN does
       const bool fine = __any_sync(0xffffffffu, !(least >= kE4m3Fine));
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -292,6 +296,8 @@ __global__ void __launch_bounds__(256, kAdamCtas) k_adamw(const __grid_constant_
           if (fine) {
             if (fabsf(m[j][k]) < kE4m3Fine) c = e4m3_fine(fabsf(m[j][k]), rnd & 0xFFFFFu);
             if (v[j][k] < kE4m3Fine) d = max(e4m3_fine(v[j][k], rnd >> 12), v[j][k] > 0.f ? 1u : 0u);
+            if (isnan(m[j][k])) c = kE4m3Nan;
+            if (isnan(v[j][k])) d = kE4m3Nan;
           }
           cm[j] |= (c | bits >> 31 << 7) << (8 * k);
           cv[j] |= d << (8 * k);

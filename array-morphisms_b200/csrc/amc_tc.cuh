@@ -260,9 +260,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ float min3(float a, float b, float c) {
+// NaN where one of them is.
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
   float d;
-  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 // Nearest tf32 by integer rounding of the bit pattern (ties away from zero),

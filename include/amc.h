@@ -462,6 +462,8 @@ int amc_diff_attention_workspace(const amc_diff_attention* p, int32_t backward, 
  * random with 20 bits mixed from element, tensor and step, because a moving
  * average that changes by less than half a code would stand still under
  * nearest rounding; a nonzero root never rounds to 0.
+ * A NaN of an 8-bit state stays in its element, an infinity makes the scale of
+ * its block infinite and the block NaN at the next step.
  * step_state is two s64 on the device: the steps done, which the call
  * increments, and a counter that must be 0 before the first call; so a
  * captured step advances at each replay.  lr_dev, if not NULL, holds lr on

@@ -760,3 +760,38 @@ def test_diff_attention_rows_whose_scores_are_all_minus_infinity(nn, dtype, nq, 
     g = c.bwd(nn, o, lse, o2)
     assert (g["dq"][0, :, at] == 0).all()
     assert all(torch.isfinite(x).all() for x in g.values())
+
+
+def test_adamw_8bit_keeps_a_nan(nn):
+    """A gradient's NaN stays in its element's parameter and states, as in 32-bit
+    states, and its block's other elements are as without it; an infinity makes
+    its block's scales infinite, and the block NaN at the next step."""
+    n = 1024
+
+    def run(bad):
+        p = randn((n,), 1, torch.float32)
+        m, v = (torch.zeros(n, dtype=torch.float8_e4m3fn, device="cuda") for _ in range(2))
+        ms, vs = torch.zeros(4, device="cuda"), torch.zeros(4, device="cuda")
+        g = randn((n,), 2, torch.float32)
+        g[5], g[256:512] = 0.0, 0.0
+        for i, x in bad.items():
+            g[i] = x
+        opt = nn.AdamW([p], [g], [m], [v], torch.tensor([0, 0], device="cuda"), m_scales=[ms], v_scales=[vs], **HYPER)
+        opt.step()
+        first = [p.clone(), m.float(), v.float(), ms.clone(), vs.clone()]
+        g.copy_(randn((n,), 3, torch.float32))
+        opt.step()
+        return first, [p.clone(), m.float(), v.float(), ms, vs]
+    nan = {5: math.nan, **{i: math.nan for i in range(256, 512)}}
+    where = torch.zeros(n, dtype=torch.bool, device="cuda")
+    where[list(nan)] = True
+    for a, b in zip(run({}), run(nan)):
+        for x, y in zip(a[:3], b[:3]):
+            assert torch.equal(y.isnan(), where) and torch.equal(x[~where], y[~where])
+        keep = [0, 2, 3]
+        assert torch.equal(a[3][keep], b[3][keep]) and torch.equal(a[4][keep], b[4][keep])
+    first, second = run({600: math.inf})
+    block = torch.arange(n, device="cuda") // 256 == 2
+    assert first[3].isinf().tolist() == first[4].isinf().tolist() == [False, False, True, False]
+    assert first[1][600].isnan() and first[2][600].isnan() and first[1].isnan().sum() == 1
+    assert second[0].isnan()[block].all() and not second[0].isnan()[~block].any()
