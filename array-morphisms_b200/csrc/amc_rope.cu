@@ -6,9 +6,11 @@
 // pairs once, into shared memory, and then go over the 16-byte vectors of every
 // head of both tensors, four in flight a lane, so a position's heads, which a
 // projection leaves side by side, move in whole lines.  The first vectors are
-// loaded before the angles are formed.  The turn count is formed and reduced to
-// half a turn in f64 (a position of 2^40 keeps its angle), its sine and cosine
-// in f32.  No table is read.
+// loaded before the angles are formed.  The turn count is a product of two-part
+// doubles: a single one, off by 2^-52 of itself, is right to f32's last bits up to
+// positions of about 2^30 only, this one up to the 2^53 that a double counts.  What
+// is left of it after whole turns goes to f32 for sine and cosine.  No table is
+// read.
 // Measured: queries and keys of 16 x 2048 tokens, 16 heads each, d 64, bf16
 // (268 MB): 48 us, 5.6 TB/s; 16 tokens: 5 us, of which the launch is most.
 #include <cmath>
@@ -23,6 +25,7 @@ namespace {
 constexpr int kRopeWarps = 4;
 constexpr int kRopeFlight = 4;       // vectors (pairs of them) in flight a lane
 constexpr int kRopeMaxRot = 1024;
+constexpr double kTurn = 0.15915494309189535, kTurnLow = -9.839338337591243e-18;   // 1 / (2 pi) and the rest of it
 
 struct RopeArgs {
   amc_rope_tensor t[2];
@@ -108,8 +111,11 @@ __global__ void __launch_bounds__(kRopeWarps * 32) k_rope(const __grid_constant_
   load(lane);
   const double p = (double)a.pos[b * a.pos_stride + i];
   for (int k = lane; k < a.rot / 2; k += 32) {
-    double turns = p * (a.freqs[k] * 0.15915494309189533577);   // 1 / (2 pi)
-    turns -= rint(turns);
+    // freq / 2 pi and its product with p each as a double and what it rounds off
+    const double f = a.freqs[k], g = f * kTurn, g_low = fma(f, kTurn, -g) + f * kTurnLow;
+    double turns = p * g;
+    const double low = fma(p, g, -turns) + p * g_low;
+    turns = (turns - rint(turns)) + low;
     float2 t;
     sincospif(2.f * (float)turns, &t.y, &t.x);
     turn[k] = make_float2(t.x * a.mscale, t.y * (a.inverse ? -a.mscale : a.mscale));

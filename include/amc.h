@@ -381,7 +381,8 @@ int amc_conv2d_wgrad_f32(const float* X, const float* dY, float* dW, int32_t N, 
 #define AMC_E4M3 18   /* 8-bit optimizer states only */
 
 /* Rotary positions.  Pair i of a row at position p turns by p * freqs[i]
- * radians (formed in f64, so far positions keep their angle) and is scaled by
+ * radians (formed in two-part f64: positions up to 2^53 keep their angle to
+ * the precision of f32) and is scaled by
  * mscale: out_a = ms (a cos - b sin), out_b = ms (b cos + a sin).  The pair is
  * elements (i, i + rot/2), or (2i, 2i + 1) when interleaved; elements from
  * rot on are copied.  inverse != 0 turns back, which is the gradient.  One or

@@ -795,3 +795,32 @@ def test_adamw_8bit_keeps_a_nan(nn):
     assert first[3].isinf().tolist() == first[4].isinf().tolist() == [False, False, True, False]
     assert first[1][600].isnan() and first[2][600].isnan() and first[1].isnan().sum() == 1
     assert second[0].isnan()[block].all() and not second[0].isnan()[~block].any()
+
+
+def turns_exactly(pos, freq):
+    """pos * freq / 2 pi less whole turns, in rationals (freq is a double, 1 / 2 pi to 60 digits)."""
+    from fractions import Fraction
+    tau = Fraction(6283185307179586476925286766559005768394338798750211641949889, 10 ** 60)
+    t = pos * Fraction(freq) / tau
+    return float(t - round(t))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_far_positions_in_32_bits(nn, interleaved):
+    """Positions up to 2^53 keep the angle of position times frequency, against an
+    exact reduction on the host: the allowance is that of near positions."""
+    d = 64
+    at = [0, 1, 4097, (1 << 20) + 7, (1 << 30) + 12345, (1 << 33) + 987654321, (1 << 40) + 1234567, (1 << 47) - 1,
+          (1 << 53) - 1, -((1 << 40) + 77)]
+    freqs, _ = nn.rope_freqs(d)
+    turns = torch.tensor([[turns_exactly(p, f) for f in freqs.tolist()] for p in at], dtype=torch.float64, device="cuda")
+    c, s = (2 * math.pi * turns).cos(), (2 * math.pi * turns).sin()
+    x = randn((1, 2, len(at), d), 7, torch.float32)
+    out = torch.empty_like(x)
+    nn.rope(x, torch.tensor(at, device="cuda"), freqs.cuda(), out, interleaved=interleaved)
+    ia, ib = (slice(0, d, 2), slice(1, d, 2)) if interleaved else (slice(0, d // 2), slice(d // 2, d))
+    xd = x.double()
+    y, terms = torch.empty_like(xd), torch.empty_like(xd)
+    y[..., ia], y[..., ib] = xd[..., ia] * c - xd[..., ib] * s, xd[..., ib] * c + xd[..., ia] * s
+    terms[..., ia] = terms[..., ib] = xd[..., ia].abs() + xd[..., ib].abs()
+    rope_close(out, y, terms, torch.float32)
