@@ -359,19 +359,30 @@ class AdamW:
                 e.master = lists["masters"][i].data_ptr()
             if bits8:
                 e.m_scale, e.v_scale = lists["m_scales"][i].data_ptr(), lists["v_scales"][i].data_ptr()
-        self._lr_dev = None
-        if isinstance(lr, torch.Tensor):
-            if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != self.device:
-                raise ValueError("AdamW: lr is a number or a float32 tensor of one element on the device")
-            self._lr_dev, lr = lr, 0.0
-        self.lr, self.betas, self.eps, self.weight_decay = float(lr), (beta1, beta2), eps, weight_decay
+        self.lr, self.betas, self.eps, self.weight_decay = lr, (beta1, beta2), eps, weight_decay
         self.state, self._table, self._n = state, table, n
         self._kinds = (_dtype(params[0], "AdamW"), _dtype(grads[0], "AdamW")) if n else (A.F32, A.F32)
         self._kinds += (A.E4M3 if bits8 else A.F32,)
         # the table's addresses stay valid, even if a tensor is given other memory
         self._keep = [t.untyped_storage() for x in (params, *lists.values()) for t in x]
 
+    @property
+    def lr(self):
+        """The rate of the next step, as it was given: a number or a tensor on the device."""
+        return self._lr if self._lr_dev is None else self._lr_dev
+
+    @lr.setter
+    def lr(self, lr) -> None:
+        import torch
+        if not isinstance(lr, torch.Tensor):
+            self._lr, self._lr_dev = float(lr), None
+        elif lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != self.device:
+            raise ValueError("AdamW: lr is a number or a float32 tensor of one element on the device")
+        else:
+            self._lr, self._lr_dev = 0.0, lr
+
     def step(self, stream=None) -> None:
-        """One update of every tensor; `lr` may be assigned between steps."""
+        """One update of every tensor; `lr`, a number or a tensor, may be assigned
+        between steps (a captured step keeps the one it was captured with)."""
         _run("amc_adamw", self.device, stream, self._table, self._n, *self._kinds, self.state.data_ptr(),
-             _ptr(self._lr_dev), self.lr, *self.betas, self.eps, self.weight_decay)
+             _ptr(self._lr_dev), self._lr, *self.betas, self.eps, self.weight_decay)

@@ -296,3 +296,23 @@ def test_c_adamw_refuses_more_than_it_can_count():
     assert "too many" in A.last_error()
     assert c_adamw(count=2, n=(1 << 42) - (1 << 12)) == 1
     assert "too many" in A.last_error()
+
+
+def test_adamw_takes_an_assigned_rate(monkeypatch):
+    """A rate assigned after the object was made is the next step's, whether it or the first was a tensor."""
+    given = []
+    monkeypatch.setattr(nn, "_run", lambda name, device, stream, *args: given.append(args[6:8]))
+    rate = torch.tensor([0.25])
+    opt = nn.AdamW(**adamw_args(lr=rate))
+    opt.step()
+    opt.lr = 0.5
+    assert opt.lr == 0.5
+    opt.step()
+    opt.lr = rate
+    assert opt.lr is rate
+    opt.step()
+    assert given == [(rate.data_ptr(), 0.0), (0, 0.5), (rate.data_ptr(), 0.0)]
+    for bad in (torch.zeros(2), torch.zeros(1, dtype=torch.float64)):
+        with pytest.raises(ValueError):
+            opt.lr = bad
+    assert opt.lr is rate
