@@ -23,6 +23,7 @@
 // 2.46 ms, 58 % of the FMA rate.
 #include <cmath>
 #include <initializer_list>
+#include <type_traits>
 
 #include "amc_diffattn.h"
 #include "amc_half.cuh"
@@ -289,6 +290,9 @@ __global__ void __launch_bounds__(256) k_diff_bwd_rows(const __grid_constant__ a
   const int sub = threadIdx.x % LANES, h = blockIdx.y, b = blockIdx.z;
   const int i0 = blockIdx.x * kAtOnce * kRows + threadIdx.x / LANES;
   const DiffLens len = diff_lens(p, b);
+  float up = 0.f;   // P is rebuilt times 2^up
+  if constexpr (std::is_same<T, __half>::value)
+    if (w.peaks) up = (float)diff_shift(p, w, b, h / (p.heads / p.kv_heads)).ds;
   float d[kAtOnce] = {}, d2[kAtOnce] = {}, nl1[kAtOnce], nl2[kAtOnce];
 #pragma unroll
   for (int r = 0; r < kAtOnce; ++r) {
@@ -297,8 +301,8 @@ __global__ void __launch_bounds__(256) k_diff_bwd_rows(const __grid_constant__ a
     if (i < p.nq && diff_limit(len, p.causal, i) > 0) {
       const float* lse = p.lse + ((int64_t)b * 2 * p.heads + 2 * h) * p.nq + i;
       // a row whose scores are all -inf has -inf here too: like a row that sees no key
-      nl1[r] = lse[0] == -INFINITY ? -INFINITY : -lse[0] * kLog2e;
-      nl2[r] = lse[p.nq] == -INFINITY ? -INFINITY : -lse[p.nq] * kLog2e;
+      nl1[r] = lse[0] == -INFINITY ? -INFINITY : fmaf(-lse[0], kLog2e, up);
+      nl2[r] = lse[p.nq] == -INFINITY ? -INFINITY : fmaf(-lse[p.nq], kLog2e, up);
       const T* o = (const T*)p.o + b * p.os[0] + h * p.os[1] + (int64_t)i * p.os[2];
       const T* o2 = (const T*)p.o2 + b * p.o2s[0] + h * p.o2s[1] + (int64_t)i * p.o2s[2];
       const T* go = (const T*)p.d_o + b * p.dos[0] + h * p.dos[1] + (int64_t)i * p.dos[2];
@@ -628,7 +632,10 @@ int launch_diff_bwd_rows(const amc_diff_attention& p, const DiffBwdWork& w, cuda
   return AMC_OK;
 }
 
-int launch_diff_bwd_simt(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s) {
+int launch_diff_bwd_simt(const amc_diff_attention& p, const DiffBwdWork& work, cudaStream_t s) {
+  DiffBwdWork w = work;
+  w.peaks = nullptr;   // all in f32
+  if (int rc = launch_diff_bwd_rows(p, w, s)) return rc;
   return by_type(p.dtype, [&](auto t) {
     using T = decltype(t);
     return p.d <= 64 && p.dv <= 128 ? bwd_simt<T, 64, 64, 128>(p, w, s) : bwd_simt<T, 32, 128, 256>(p, w, s);
@@ -734,7 +741,6 @@ int amc_diff_attention_bwd(const amc_diff_attention* p, void* stream) {
   if (!p->batch || !p->nq)
     if (int rc = launch_no_dlam(*p, s)) return rc;
   if (!p->batch) return AMC_OK;
-  if (int rc = launch_diff_bwd_rows(*p, w, s)) return rc;
   bool handled = false;
   if (int rc = diff_bwd_tc(*p, w, s, &handled)) return rc;
   if (handled) return AMC_OK;

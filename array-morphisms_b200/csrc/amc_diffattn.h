@@ -44,6 +44,15 @@ __device__ __forceinline__ float row_lse(float top, float sum) {
 // (rows padded to a multiple of 4, so that a tile of them is a bulk copy),
 // then lam and a counter for every head, then one partial of sum P_2 G for
 // every (head, batch, row tile).
+//
+// fp16 tensors on the tensor cores have the operands that the threads make in
+// fp16 too, whose range (2^-24 .. 65504) dS = P (G - D) leaves easily: upstream
+// gradients of 2^-17 over 2000 keys came out wrong by twice the rounding of
+// their terms.  So dS and P_1 - lam P_2 are formed times powers of two, the same
+// for all that add up in a CTA, and the sums are scaled back in f32.  `peaks`
+// holds what bounds them: for every (batch, key head) the largest |dO row|^2 and
+// |V row|^2, for every key head the largest |lam|, as bits (a maximum's order does
+// not change it).
 constexpr int kDiffTile = 32;
 struct DiffBwdWork {
   float4* nlse;
@@ -51,6 +60,7 @@ struct DiffBwdWork {
   float* lam;
   unsigned* done;      // CTAs of this row of lam that have written their partials
   float* partials;
+  unsigned* peaks;     // null: nothing is scaled
   int pitch;   // rows of a (batch, head)
 };
 // The value of row r of map m in such an array.
@@ -58,10 +68,14 @@ __device__ __forceinline__ float diff_row(const float4* x, int64_t first_row, in
   return reinterpret_cast<const float*>(x + (first_row + r) / 2)[2 * m + (r & 1)];
 }
 inline int diff_row_pitch(const amc_diff_attention& p) { return (p.nq + 3) & ~3; }
+inline size_t diff_peaks(const amc_diff_attention& p) {
+  return p.dtype == AMC_F16 ? (size_t)(2 * p.batch + 1) * p.kv_heads : 0;
+}
 inline size_t diff_bwd_bytes(const amc_diff_attention& p) {
   const size_t rows = (size_t)p.batch * p.heads * diff_row_pitch(p);
   const size_t partials = (size_t)p.batch * p.heads * ((p.nq + kDiffTile - 1) / kDiffTile);
-  return rows * sizeof(float4) + 2 * (size_t)p.heads * sizeof(float) + partials * sizeof(float);
+  return rows * sizeof(float4) + 2 * (size_t)p.heads * sizeof(float) + partials * sizeof(float) +
+         diff_peaks(p) * sizeof(unsigned);
 }
 inline DiffBwdWork diff_bwd_work(const amc_diff_attention& p) {
   const size_t rows = (size_t)p.batch * p.heads * diff_row_pitch(p);
@@ -71,8 +85,25 @@ inline DiffBwdWork diff_bwd_work(const amc_diff_attention& p) {
   w.lam = (float*)(w.nsum + rows / 2);
   w.done = (unsigned*)(w.lam + p.heads);
   w.partials = (float*)(w.done + p.heads);
+  w.peaks = (unsigned*)(w.partials + (size_t)p.batch * p.heads * ((p.nq + kDiffTile - 1) / kDiffTile));
   w.pitch = diff_row_pitch(p);
   return w;
+}
+// The exponents of those powers for (batch b, key head g): of dS, which
+// |dO| |V| max(1, |lam|) 2 bounds, and of P_1 - lam P_2, bounded by 1 + |lam|; the
+// bounds land in 2^14 .. 2^15.  0 where a bound is 0 or not finite.
+struct DiffShift {
+  int ds, w;
+};
+__device__ __forceinline__ float diff_pow2(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ DiffShift diff_shift(const amc_diff_attention& p, const DiffBwdWork& w, int b, int g) {
+  const unsigned* x = w.peaks + 2 * ((int64_t)b * p.kv_heads + g);
+  const float lam = __uint_as_float(w.peaks[2 * (int64_t)p.batch * p.kv_heads + g]);
+  auto up = [](float bound) {
+    const int e = (int)(__float_as_uint(bound) >> 23) - 127;
+    return bound > 0.f && e < 128 ? max(-60, min(60, 14 - e)) : 0;
+  };
+  return {up(sqrtf(__uint_as_float(x[0])) * sqrtf(__uint_as_float(x[1])) * 2.f * fmaxf(1.f, lam)), up(1.f + lam)};
 }
 
 // Tensor-core forward; *handled = false (and nothing launched) for other
@@ -89,7 +120,7 @@ int launch_diff_fwd_simt(const amc_diff_attention& p, cudaStream_t s);
 int diff_share(const amc_diff_attention& p, int64_t ctas);
 int launch_diff_bwd_rows(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s);
 int launch_diff_bwd_simt(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s);
-// Tensor-core gradients (after the rows), likewise.
+// Tensor-core gradients (with the rows), likewise.
 int diff_bwd_tc(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t s, bool* handled);
 
 // exp(l0 . l1) and exp(l2 . l3) of row `row` of lam, on every lane of a converged warp.

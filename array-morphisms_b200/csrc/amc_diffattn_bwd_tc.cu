@@ -99,6 +99,51 @@ __device__ __forceinline__ void zero_row(unsigned char* row) {
 
 }  // namespace
 
+// ------------------------------------------------------------------ what bounds fp16 operands
+// The peaks of the workspace, zero before: rows of dO of every head, then rows of
+// V of every key head, 64 a CTA, 16 lanes a row.  What is behind the lengths is
+// left out, and a NaN, whose row is NaN at any scale.
+constexpr int kPeakRows = 64;
+__global__ void __launch_bounds__(256) k_diff_peaks(const __grid_constant__ amc_diff_attention p,
+                                                    const __grid_constant__ DiffBwdWork w) {
+  __shared__ float top[8];
+  const bool values = (int)blockIdx.y >= p.heads;
+  const int h = values ? blockIdx.y - p.heads : blockIdx.y, b = blockIdx.z;
+  const int g = values ? h : h / (p.heads / p.kv_heads), sub = threadIdx.x & 15;
+  const DiffLens len = diff_lens(p, b);
+  const int64_t* st = values ? p.vs : p.dos;
+  const __half* x = (const __half*)(values ? p.v : p.d_o) + b * st[0] + h * st[1];
+  float most = 0.f;
+#pragma unroll
+  for (int k = 0; k < kPeakRows / 16; ++k) {
+    const int64_t r = (int64_t)blockIdx.x * kPeakRows + 16 * k + threadIdx.x / 16;
+    float n = 0.f;
+    if (8 * sub < p.dv && (values ? r < len.nk : r < p.nq && diff_limit(len, p.causal, (int)r) > 0)) {
+      const uint4 v = *reinterpret_cast<const uint4*>(x + r * st[2] + 8 * sub);
+      const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack2<__half>(e[i]);
+        n = fmaf(f.x, f.x, fmaf(f.y, f.y, n));
+      }
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    most = fmaxf(most, n);
+  }
+  most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+  if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) most = fmaxf(most, top[i]);
+    atomicMax(w.peaks + 2 * ((int64_t)b * p.kv_heads + g) + values, __float_as_uint(most));
+  }
+  if (!values && blockIdx.x == 0 && b == 0 && threadIdx.x < 32) {
+    const float lam = fabsf(lam_of<__half>(p, h));
+    if (threadIdx.x == 0) atomicMax(w.peaks + 2 * (int64_t)p.batch * p.kv_heads + g, __float_as_uint(lam));
+  }
+}
+
 // ------------------------------------------------------------------ dK, dV
 // Tensor memory: four 64-column buffers, dV at 256, dK_1, dK_2 at 384 and 448.
 // Even tiles have S_1, S_2 and G in buffers 0, 1 and 2, odd ones in 3, 2 and 1.
@@ -166,6 +211,14 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap
   tc_fence_after();
   const uint32_t tmem = warp_uniform(*tslot);
   const uint32_t t_dv = tmem + 256, t_dk = tmem + 384;
+  // what the sums of dS and of P_1 - lam P_2 are multiplied with, and the latter's scale over the former's
+  float f_dk = p.scale, f_dv = 1.f, to_w = 1.f;
+  if constexpr (!kBf16) {
+    const DiffShift up = diff_shift(p, wk, b, g);
+    f_dk *= diff_pow2(-up.ds);
+    f_dv = diff_pow2(-up.w);
+    to_w = diff_pow2(up.w - up.ds);
+  }
   float* part = (float*)sm;   // [128 keys][kPartPitch] once all products are done
 
   if (warp == 16) {
@@ -276,6 +329,7 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap
     bool ok = true;
     int h = head0, r0 = first;
     float nlam = nt > 0 ? -wk.lam[h] : 0.f;
+    const float2 rw = make_float2(to_w, to_w);
     if (nt > 0) ok = __all_sync(0xffffffffu, mbar_wait(&f_full[0], 0));
     for (int i = 0; i < nt && ok; ++i) {
       const int s = i % kStages;
@@ -350,7 +404,8 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap
       for (int j = 0; j < 8; ++j) {
         const float4 d = rp[j];
         const float2 gg = make_float2(__uint_as_float(gv[2 * j]), __uint_as_float(gv[2 * j + 1]));
-        const float2 both = add2(p1[j], p2[j]);
+        float2 both = add2(p1[j], p2[j]);
+        if constexpr (!kBf16) both = mul2(both, rw);
         const float2 a = mul2(p1[j], add2(gg, make_float2(d.x, d.y))), c = mul2(p2[j], add2(gg, make_float2(d.z, d.w)));
         v[j] = __uint_as_float(pack2<T>(both.x, both.y));
         v1[j] = __uint_as_float(pack2<T>(a.x, a.y));
@@ -380,7 +435,7 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap
                      : (T*)p.dv_ + b * p.dvs[0] + g * p.dvs[1] + (int64_t)key * p.dvs[2] + 64 * (w - 2);
       const uint32_t src = (w < 2 ? t_dk + 64 * w : t_dv + 64 * (w - 2)) + lane_base;
       const int cols = w < 2 ? p.d : p.dv - 64 * (w - 2);
-      const float f = w < 2 ? p.scale : 1.f;
+      const float f = w < 2 ? f_dk : f_dv;
       if (NV == 128 || w < 3) {
 #pragma unroll 1
         for (int c = 0; c < 64; c += 16) {
@@ -430,7 +485,7 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap
       }
       const int m = c / 64, cc = m < 2 ? c % 64 : c - 128;
       if (cc >= (m < 2 ? p.d : p.dv)) continue;
-      const float f = m < 2 ? p.scale : 1.f;
+      const float f = m < 2 ? f_dk : f_dv;
       T* dst = m < 2 ? (T*)p.dk + b * p.dks[0] + (2 * g + m) * p.dks[1] + (int64_t)key * p.dks[2]
                      : (T*)p.dv_ + b * p.dvs[0] + g * p.dvs[1] + (int64_t)key * p.dvs[2];
       *reinterpret_cast<uint2*>(dst + cc) = make_uint2(pack2<T>(sum.x * f, sum.y * f), pack2<T>(sum.z * f, sum.w * f));
@@ -490,6 +545,8 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap& mQ, const CUtensorMap&
   tc_fence_after();
   const uint32_t tmem = warp_uniform(*tslot);
   const uint32_t t_dq = tmem + 384;
+  float back = 1.f;   // P carries the scale of dS
+  if constexpr (!kBf16) back = diff_pow2(-diff_shift(p, wk, b, g).ds);
 
   if (warp == 16) {
     if (lane == 0 && nt > 0) {
@@ -626,12 +683,12 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap& mQ, const CUtensorMap&
         else
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[i] = 0.f;
-        if (row < p.nq && c < p.d) store16<T>(dq + c, v, p.scale, p.d - c);
+        if (row < p.nq && c < p.d) store16<T>(dq + c, v, p.scale * back, p.d - c);
       }
       if (tid == 0) {
         float sum = 0.f;
         for (int i = 0; i < kRowWarps; ++i) sum += red[i];
-        wk.partials[((int64_t)h * p.batch + b) * tiles + tile] = sum;
+        wk.partials[((int64_t)h * p.batch + b) * tiles + tile] = sum * back;
       }
     } else if (tid == 0) {
       *abort_flag = 1;
@@ -709,6 +766,13 @@ int diff_bwd_tc(const amc_diff_attention& p, const DiffBwdWork& w, cudaStream_t 
   if (rc == AMC_ERR_UNSUPPORTED) return AMC_OK;
   if (rc) return rc;
   *handled = true;
+  if (!bf16) {
+    AMC_CUDA(cudaMemsetAsync(w.peaks, 0, diff_peaks(p) * sizeof(unsigned), s));
+    const int rows = p.nq > p.nk ? p.nq : p.nk;
+    k_diff_peaks<<<dim3((rows + kPeakRows - 1) / kPeakRows, p.heads + p.kv_heads, p.batch), 256, 0, s>>>(p, w);
+    AMC_CUDA(cudaGetLastError());
+  }
+  if ((rc = launch_diff_bwd_rows(p, w, s))) return rc;
   if (bf16) return p.dv <= 64 ? bwd_tc<__nv_bfloat16, 64>(p, w, map, s) : bwd_tc<__nv_bfloat16, 128>(p, w, map, s);
   return p.dv <= 64 ? bwd_tc<__half, 64>(p, w, map, s) : bwd_tc<__half, 128>(p, w, map, s);
 }

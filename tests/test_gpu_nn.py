@@ -824,3 +824,44 @@ def test_rope_far_positions_in_32_bits(nn, interleaved):
     y[..., ia], y[..., ib] = xd[..., ia] * c - xd[..., ib] * s, xd[..., ib] * c + xd[..., ia] * s
     terms[..., ia] = terms[..., ib] = xd[..., ia].abs() + xd[..., ib].abs()
     rope_close(out, y, terms, torch.float32)
+
+
+SMALL_AND_LARGE = [
+    # upstream gradients far below 1, as before a loss is scaled up: dS is below fp16's least number, its sums are not
+    dict(B=2, H=2, K=2, nq=300, nk=2000, d=64, up=2.0 ** -17, shift=4.0),
+    dict(B=2, H=4, K=1, nq=1000, nk=1000, d=64, up=2.0 ** -19, shift=4.0, causal=True, q_lens=[1000, 700], kv_lens=[1000, 900]),
+    dict(B=1, H=2, K=1, nq=1500, nk=1500, d=32, up=2.0 ** -19, shift=4.0),
+    # and far above it: dS passes 65504, and the products with a small scale do not
+    dict(B=1, H=2, K=1, nq=40, nk=4, d=64, up=2.0 ** 13, gain=8.0, scale=1 / 64),
+    dict(B=2, H=4, K=2, nq=40, nk=3, d=32, up=2.0 ** 13, gain=8.0, scale=1 / 64, causal=True),
+    # keys whose weight is below fp16's least in every row: dV is a sum of many
+    dict(B=1, H=2, K=2, nq=2000, nk=64, d=64, up=8.0, far=17.0),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("case", range(len(SMALL_AND_LARGE)))
+def test_diff_attention_gradients_of_any_size(nn, dtype, case):
+    """Where the operands of the gradients' products would leave the range of
+    fp16, the gradients are still as near as `check` has them."""
+    a = dict(SMALL_AND_LARGE[case])
+    up, shift, gain, far = (a.pop(n, 0.0) for n in ("up", "shift", "gain", "far"))
+    c = Case(dtype=dtype, **a)
+    c.do *= up
+    c.q[..., 0] += shift
+    c.lam *= 0.25
+    if gain:
+        c.q *= gain
+    if far:
+        # half of the keys lie 17 nats behind the others: weights of about 2^-30
+        c.q[..., 1], c.k[..., 1] = 4.0, 0.0
+        c.k[:, :, ::2, 1] = -far / 4 / c.scale
+    got, ref = c.bwd(nn, *c.fwd(nn)), c.reference(backward=True)
+    for name, x in got.items():
+        # a result within its rounding, u and twice u of its terms, of the type's
+        # largest number may be infinite; there are few of them
+        y, terms = ref[name]
+        over = y.abs() + 4 * half_step(c.t) * terms > torch.finfo(c.t).max
+        assert over.sum() < 0.1 * over.numel() and ((x[over].double() - y[over]).abs() < 2 * terms[over]).logical_or(x[over] == y[over].sign() * math.inf).all()
+        x[over] = y[over] = 0
+    c.check(got, ref, max(c.k.shape[2], c.q.shape[2] * c.H // c.K))
