@@ -335,7 +335,7 @@ class AdamW:
         kinds = {"m": state_type, "v": state_type, "masters": torch.float32, "m_scales": torch.float32,
                  "v_scales": torch.float32, "grads": grads[0].dtype if n else None}
         table = (A.AdamwTensor * max(n, 1))()
-        seen = set()
+        written = []
         for i, p in enumerate(params):
             if p.dtype != params[0].dtype or p.device != self.device or not p.is_contiguous():
                 raise ValueError("AdamW: parameters share a type and device and are contiguous")
@@ -352,13 +352,15 @@ class AdamW:
                 at = x[i].data_ptr()
                 if name == "grads" or not x[i].numel() or (name == "masters" and at == p.data_ptr()):
                     continue
-                if at in seen:
-                    raise ValueError(f"AdamW: {name}[{i}] is another tensor of the step as well")
-                seen.add(at)
+                written.append((at, at + x[i].numel() * x[i].element_size(), name, i))
             if masters is not None:
                 e.master = lists["masters"][i].data_ptr()
             if bits8:
                 e.m_scale, e.v_scale = lists["m_scales"][i].data_ptr(), lists["v_scales"][i].data_ptr()
+        written.sort()
+        for (_, end, *_), (at, _, name, i) in zip(written, written[1:]):
+            if at < end:
+                raise ValueError(f"AdamW: memory of {name}[{i}] is another tensor of the step as well")
         self.lr, self.betas, self.eps, self.weight_decay = lr, (beta1, beta2), eps, weight_decay
         self.state, self._table, self._n = state, table, n
         self._kinds = (_dtype(params[0], "AdamW"), _dtype(grads[0], "AdamW")) if n else (A.F32, A.F32)

@@ -316,3 +316,12 @@ def test_adamw_takes_an_assigned_rate(monkeypatch):
         with pytest.raises(ValueError):
             opt.lr = bad
     assert opt.lr is rate
+
+
+def test_adamw_refuses_tensors_that_share_some_memory():
+    z = torch.zeros(600)
+    nn.AdamW(**adamw_args(params=[z[:300], z[300:]]))
+    for change in ({"params": [z[:300], z[299:599]]}, {"m": [z[1:301], torch.zeros(300)], "v": [z[:300], torch.zeros(300)]},
+                   {"params": [torch.zeros(300), z[:300]], "masters": [z[200:500], torch.zeros(300)]}):
+        with pytest.raises(ValueError, match="as well"):
+            nn.AdamW(**adamw_args(**change))
