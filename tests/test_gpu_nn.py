@@ -865,3 +865,83 @@ def test_diff_attention_gradients_of_any_size(nn, dtype, case):
         assert over.sum() < 0.1 * over.numel() and ((x[over].double() - y[over]).abs() < 2 * terms[over]).logical_or(x[over] == y[over].sign() * math.inf).all()
         x[over] = y[over] = 0
     c.check(got, ref, max(c.k.shape[2], c.q.shape[2] * c.H // c.K))
+
+
+SINGLE_TOKENS = [dict(B=40, H=2, K=1, nq=3, nk=5000, d=16), dict(B=3, H=4, K=1, nq=1, nk=1500, d=64, causal=True),
+                 dict(B=7, H=4, K=2, nq=1, nk=3001, d=64, causal=True, kv_lens=[3001, 64, 500, 0, 65, 1, 2900]),
+                 dict(B=1, H=16, K=1, nq=1, nk=20000, d=64), dict(B=2, H=12, K=1, nq=1, nk=4099, d=32, dv=128),
+                 dict(B=300, H=2, K=2, nq=1, nk=900, d=64)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("case", range(len(SINGLE_TOKENS)))
+def test_single_tokens_round_no_weight(nn, dtype, case):
+    """The single-token form carries a weight as two 16-bit values: what is left
+    out is u^2 of it, not u, so a box of 16 keys that went missing would show.
+    Beside it the scores' 2^-16 (as in `check`), and f32 sums: a warp's chain of
+    nk / 64 products at most, 16 terms in each, and one of all CTAs' parts."""
+    c = Case(dtype=dtype, **SINGLE_TOKENS[case])
+    assert c.H // c.K * c.q.shape[2] <= 16
+    u, nk = half_step(c.t), c.k.shape[2]
+    o, _, o2 = c.fwd(nn)
+    ref = c.reference()
+    for x, (y, terms) in ((o, ref["o"]), (o2, ref["o2"])):
+        tol = u * y.abs() + (2.0 ** -16 + u * u + 2.0 ** -23 * (nk / 64 + 16 + 296)) * terms + 1e-30
+        if dtype == "f16":
+            tol = tol + 2.0 ** -24
+        assert ((x.double() - y).abs() <= tol).all(), ((x.double() - y).abs() / tol).max()
+
+
+EVERY_KEY = [dict(B=2, H=4, K=1, nq=1, nk=3001, d=64, kv_lens=[3001, 2900]), dict(B=1, H=16, K=1, nq=1, nk=9000, d=64),
+             dict(B=300, H=2, K=2, nq=1, nk=300, d=64), dict(B=1, H=2, K=1, nq=140, nk=700, d=64, kv_lens=[641]),
+             dict(B=20, H=8, K=2, nq=200, nk=521, d=64, kv_lens=[521 - 7 * i for i in range(20)]),
+             dict(B=1, H=2, K=1, nq=40, nk=300, d=100, dv=128)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("case", range(len(EVERY_KEY)))
+def test_every_key_counts(nn, dtype, case):
+    """Each column of V is 1 at one key and 0 elsewhere, keys at the edges of boxes,
+    steps and tiles among them: a result is that key's weight alone, to the
+    rounding of that weight."""
+    c = Case(dtype=dtype, **EVERY_KEY[case])
+    nk, dv = c.k.shape[2], c.v.shape[3]
+    keys = sorted({k for e in (0, 16, 32, 48, 64, 128, 256, 512, 1024, nk) for k in (e - 1, e, e + 1) if 0 <= k < nk})
+    rest = torch.randperm(nk, generator=torch.Generator().manual_seed(1)).tolist()
+    keys += [k for k in rest if k not in keys][:dv - len(keys)]
+    c.v.zero_()
+    c.v[:, :, keys, list(range(dv))] = 1
+    o, lse, o2 = c.fwd(nn)
+    c.check({"o": o, "lse": lse, "o2": o2}, c.reference(), 64)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("d,dv", [(128, 256), (128, 8), (72, 136), (96, 192), (64, 256), (65, 129), (1, 1), (8, 8)])
+@pytest.mark.parametrize("nq", [1, 70])
+def test_head_dims_up_to_their_limits(nn, dtype, d, dv, nq):
+    c = Case(B=2, H=4, K=2, nq=nq, nk=100, d=d, dv=dv, dtype=dtype, causal=True, q_lens=[nq, min(nq, 40)], kv_lens=[100, 61])
+    o, lse, o2 = c.fwd(nn)
+    got = {"o": o, "lse": lse, "o2": o2, **c.bwd(nn, o, lse, o2)}
+    c.check(got, c.reference(backward=True), 140)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("a", [dict(B=4, H=6, K=2, nq=333, nk=333, d=48, causal=True),      # heads of a key head shared by a cluster
+                               dict(B=4, H=2, K=2, nq=150, nk=290, d=32),
+                               dict(B=10, H=16, K=4, nq=150, nk=290, d=64, causal=True),
+                               dict(B=4, H=4, K=1, nq=1, nk=300, d=64, causal=True),
+                               dict(B=4, H=2, K=1, nq=45, nk=70, d=100, causal=True)])
+def test_gradients_of_batches_that_are_not_filled(nn, dtype, a):
+    """NaN and infinities behind the lengths change no gradient, in every form of the backward."""
+    B, nq, nk = a["B"], a["nq"], a["nk"]
+    kv = [nk - (37 * i + 1) % nk for i in range(B)]
+    ql = kv if nq == nk else [max(nq - 5 * i, 0) if nq > 1 else 1 for i in range(B)]
+    make = lambda: Case(dtype=dtype, q_lens=ql, kv_lens=kv, **a)
+    c, e = make(), make()
+    for i in range(B):
+        for x, n in ((c.q, ql), (c.do, ql), (c.k, kv), (c.v, kv)):
+            x[i, :, n[i]:] = 0
+        for x, n in ((e.q, ql), (e.do, ql), (e.k, kv), (e.v, kv)):
+            x[i, :, n[i]:] = math.inf if i % 2 else math.nan
+    ga, gb = c.bwd(nn, *c.fwd(nn)), e.bwd(nn, *e.fwd(nn))
+    assert all(torch.equal(ga[n], gb[n]) for n in ga) and all(torch.isfinite(x).all() for x in ga.values())
