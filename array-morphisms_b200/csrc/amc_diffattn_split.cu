@@ -1,11 +1,11 @@
 // Differential attention of few rows over many keys (the single-token form),
 // 16-bit tensors with d <= 64 and dv <= 128, both multiples of 8.
 //
-// The bound is HBM: every key and value is read once, for all rows (query
-// heads that share the key head, times their rows) of a 16-row block.  The
-// keys of all sequences and key heads, in blocks of 64, are one line of work
-// that the CTAs, two a SM, share evenly, so sequences of different lengths
-// leave none idle; a CTA's share may end one sequence and begin another.
+// The bound is HBM: every key and value is read once, for all rows of its key
+// head (the query heads that share it times their rows, 16 at most).  The keys of
+// all sequences and key heads, in blocks of 64, are one line of work that the
+// CTAs, two a SM, share evenly, so sequences of different lengths leave none
+// idle; a CTA's share may end one sequence and begin another.
 // Within a CTA the four warps take a block's four boxes of 16 keys.  Warps do
 // not wait for each other: each has its own ring of TMA boxes (K_1, K_2 and V
 // rows of 16 keys, 8 KB), its own running maximum, sum and output, and they
@@ -39,7 +39,7 @@ constexpr int kStages = 3;           // boxes in flight per warp
 constexpr int kBox = 8192;           // 16 keys: K_1 2 KB, K_2 2 KB, V 4 KB
 constexpr int kStageBytes = kWarps * kStages * kBox;
 constexpr int kSplitSmem = kStageBytes + 512 + 1024;
-constexpr int kShareCtas = 148 * 2;  // CTAs that share the keys
+constexpr int kShareCtas = 148 * 2;  // CTAs that share the keys: two a SM of the B200, and the workspace's size
 constexpr int kMinShare = 4;         // blocks of 64 keys: 4 boxes a warp
 constexpr int kMaxBatch = 1024;      // sequences whose lengths a CTA sums up
 constexpr float kLog2e = 1.4426950408889634f;
@@ -47,15 +47,15 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ int g_diff_split_error;
 
 struct SplitArgs {
-  int group, row_blocks, shared;   // shared: the keys are shared out (else a unit a CTA)
+  int group, shared;   // shared: the keys are shared out (else a unit a CTA)
   float* part;       // [CTA][first or last unit][row][map][dv] unscaled outputs
   float2* part_ml;   // [CTA][first or last unit][row][map] maximum (log2 units) and sum
 };
 
-// A unit is one sequence, key head and block of 16 rows.  Its blocks of 64
+// A unit is one sequence and key head with its rows, 16 at most.  Its blocks of 64
 // keys stand on one line after those of the units before it.
 struct Unit {
-  int b, u, blocks;      // u: key head and row block
+  int b, g, blocks;      // sequence, key head, blocks
   int64_t first;         // its first block on the line
 };
 __device__ __forceinline__ int seq_blocks(const amc_diff_attention& p, int b) {
@@ -87,8 +87,8 @@ __device__ __forceinline__ Unit find_unit(const amc_diff_attention& p, int per_s
       r.b = b0 + l;
       r.blocks = (int)(__shfl_sync(0xffffffffu, mine, l) / per_seq);
       const int64_t start = before + __shfl_sync(0xffffffffu, upto, l) - (int64_t)r.blocks * per_seq;
-      r.u = (int)((x - start) / r.blocks);
-      r.first = start + (int64_t)r.u * r.blocks;
+      r.g = (int)((x - start) / r.blocks);
+      r.first = start + (int64_t)r.g * r.blocks;
       return r;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane >> 2, pos = lane & 3;
   uint64_t* full = (uint64_t*)(sm + kStageBytes) + warp * kStages;
   volatile int* failed = (volatile int*)(sm + kStageBytes + 256);
-  const int per_seq = p.kv_heads * a.row_blocks;
+  const int per_seq = p.kv_heads;
   int64_t at, end;   // this CTA's blocks on the line
   Unit first_unit{0, 0, 0, 0};
   if (a.shared) {
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
     }
   } else {
     first_unit.b = blockIdx.x / per_seq;
-    first_unit.u = blockIdx.x % per_seq;
+    first_unit.g = blockIdx.x % per_seq;
     first_unit.blocks = seq_blocks(p, first_unit.b);
     at = 0;
     end = first_unit.blocks;
@@ -176,8 +176,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
   int used = 0;   // boxes of this warp before this part
   do {
   const Unit unit = a.shared ? find_unit(p, per_seq, at) : first_unit;
-  const int rb = unit.u % a.row_blocks, g = unit.u / a.row_blocks, b = unit.b;
-  const int rows = min(kRows, a.group * p.nq - rb * kRows);
+  const int g = unit.g, b = unit.b, rows = a.group * p.nq;
   const DiffLens len = diff_lens(p, b);
   const int64_t stop = min(end, unit.first + unit.blocks);
   const int kbeg = (int)(at - unit.first) * 64, kend = min(len.nq > 0 ? len.nk : 0, (int)(stop - unit.first) * 64);
@@ -186,7 +185,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
   for (int r = 0; r < RR; ++r) {
     const int rr = quad + 8 * r;
     int h, i;
-    unit_row(p, a, g, rb * kRows + min(rr, rows - 1), h, i);
+    unit_row(p, a, g, min(rr, rows - 1), h, i);
     lim[r] = rr < rows ? diff_limit(len, p.causal, i) : 0;
   }
   // box n of this warp starts at key kbeg + 16 (warp + 4 n)
@@ -215,7 +214,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
         continue;
       }
       int h, i;
-      unit_row(p, a, g, rb * kRows + min(quad + 8 * r, rows - 1), h, i);
+      unit_row(p, a, g, min(quad + 8 * r, rows - 1), h, i);
       const T* src = (const T*)p.q + b * p.qs[0] + (2 * h + m) * p.qs[1] + (int64_t)i * p.qs[2];
       const bool use = quad + 8 * r < rows && i < len.nq;
 #pragma unroll
@@ -359,7 +358,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_diff_split(const __grid_constan
   __syncthreads();
   for (int row = warp; row < rows; row += kWarps) {
     int h, i;
-    unit_row(p, a, g, rb * kRows + row, h, i);
+    unit_row(p, a, g, row, h, i);
     float mx[2], l[2], acc[2][NV / 32];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -418,7 +417,7 @@ __global__ void __launch_bounds__(256) k_diff_join(const __grid_constant__ amc_d
   __shared__ float2 ml[2][kShareCtas + 1];
   __shared__ float other[256];
   const int i = blockIdx.x % p.nq, h = blockIdx.x / p.nq % p.heads, b = blockIdx.x / p.nq / p.heads;
-  const int g = h / a.group, rr = (h - g * a.group) * p.nq + i, per_seq = p.kv_heads * a.row_blocks;
+  const int g = h / a.group, rr = (h - g * a.group) * p.nq + i, per_seq = p.kv_heads;
   const int tid = threadIdx.x, m = tid >> 7, c = tid & 127;
   const int blocks = seq_blocks(p, b);
   int n = 0, c0 = 0;
@@ -436,7 +435,7 @@ __global__ void __launch_bounds__(256) k_diff_join(const __grid_constant__ amc_d
       total += __shfl_xor_sync(0xffffffffu, total, o);
     }
     share = share_of(total * per_seq);
-    first = before * per_seq + (int64_t)(g * a.row_blocks + rr / kRows) * blocks;
+    first = before * per_seq + (int64_t)g * blocks;
     c0 = (int)(first / share);
     n = (int)((first + blocks - 1) / share) - c0 + 1;
   }
@@ -447,7 +446,7 @@ __global__ void __launch_bounds__(256) k_diff_join(const __grid_constant__ amc_d
   // CTA c0 + k holds this unit as its first, but for c0 itself if its share began before
   auto slot = [&](int k) -> int64_t {
     const int second = k == 0 && first > c0 * share;
-    return (((int64_t)(c0 + k) * 2 + second) * kRows + rr % kRows) * 2 + m;
+    return (((int64_t)(c0 + k) * 2 + second) * kRows + rr) * 2 + m;
   };
   for (int k = c; k < n; k += 128) ml[m][k] = a.part_ml[slot(k)];
   __syncthreads();
@@ -481,10 +480,9 @@ namespace {
 SplitArgs plan(const amc_diff_attention& p) {
   SplitArgs a{};
   a.group = p.heads / p.kv_heads;
-  a.row_blocks = (int)(((int64_t)a.group * p.nq + kRows - 1) / kRows);
   // Units go to a CTA each where there are plenty of them, or where a cache
   // is so short that a second kernel would cost more than it shares out.
-  const int64_t units = (int64_t)p.batch * p.kv_heads * a.row_blocks;
+  const int64_t units = (int64_t)p.batch * p.kv_heads;
   a.shared = units < 2 * kShareCtas && p.batch <= kMaxBatch && p.nk > 64 * kMinShare;
   return a;
 }
@@ -495,7 +493,7 @@ template <typename T, int NV, bool PACK>
 int split_main(const amc_diff_attention& p, const SplitArgs& a, const CUtensorMap (&map)[2], cudaStream_t s) {
   static std::atomic<uint64_t> attr{0};
   if (int rc = smem_attr_once(k_diff_split<T, NV, PACK>, kSplitSmem, attr)) return rc;
-  const unsigned grid = a.shared ? kShareCtas : (unsigned)((int64_t)p.batch * p.kv_heads * a.row_blocks);
+  const unsigned grid = a.shared ? kShareCtas : (unsigned)((int64_t)p.batch * p.kv_heads);
   k_diff_split<T, NV, PACK><<<grid, kWarps * 32, kSplitSmem, s>>>(map[0], map[1], p, a);
   AMC_CUDA(cudaGetLastError());
   return AMC_OK;

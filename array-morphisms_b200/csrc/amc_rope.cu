@@ -44,10 +44,7 @@ struct Vec {
   static constexpr int bytes = V * (int)sizeof(T);
   T e[V];
   __device__ __forceinline__ void load(const T* p) {
-    if constexpr (bytes == 32) {
-      reinterpret_cast<int4*>(e)[0] = reinterpret_cast<const int4*>(p)[0];
-      reinterpret_cast<int4*>(e)[1] = reinterpret_cast<const int4*>(p)[1];
-    } else if constexpr (bytes == 16) {
+    if constexpr (bytes == 16) {
       *reinterpret_cast<int4*>(e) = *reinterpret_cast<const int4*>(p);
     } else {
 #pragma unroll
@@ -55,10 +52,7 @@ struct Vec {
     }
   }
   __device__ __forceinline__ void store(T* p) const {
-    if constexpr (bytes == 32) {
-      reinterpret_cast<int4*>(p)[0] = reinterpret_cast<const int4*>(e)[0];
-      reinterpret_cast<int4*>(p)[1] = reinterpret_cast<const int4*>(e)[1];
-    } else if constexpr (bytes == 16) {
+    if constexpr (bytes == 16) {
       *reinterpret_cast<int4*>(p) = *reinterpret_cast<const int4*>(e);
     } else {
 #pragma unroll
