@@ -16,7 +16,15 @@
 // groups' exponentials met and the pipes took turns: 3550 clocks a tile.)
 //   p = 2^(scale log2e s - m), rounded to the tensors' type for P V and
 //   summed unrounded; m follows the row maximum only when it rises by more
-//   than 2^8, and O is rescaled then, once P V of the step before is complete.
+//   than 2^8 (a rule known from published attention kernels; any bound is right
+//   that leaves 2^bound times a sum of weights in range), and O is rescaled then,
+//   once P V of the step before is complete.
+// P's rounding, half a step of the type for each weight, is the price of feeding
+// it to the tensor pipe: o is 1.5 times as far from 64 bits as from f32 products
+// rounded once (0.0025 against 0.0017 of its norm in bf16).
+// That S(j+2) may follow P(j) V into the buffer that holds P(j) without a wait rests
+// on one thread's products running in the order of their issue, which is observed;
+// the PTX document states it for products of one accumulator and shape.
 // The two rows' results meet in the epilogue: O = O_0 / l_0 - lam O_1 / l_1.
 //
 // Bound: per 128 x 128 tile of both maps the products take 1536 clocks of the
@@ -24,9 +32,10 @@
 // exponentials 2048 of the special-function unit.  Taking a part of those on
 // the FMA pipe by a polynomial gained nothing: the softmax threads' other
 // instructions then fill the time.
-// Measured: 333 rows that continue 777 keys, causal, 8 heads, 6 sequences of
-// mixed lengths, d 64: 21 us; 1000 x 1000, causal, 6 heads, 5 sequences of mixed
-// lengths, d 48: 27 us.
+// Measured: 4096 x 4096, causal, 16 heads (4 key heads), 4 sequences, d 64: 446 us
+// in a short run, 496 in a long one (412 GFLOP: 924 and 831 TFLOP/s); 333 rows that
+// continue 777 keys, causal, 8 heads, 6 sequences of mixed lengths, d 64: 21 us;
+// 1000 x 1000, causal, 6 heads, 5 sequences of mixed lengths, d 48: 27 us.
 // Every wait is bounded; on expiry the kernel records AMC_ERR_TIMEOUT and
 // leaves after its copies and products have drained.
 #include <cmath>
@@ -338,10 +347,9 @@ __global__ void __launch_bounds__(kThreadsF, 1) k_diff_fwd_tc(const __grid_const
 }
 
 // ------------------------------------------------------------------ CTA pairs
-// The kernel for more than 128 rows.  One CTA of 128 rows asks the L2 for 512
-// bytes a key (d = 64), 7.6 TB/s at 150 clocks a key: that, not the pipes,
-// bounded the kernel above.  Here two CTAs own 256 rows of one head and their
-// products are cta_group::2: each CTA stages half the keys of K (N of the
+// The kernel for many rows over few keys.  One CTA of 128 rows asks the L2 for 512
+// bytes a key (d = 64), 7.6 TB/s at 150 clocks a key.  Here two CTAs own 256 rows of
+// one head and their products are cta_group::2: each CTA stages half the keys of K (N of the
 // scores) and half the columns of V (N of P V), so the traffic per row halves,
 // and so do the products to issue.  The CTAs are persistent, one pair per two
 // SMs: the next tile's Q, K and V load, and its first scores run, while the
@@ -354,14 +362,15 @@ __global__ void __launch_bounds__(kThreadsF, 1) k_diff_fwd_tc(const __grid_const
 // before needs none of its own: the scores after next follow it on the pipe,
 // and their barrier is committed even where there is no such step.
 // What the odd CTA's shared memory holds (loaded tiles, cleared rows of V) is
-// released and acquired at cluster scope; that costs nothing measurable (507 us
-// with and without it, 16 heads x 4 sequences, 4096 x 4096, causal).
-// Measured, causal, 16 heads x 4 sequences, 4096 x 4096, d 64: 470 to 515 us with
-// the GPU's power limit (412 GFLOP: 800 to 876 TFLOP/s); 8 x 16, 2048 x 2048
-// without a mask: 440 to 490 us.  A step takes 1577 clocks, of which the tensor
-// pipe is busy 847 and the special-function unit 1024: what is left is the
-// softmax threads' other instructions and the waits for one another.  Staggering
-// the two maps by half a step, 16 softmax warps instead of 8, and a part of the
+// released and acquired at cluster scope; that costs nothing measurable (16 heads
+// x 4 sequences, 4096 x 4096, causal: the same with and without it).
+// Measured, 8 heads x 16 sequences, 2048 x 2048, d 64, no mask: 466 us in a short
+// run, 543 in a long one at the power limit (412 GFLOP: 884 and 759 TFLOP/s), of
+// which about a sixth is the turnover from tile to tile (843,727 cycles of the
+// kernel, of which the 14 tiles' 32 steps of 1577 are 706,496).  Within a step the
+// tensor pipe is busy for 847 clocks and the special-function unit for 1024, and
+// issue slots are 38 % taken: the rest are waits for one another.  Staggering the
+// two maps by half a step, 16 softmax warps instead of 8, and a part of the
 // exponentials on the FMA pipe each made it slower or gained nothing.
 namespace {
 
@@ -791,12 +800,17 @@ int diff_fwd_tc(const amc_diff_attention& p, cudaStream_t s, bool* handled) {
   if (!diff_tc_shape(p) || !(p.scale > 0.f) || !aligned_rows(p.o, p.os, p) || (p.o2 && !aligned_rows(p.o2, p.o2s, p))) return AMC_OK;
   if ((int64_t)((p.nq + 127) / 128) * p.heads * p.batch > 0x7fffffff) return AMC_OK;
   CUtensorMap map[3];
-  // Pairs take 256-row tiles, two SMs each, and gain over many rounds of tiles:
-  // with few, 128-row CTAs fill the GPU better (96 tiles of 333-row sequences:
-  // 22 us against 46, 120 of 1000 rows: 27 against 39, 128 of 2048: 75 against
-  // 76; 1024 of 2048: 550 against 440).
+  // Pairs halve what a row asks of the L2 and with it the power that limits long
+  // runs, and load a tile behind the one before; but their step takes longer, a
+  // causal mask leaves them uneven rounds, and a half-empty last tile costs two SMs.
+  // In loops of calls, d 64, us on single CTAs against pairs: no mask, 1024 tiles
+  // of 256 rows over 2048 keys 597 : 543, over 512 keys 207 : 181, 512 tiles over
+  // 1024 150 : 144, 160 over 512 63 : 62; on the other side over 4096 keys 451 : 468,
+  // over 16384 1495 : 1846, 777 rows and keys 174 : 187, causal 4096 x 4096 446 : 538,
+  // 2048 x 2048 335 : 335, 777 x 777 129 : 154, and 80 to 128 tiles 65 : 72 and 68 : 73.
   const int64_t tiles = (int64_t)((p.nq + 255) / 256) * p.heads * p.batch;
-  const bool bf16 = p.dtype == AMC_BF16, pair = p.nq > 128 && tiles >= 2 * (num_sms() / 2);
+  const bool bf16 = p.dtype == AMC_BF16;
+  const bool pair = !p.causal && p.nk <= 2048 && (p.nq - 1) % 256 >= 128 && tiles >= 2 * (num_sms() / 2);
   int rc = make_tmap_4d_16(&map[0], p.q, bf16, p.batch, 2 * p.heads, p.nq, p.d, p.qs, 128);
   if (!rc) rc = make_tmap_4d_16(&map[1], p.k, bf16, p.batch, 2 * p.kv_heads, p.nk, p.d, p.ks, pair ? 32 : 128);
   if (!rc) rc = make_tmap_4d_16(&map[2], p.v, bf16, p.batch, p.kv_heads, p.nk, p.dv, p.vs, 128);

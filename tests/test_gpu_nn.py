@@ -683,12 +683,13 @@ def test_a_layer_trains(nn):
 
 @pytest.mark.parametrize("dtype,d", [("bf16", 64), ("f16", 64), ("bf16", 32)])
 @pytest.mark.parametrize("causal", [False, True])
-def test_pairs_of_ctas_see_the_values_that_either_cleared(nn, dtype, d, causal):
+@pytest.mark.parametrize("nq", [300, 400])      # 400 without a mask: pairs of CTAs
+def test_pairs_of_ctas_see_the_values_that_either_cleared(nn, dtype, d, causal, nq):
     """Both CTAs of a pair clear their columns of V behind the length, and one of
     them issues the products that read both: over lengths on every side of a
     step of 64 keys, and many launches, NaN there never reaches a result."""
     lens = [521, 520, 513, 512, 449, 447, 385, 383, 65, 1]
-    make = lambda: Case(B=10, H=16, K=4, nq=300, nk=521, d=d, dtype=dtype, causal=causal, kv_lens=lens)
+    make = lambda: Case(B=10, H=16, K=4, nq=nq, nk=521, d=d, dtype=dtype, causal=causal, kv_lens=lens)
     c, e = make(), make()
     for i, n in enumerate(lens):
         c.k[i, :, n:], c.v[i, :, n:] = 0, 0
@@ -945,3 +946,37 @@ def test_gradients_of_batches_that_are_not_filled(nn, dtype, a):
             x[i, :, n[i]:] = math.inf if i % 2 else math.nan
     ga, gb = c.bwd(nn, *c.fwd(nn)), e.bwd(nn, *e.fwd(nn))
     assert all(torch.equal(ga[n], gb[n]) for n in ga) and all(torch.isfinite(x).all() for x in ga.values())
+
+
+PAIRS = [dict(B=10, H=16, K=4, nq=400, nk=257, d=64, q_lens=[400, 0, 1, 129, 128, 127, 257, 400, 256, 2],
+              kv_lens=[257, 257, 0, 5, 256, 255, 129, 64, 65, 200]),
+         dict(B=5, H=16, K=16, nq=512, nk=300, d=32, kv_lens=[300, 0, 299, 128, 1]),
+         dict(B=3, H=25, K=5, nq=390, nk=700, d=48),
+         dict(B=19, H=8, K=8, nq=256, nk=1, d=64),
+         dict(B=2, H=40, K=8, nq=1024, nk=2048, d=64, q_lens=[1024, 900], kv_lens=[2048, 1985])]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("case", range(len(PAIRS)))
+def test_many_rows_over_few_keys(nn, dtype, case):
+    """The form of the forward on pairs of CTAs, several tiles a pair: its results,
+    their repetition, in a graph too, and rows that hold NaN."""
+    c = Case(dtype=dtype, **PAIRS[case])
+    got = c.fwd(nn)
+    c.check(dict(zip(("o", "lse", "o2"), got)), c.reference(), c.k.shape[2])
+    again = [torch.empty_like(x) for x in got]
+    ws = torch.empty(nn.diff_attention_workspace(c.q, c.k, c.v), dtype=torch.uint8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        nn.diff_attention_fwd(c.q, c.k, c.v, c.lam, again[0], again[1], LAM_INIT, c.scale, q_lens=c.q_lens,
+                              kv_lens=c.kv_lens, o2=again[2], workspace=ws)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, again))
+    c.q[0, 3, 140, 5] = math.nan
+    o, lse, o2 = c.fwd(nn)
+    assert lse[0, 3, 140].isnan() and lse.isnan().sum() == 1 and o[0, 1, 140].isnan().all()
+    assert all(torch.equal(x[~y.isnan()], y[~y.isnan()]) for x, y in zip(got, (o, lse, o2)))
+    from amcuda import _abi
+    _abi.call("amc_synchronize")      # no wait of the kernels gave up
