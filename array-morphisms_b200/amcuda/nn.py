@@ -5,8 +5,11 @@ gradient, and the single-token form) and the AdamW step.
 Tensors are (batch, heads, rows, dim) with unit stride along dim and any
 strides over the other axes, so a projection's (batch, rows, heads, dim)
 output is passed as its transpose(1, 2).  Types are float32, bfloat16 and
-float16; arithmetic is f32 or wider.  Results go into tensors the caller
-gives; nothing is allocated.  Calls run on `stream` (the current stream of the
+float16; arithmetic is f32 or wider, but for the weights (and the gradients'
+operands made of them) that the attention of 16-bit tensors with d up to 64 and
+dv up to 128 rounds once to their type for the tensor cores; its single-token
+form rounds none.  Results go into tensors the caller gives; nothing is
+allocated, and torch's autograd does not see the calls.  Calls run on `stream` (the current stream of the
 tensors' device when None) and may be captured into CUDA graphs.
 
     freqs, mscale = rope_freqs(64, factor=8.0, kind="parts", original_len=4096)
@@ -272,7 +275,9 @@ def diff_attention_fwd(q, k, v, lam, o, lse, lam_init: float, scale: float, caus
     What the tensors hold behind the lengths is not used.  lse (B, 2H, nq)
     float32 (or None) receives the row log-sum-exps; o2 (like o) the second
     map's part, which the backward needs.  One query row (or few) a head runs
-    the single-token form, split over the keys."""
+    the single-token form, split over the keys.  A cache that fills up is best
+    given whole with its kv_lens: each new shape of a slice of it is checked anew
+    on the host, which costs more than a short call's kernel."""
     _diff_call("diff_attention_fwd", q, k, v, lam, o, lse, o2, q_lens, kv_lens, workspace, None, causal, scale,
                lam_init, stream)
 
@@ -281,7 +286,7 @@ def diff_attention_bwd(q, k, v, lam, o, o2, lse, do, dq, dk, dv, dlam, lam_init:
                        causal: bool = False, q_lens=None, kv_lens=None, workspace=None, stream=None) -> None:
     """Gradients of diff_attention_fwd for upstream `do` (like o), from its o,
     o2 and lse: dq, dk, dv and dlam, shaped like their tensors, gradients of
-    shared heads summed, zero behind the lengths.  No atomics: repeated calls
+    shared heads summed, zero behind the lengths.  No sums by atomics: repeated calls
     give identical bits."""
     _diff_call("diff_attention_bwd", q, k, v, lam, o, lse, o2, q_lens, kv_lens, workspace, (do, dq, dk, dv, dlam),
                causal, scale, lam_init, stream)

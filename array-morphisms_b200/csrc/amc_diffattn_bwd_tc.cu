@@ -17,7 +17,9 @@
 //                  and sums P_2 G (dlam) in f32 on the way; the last CTA of a
 //                  row of lam adds its partial sums up, in their order.
 // The operands that the threads make (the difference of the maps, dS_1, dS_2)
-// are rounded to the tensors' type and stay in tensor memory, written over
+// are rounded to the tensors' type (half a step each, which makes the gradients
+// 1.5 times as far from 64 bits as f32 products rounded once; fp16 ones times
+// powers of two, see amc_diffattn.h) and stay in tensor memory, written over
 // the scores they came from; a thread writes only columns it has read.  A
 // 16-bit tile in the 128-byte swizzle serves K-major (its rows as N) and
 // MN-major (its rows as K) alike, so one copy of Q, K and dO feeds both
@@ -155,7 +157,9 @@ __global__ void __launch_bounds__(256) k_diff_peaks(const __grid_constant__ amc_
 // G after the exponentials.  (With both scores issued when G had been read, the
 // warps waited 450 to 900 clocks a tile for them: 2800 a tile, now 2300.)  One thread
 // issues everything, so a buffer that an earlier product reads may be the target
-// of a later one.
+// of a later one: products run in the order of their issue.  That is what is
+// observed, and common in such kernels; the PTX document states it for products
+// of one accumulator and shape, which these are not.
 template <typename T, int NV>
 __device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap& mK, const CUtensorMap& mV,
                                         const CUtensorMap& mG, const amc_diff_attention& p, const DiffBwdWork& wk,
@@ -497,8 +501,8 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap& mQ, const CUtensorMap
 // ------------------------------------------------------------------ dQ, dlam
 // Tensor memory: two buffers of S_1, S_2, G (64 columns each) at 0 and 192,
 // dQ_1, dQ_2 at 384 and 448.  Tile j+2 is computed into the buffer of tile j
-// right after the products that read dS(j) from it, while the threads work on
-// tile j+1.
+// right after the products that read dS(j) from it (in the order of issue, as
+// above), while the threads work on tile j+1.
 template <typename T, int NV>
 __device__ __forceinline__ void dq_cta(const CUtensorMap& mQ, const CUtensorMap& mK, const CUtensorMap& mV,
                                        const CUtensorMap& mG, const amc_diff_attention& p, const DiffBwdWork& wk,

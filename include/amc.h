@@ -373,9 +373,15 @@ int amc_conv2d_wgrad_f32(const float* X, const float* dY, float* dW, int32_t N, 
  * reference (its attention is one unmasked map, realization.scm:279-396, and
  * its optimizer the plain step of example 9).  Tensors are (batch, heads,
  * rows, dim) with any element strides over the first three axes and unit
- * stride along dim; dtype is AMC_F32, AMC_BF16 or AMC_F16.  All arithmetic
- * between loads and stores is f32 or wider.  Nothing is allocated: scratch is
- * the caller's `workspace`, which two calls that may overlap must not share. */
+ * stride along dim; dtype is AMC_F32, AMC_BF16 or AMC_F16.  Arithmetic between
+ * loads and stores is f32 or wider, but for the operands that the attention of
+ * 16-bit tensors with d up to 64 and dv up to 128 makes for the tensor cores:
+ * the weights before their product with V, and in the gradients P_1 - lam P_2
+ * and the scores' gradients, are rounded to `dtype` once, half a step of each
+ * (fp16: times powers of two that keep the gradients' operands in its range).
+ * Calls with 16 rows or fewer for a key head round no weight.  Nothing is
+ * allocated: scratch is the caller's `workspace`, which two calls that may
+ * overlap must not share. */
 #define AMC_BF16 16
 #define AMC_F16  17
 #define AMC_E4M3 18   /* 8-bit optimizer states only */
@@ -425,7 +431,8 @@ int amc_rope_freqs(double* host_out, int32_t rot, double base, int32_t kind, dou
  * last key.  Rows from q_lens[b] on, and rows that see no key, give 0 (lse
  * -inf) and no gradient.  Elements of q, k, v and d_o behind q_lens and
  * kv_lens are not used, whatever they hold; within the lengths a NaN or an
- * infinity spreads as products spread it, masked or not.  Results must not
+ * infinity spreads as products spread it, masked or not, and the lse of a row
+ * with a NaN among its scores is NaN.  Results must not
  * overlap one another or what is read.
  * lse (batch, 2 heads, nq, contiguous) receives the natural-log row
  * log-sum-exp of each map, o2 (optional; the backward needs it) the second
@@ -433,7 +440,7 @@ int amc_rope_freqs(double* host_out, int32_t rot, double base, int32_t kind, dou
  * (one lam for all heads) or heads.  d 1..128, dv 1..256.
  * The backward reads o, o2 and lse of the forward and writes dq, dk, dv
  * (gradients of shared heads summed) and dlam, the gradients of all 4 rows.
- * No atomics: repeated calls give identical bits. */
+ * No sums by atomics: repeated calls give identical bits. */
 typedef struct amc_diff_attention {
   int32_t dtype, causal;
   int32_t batch, heads, kv_heads, nq, nk, d, dv, lam_rows;
